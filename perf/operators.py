@@ -1,0 +1,492 @@
+"""What is measured of the graph encoder's training block: attention over sampled neighbour lists (forward and backward), the normalised and gated
+residual between two blocks (forward and backward), and the AdamW step over all parameter tensors (states in 32 or in 8 bits).
+
+Every case is a dict of plain values; `prepare` makes its inputs on the GPU from a seed, `run` is one pass: the plain form in elementary torch
+operations where `own` is false, the framework's entry points where it is true. `exact` is the same from the definition in 64 bits."""
+import math
+import random
+
+import torch
+
+own = False
+
+TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+BYTES = {"fp32": 4, "bf16": 2, "fp16": 2}
+BLOCK = 256          # elements of an 8-bit state that share one scale
+ALIGN = 256          # elements: where a tensor starts in the flat buffers of the AdamW cases
+LR, BETA1, BETA2, EPS, DECAY = 1e-3, 0.9, 0.999, 1e-8, 1e-2
+NORM_EPS = 1e-6
+
+
+# ---------------------------------------------------------------------------------------------------------------- cases
+def _attention(name, way, n, rows, edges, heads, kv_heads, dim, kind, hubs=1.0, bias=False):
+    return {"name": name, "op": "attention", "way": way, "n": n, "rows": rows, "edges": edges, "heads": heads, "kv_heads": kv_heads, "dim": dim, "type": kind,
+            "hubs": hubs, "bias": bias}
+
+
+def _norm(name, way, n, d, stream, kind, norm, post, pre, gate, act, affine_bias, scale):
+    return {"name": name, "op": "norm", "way": way, "n": n, "d": d, "stream": stream, "type": kind, "norm": norm, "post": post, "pre": pre, "gate": gate, "act": act,
+            "affine_bias": affine_bias, "scale": scale}
+
+
+def _adamw(name, tensors, total, bits, kind, grad, clipped, layout):
+    return {"name": name, "op": "adamw", "tensors": tensors, "total": total, "bits": bits, "type": kind, "grad": grad, "clipped": clipped, "layout": layout}
+
+
+def listed():
+    return [
+        # one request of 64 target nodes with 15 sampled neighbours each, answered by a served encoder: the smallest call, latency counts
+        _attention("attention fwd 64 nodes", "forward", 64, 1024, 960, 4, 4, 32, "fp32", 0.0),
+        # a batch of 16,384 nodes evaluated with all their neighbours (degrees as they come, a few without any), wide heads that share keys
+        _attention("attention fwd bf16 shared", "forward", 16384, 120000, 250000, 8, 2, 64, "bf16", 1.0),
+        # first layer of a sampled mini-batch: 1000 seeds, fan-outs 15-10-5 over a 128-wide table: 150,000 targets, 800,000 rows
+        _attention("attention train fan-out", "train", 150000, 800000, 900000, 4, 4, 32, "fp32", 0.0),
+        # a power-law graph with all neighbours: hubs with tens of thousands of entries, relation biases that mask some of the edges
+        _attention("attention train hubs bf16", "train", 100000, 100000, 1500000, 8, 4, 64, "bf16", 3.0, True),
+        # embedding width 100 in four heads of 25: nothing is a multiple of a vector load
+        _attention("attention train odd fp16", "train", 20011, 30011, 200003, 4, 4, 25, "fp16", 1.5, True),
+        # the norm in front of a block for one request: rows of a 128-wide encoder
+        _norm("norm fwd 64 rows", "forward", 64, 128, "fp32", "fp32", "RMS", False, True, "none", "NONE", False, 1.0),
+        # residual stream in 32 bits, blocks in bfloat16, norms on both sides and a gate for each channel: the forward of a wide encoder
+        _norm("norm fwd fp32 + bf16", "forward", 100000, 512, "fp32", "bf16", "RMS", True, True, "channel", "NONE", False, 0.8),
+        # the embedding width of the link-prediction configuration, one batch of its unique rows, LayerNorm with bias
+        _norm("norm bwd d=100", "backward", 160000, 100, "fp32", "fp32", "LAYER", False, True, "channel", "NONE", True, 1.0),
+        # bfloat16 throughout, a learned sigmoid gate for every element, norms on both sides
+        _norm("norm bwd bf16 gated", "backward", 50000, 1024, "bf16", "bf16", "RMS", True, True, "element", "SIGMOID", False, 1.0),
+        # the parameters of a three-layer encoder and its relation tables: a few small tensors, the launch is what costs
+        _adamw("adamw encoder", 16, 160000, 32, "fp32", "fp32", False, 1),
+        # many ragged tensors, clipped, parameters and gradients in bfloat16, states in 8 bits
+        _adamw("adamw ragged 8-bit", 300, 20000000, 8, "bf16", "bf16", True, 2),
+        # a trained feature table with its encoder: 200 M parameters in 32 bits
+        _adamw("adamw table", 6, 200000000, 32, "fp32", "fp32", True, 3),
+    ]
+
+
+def _log(rng, lo, hi):
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    """one more case of the same ranges; the largest sizes are those of the listed cases"""
+    op = rng.choice(["attention", "norm", "adamw"])
+    if op == "attention":
+        heads = rng.choice([1, 2, 3, 4, 6, 8, 12, 16])
+        kv_heads = rng.choice([h for h in range(1, heads + 1) if heads % h == 0])
+        dim = rng.choice([16, 25, 32, 33, 50, 64, 80, 96, 100, 128])
+        most = 100000 * 8 * 64 // (heads * dim)                      # rows of this width that the largest listed case has
+        edges = _log(rng, 16, min(1500000, 15 * most))
+        least = 1 + edges // 8192                                    # lists of a few thousand entries, as the hubs of the listed cases have them
+        n = _log(rng, least, max(least, min(150000, most, edges // 2)))
+        c = _attention("", rng.choice(["forward", "train"]), n, _log(rng, max(4, least), max(4, least, min(800000, most))), edges, heads, kv_heads, dim, rng.choice(["fp32", "bf16", "fp16"]),
+                       rng.choice([0.0, 1.0, 1.5, 3.0]), rng.random() < 0.4)
+    elif op == "norm":
+        d = _log(rng, 8, 4096)
+        n = _log(rng, 1, max(1, min(160000, 50000 * 1024 // d)))
+        stream, kind = rng.choice([("fp32", "fp32"), ("fp32", "bf16"), ("fp32", "fp16"), ("bf16", "bf16"), ("fp16", "fp16")])
+        gate = rng.choice(["none", "channel", "element"])
+        post, pre = rng.choice([(False, True), (True, False), (True, True)])
+        c = _norm("", rng.choice(["forward", "backward"]), n, d, stream, kind, rng.choice(["RMS", "LAYER"]), post, pre, gate,
+                  rng.choice(["NONE", "SIGMOID", "RELU"]) if gate != "none" else "NONE", rng.random() < 0.5, rng.choice([1.0, 0.8, 2.0]))
+    else:
+        bits = rng.choice([8, 32])
+        total = _log(rng, 64, 200000000 if bits == 32 else 100000000)
+        c = _adamw("", min(total // 8, _log(rng, 1, 300)), total, bits, rng.choice(["fp32", "bf16", "fp16"]), rng.choice(["fp32", "bf16", "fp16"]),
+                   rng.random() < 0.5, rng.randrange(1 << 20))
+    del c["name"]
+    return c
+
+
+# ---------------------------------------------------------------------------------------------------------------- attention over neighbour lists
+def _prepare_attention(c, g, dev):
+    n, rows, E, H, K, D, t = c["n"], c["rows"], c["edges"], c["heads"], c["kv_heads"], c["dim"], TYPES[c["type"]]
+    if c["hubs"] == 0.0:    # a fixed fan-out, as a uniform sampler leaves it
+        owner = torch.arange(E, device=dev) * n // E
+    else:                   # degrees as they come: u^hubs gives the first nodes the long lists
+        owner = (torch.rand(E, device=dev, generator=g, dtype=torch.float64).pow(c["hubs"]) * n).long().clamp_(max=n - 1).sort()[0]
+    index = (torch.rand(E, device=dev, generator=g, dtype=torch.float64).pow(max(c["hubs"], 1.0)) * rows).long().clamp_(max=rows - 1)
+    index = torch.randperm(rows, device=dev, generator=g)[index]
+    offsets = torch.searchsorted(owner, torch.arange(n, device=dev))   # [n] first entry of every target's list, as the sampler's graphs have them
+    s = {"c": c, "index": index, "offsets": offsets, "plan": None, "bias": None,
+         "q": torch.randn(n, H, D, device=dev, generator=g).to(t), "k": torch.randn(rows, K, D, device=dev, generator=g).to(t),
+         "v": torch.randn(rows, K, D, device=dev, generator=g).to(t)}
+    if c["bias"]:           # a bias for each relation and head; the last of eight relations is masked out
+        table = torch.randn(8, H, device=dev, generator=g)
+        table[7] = -math.inf
+        s["bias"] = table[torch.randint(8, (E,), device=dev, generator=g)].contiguous()
+    if c["way"] == "train":
+        s["grad"] = torch.randn(n, H, D, device=dev, generator=g).to(t)
+    if own:                 # what a program keeps beside its graph: the lists in both directions, made once for a batch or for a whole graph
+        from marius_amd import hip
+
+        s["plan"] = hip.NeighborPlan(index, offsets, rows)
+    return s
+
+
+def _run_attention_own(s):
+    from marius_amd import hip
+
+    out, lse = hip.neighbor_attention(s["q"], s["k"], s["v"], s["plan"], bias=s["bias"])
+    if s["c"]["way"] == "forward":
+        return {"out": out, "lse": lse}
+    dq, dk, dv, dbias = hip.neighbor_attention_backward(s["grad"], s["q"], s["k"], s["v"], lse, s["plan"], bias=s["bias"])
+    return {"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv, "dbias": dbias}
+
+
+def _run_attention_plain(s):
+    c, index = s["c"], s["index"]
+    n, E, H, K, D, t = c["n"], c["edges"], c["heads"], c["kv_heads"], c["dim"], TYPES[c["type"]]
+    dev, R, scale = index.device, c["heads"] // c["kv_heads"], 1.0 / math.sqrt(c["dim"])
+    q, k, v = s["q"].float().view(n, K, R, D), s["k"].float().unsqueeze(2), s["v"].float().unsqueeze(2)
+    ends = torch.cat([s["offsets"][1:], torch.full((1,), E, device=dev)])
+    owner = torch.repeat_interleave(torch.arange(n, device=dev), ends - s["offsets"], output_size=E)
+    score = (q[owner] * k[index]).sum(-1) * scale
+    if s["bias"] is not None:
+        score = score + s["bias"].view(E, K, R)
+    top = torch.full((n, K, R), -math.inf, device=dev).scatter_reduce_(0, owner.view(E, 1, 1).expand(E, K, R), score, "amax")
+    p = torch.exp(score - torch.where(top == -math.inf, 0.0, top)[owner])
+    total = torch.zeros(n, K, R, device=dev).index_add_(0, owner, p)
+    safe = torch.where(total > 0, total, 1.0)
+    out = torch.zeros(n, K, R, D, device=dev).index_add_(0, owner, p.unsqueeze(-1) * v[index]) / safe.unsqueeze(-1)
+    lse = (top + torch.log(safe)).view(n, H)
+    if c["way"] == "forward":
+        return {"out": out.view(n, H, D).to(t), "lse": lse}
+    g = s["grad"].float().view(n, K, R, D)
+    p = p / safe[owner]
+    dp = (g[owner] * v[index]).sum(-1)
+    ds = p * (dp - (g * out).sum(-1)[owner])
+    dq = torch.zeros(n, K, R, D, device=dev).index_add_(0, owner, ds.unsqueeze(-1) * k[index]) * scale
+    dk = torch.zeros(c["rows"], K, D, device=dev).index_add_(0, index, (ds.unsqueeze(-1) * q[owner]).sum(2)) * scale
+    dv = torch.zeros(c["rows"], K, D, device=dev).index_add_(0, index, (p.unsqueeze(-1) * g[owner]).sum(2))
+    return {"out": out.view(n, H, D).to(t), "lse": lse, "dq": dq.view(n, H, D).to(t), "dk": dk.to(t), "dv": dv.to(t), "dbias": ds.view(E, H) if c["bias"] else None}
+
+
+def _exact_attention(s):
+    """softmax over each target's list by definition, head after head; the gradients by differentiating it"""
+    c = s["c"]
+    n, E, H, D, R = c["n"], c["edges"], c["heads"], c["dim"], c["heads"] // c["kv_heads"]
+    q, k, v = (s[x].double().requires_grad_(True) for x in ("q", "k", "v"))
+    bias = None if s["bias"] is None else s["bias"].double().requires_grad_(True)
+    owner = torch.searchsorted(s["offsets"], torch.arange(E, device=q.device), right=True) - 1
+    outs, lses = [], []
+    for h in range(H):
+        score = torch.einsum("ed,ed->e", q[:, h].index_select(0, owner), k[:, h // R].index_select(0, s["index"])) / math.sqrt(D)
+        if bias is not None:
+            score = score + bias[:, h]
+        shift = score.detach().clone()
+        shift[shift == -math.inf] = -1e300
+        top = torch.full((n,), -1e300, dtype=torch.float64, device=q.device).index_reduce_(0, owner, shift, "amax")
+        dead = top == -1e300
+        w = torch.exp(score - torch.where(dead, 0.0, top).index_select(0, owner))
+        total = torch.zeros(n, dtype=torch.float64, device=q.device).index_add(0, owner, w)
+        num = torch.zeros(n, D, dtype=torch.float64, device=q.device).index_add(0, owner, w.unsqueeze(1) * v[:, h // R].index_select(0, s["index"]))
+        outs.append(num / torch.where(dead, 1.0, total).unsqueeze(1))
+        lses.append(torch.where(dead, -math.inf, top + torch.log(torch.where(dead, 1.0, total.detach()))))
+    out, lse = torch.stack(outs, 1), torch.stack(lses, 1)
+    if c["way"] == "forward":
+        return {"out": out.detach(), "lse": lse}
+    out.backward(s["grad"].double())
+    return {"out": out.detach(), "lse": lse, "dq": q.grad, "dk": k.grad, "dv": v.grad, "dbias": None if bias is None else bias.grad}
+
+
+def _work_attention(c):
+    n, E, H, K, D, b = c["n"], c["edges"], c["heads"], c["kv_heads"], c["dim"], BYTES[c["type"]]
+    read = c["rows"] * (1.0 - math.exp(-E / c["rows"]))          # rows that any list names
+    lists = 4 * E + 4 * n + (4 * E * H if c["bias"] else 0)
+    forward = {"bytes": b * (2 * n * H * D + 2 * read * K * D) + 4 * n * H + lists, "flops": 4.0 * E * H * D}
+    if c["way"] == "forward":
+        return forward
+    # the backward pass reads q, k, v, the gradient and the statistics, recomputes the scores and writes dq, dk, dv (and the bias' gradient)
+    backward = {"bytes": b * (3 * n * H * D + 2 * read * K * D + 2 * c["rows"] * K * D) + 4 * n * H + lists + (4 * E * H if c["bias"] else 0), "flops": 10.0 * E * H * D}
+    return {x: forward[x] + backward[x] for x in forward}
+
+
+# ---------------------------------------------------------------------------------------------------------------- norms around the residual
+def _prepare_norm(c, g, dev):
+    n, d, S, T = c["n"], c["d"], TYPES[c["stream"]], TYPES[c["type"]]
+    s = {"c": c, "gate": None, "x": None, "grad_h": None}
+    s["stream"] = (torch.randn(n, d, device=dev, generator=g) * 2 + 0.3).to(S)   # x of the forward pass, the stored y of the backward one
+    s["block"] = torch.randn(n, d, device=dev, generator=g).to(T)
+    if c["gate"] == "channel":
+        s["gate"] = torch.randn(d, device=dev, generator=g) * 0.5 + 0.5
+    elif c["gate"] == "element":
+        s["gate"] = torch.randn(n, d, device=dev, generator=g).to(T)
+    for side in ("post", "pre"):
+        s[side + "_weight"] = 1 + 0.1 * torch.randn(d, device=dev, generator=g) if c[side] else None
+        s[side + "_bias"] = 0.1 * torch.randn(d, device=dev, generator=g) if c[side] and c["affine_bias"] else None
+    if c["way"] == "backward":
+        s["grad_y"] = torch.randn(n, d, device=dev, generator=g).to(S)
+        s["grad_h"] = torch.randn(n, d, device=dev, generator=g).to(T) if c["pre"] else None
+    return s
+
+
+def _run_norm_own(s):
+    from marius_amd import hip
+
+    c = s["c"]
+    how = dict(post_norm=c["post"], pre_norm=c["pre"], kind=c["norm"], eps=NORM_EPS, residual_scale=c["scale"], gate_activation=c["act"])
+    args = {x: s[x] for x in ("gate", "post_weight", "post_bias", "pre_weight", "pre_bias")}
+    if c["way"] == "forward":
+        y, h = hip.residual_norm(s["stream"], s["block"], **args, **how)
+        return {"y": y, "h": h}
+    return dict(hip.residual_norm_backward(s["grad_y"], s["grad_h"], s["stream"], s["block"], **args, **how))
+
+
+def _normalised(x, c):
+    """(normalised rows, 1 / their root mean square deviation)"""
+    if c["norm"] == "LAYER":
+        x = x - x.mean(1, keepdim=True)
+    r = 1.0 / torch.sqrt((x * x).mean(1, keepdim=True) + NORM_EPS)
+    return x * r, r
+
+
+def _norm_gradient(a, xhat, r, c):
+    """the gradient of _normalised's input from the gradient `a` of its output"""
+    a = a - xhat * (a * xhat).mean(1, keepdim=True) if c["norm"] == "RMS" else a - a.mean(1, keepdim=True) - xhat * (a * xhat).mean(1, keepdim=True)
+    return a * r
+
+
+def _act(g, c):
+    return torch.sigmoid(g) if c["act"] == "SIGMOID" else torch.clamp(g, min=0) if c["act"] == "RELU" else g
+
+
+def _run_norm_plain(s):
+    c, S, T = s["c"], TYPES[s["c"]["stream"]], TYPES[s["c"]["type"]]
+    z = s["block"].float()
+    gate = None if s["gate"] is None else s["gate"].float()
+    if c["post"]:
+        zhat, rz = _normalised(z, c)
+        u = zhat * s["post_weight"]
+        u = u + s["post_bias"] if s["post_bias"] is not None else u
+    else:
+        u = z
+    open_ = 1.0 if gate is None else _act(gate, c)
+    if c["way"] == "forward":
+        y, h = c["scale"] * s["stream"].float() + open_ * u, None
+        if c["pre"]:
+            h = _normalised(y, c)[0] * s["pre_weight"]
+            h = (h + s["pre_bias"] if s["pre_bias"] is not None else h).to(T)
+        return {"y": y.to(S), "h": h}
+    dy, got = s["grad_y"].float(), {}
+    if c["pre"]:
+        yhat, ry = _normalised(s["stream"].float(), c)
+        dh = s["grad_h"].float()
+        dy = dy + _norm_gradient(dh * s["pre_weight"], yhat, ry, c)
+        got["dpre_weight"] = (dh * yhat).sum(0)
+        got["dpre_bias"] = dh.sum(0) if s["pre_bias"] is not None else None
+    got["dx"] = (c["scale"] * dy).to(S)
+    du = dy * open_
+    if gate is not None:
+        slope = open_ * (1 - open_) if c["act"] == "SIGMOID" else (gate > 0).float() if c["act"] == "RELU" else 1.0
+        got["dgate"] = (dy * u).sum(0) * slope if c["gate"] == "channel" else (dy * u * slope).to(T)
+    if c["post"]:
+        got["dpost_weight"] = (du * zhat).sum(0)
+        got["dpost_bias"] = du.sum(0) if s["post_bias"] is not None else None
+        du = _norm_gradient(du * s["post_weight"], zhat, rz, c)
+    got["dblock"] = du.to(T)
+    return got
+
+
+def _exact_norm(s):
+    c = s["c"]
+    d = {x: None if s[x] is None else s[x].double() for x in ("stream", "block", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias")}
+
+    def norm(x, side):
+        mu = x.mean(1, keepdim=True) if c["norm"] == "LAYER" else 0.0
+        var = ((x - mu) ** 2).sum(1, keepdim=True) / c["d"]
+        out = (x - mu) * (var + NORM_EPS).rsqrt() * d[side + "_weight"]
+        return out if d[side + "_bias"] is None else out + d[side + "_bias"]
+
+    def branch():
+        u = norm(d["block"], "post") if c["post"] else d["block"]
+        if d["gate"] is None:
+            return u
+        return u * {"NONE": lambda t: t, "SIGMOID": torch.sigmoid, "RELU": torch.relu}[c["act"]](d["gate"])
+
+    if c["way"] == "forward":
+        y = d["stream"] * c["scale"] + branch()
+        return {"y": y, "h": norm(y, "pre") if c["pre"] else None}
+    for t in d.values():
+        if t is not None:
+            t.requires_grad_(True)
+    dy = s["grad_y"].double()
+    if c["pre"]:          # the norm at the stored stream, then what goes back through the residual
+        norm(d["stream"], "pre").backward(s["grad_h"].double())
+        dy = dy + d["stream"].grad
+    branch().backward(dy)
+    got = {"dx": c["scale"] * dy, "dblock": d["block"].grad}
+    for out, x in (("dgate", "gate"), ("dpost_weight", "post_weight"), ("dpost_bias", "post_bias"), ("dpre_weight", "pre_weight"), ("dpre_bias", "pre_bias")):
+        if d[x] is not None:
+            got[out] = d[x].grad
+    return got
+
+
+def _work_norm(c):
+    e, S, T = c["n"] * c["d"], BYTES[c["stream"]], BYTES[c["type"]]
+    gate = e * T if c["gate"] == "element" else 0
+    if c["way"] == "forward":    # x and the block in, y and h out
+        return {"bytes": e * (2 * S + T + (T if c["pre"] else 0)) + gate, "flops": 10.0 * e}
+    reads_block = c["post"] or c["gate"] != "none"
+    return {"bytes": e * (2 * S + T + (T if reads_block else 0) + (S + T if c["pre"] else 0)) + 2 * gate, "flops": 25.0 * e}
+
+
+# ---------------------------------------------------------------------------------------------------------------- AdamW over many tensors
+def _sizes(c):
+    """element counts of the case's tensors: ragged, their sum the case's total"""
+    r, n = random.Random(c["layout"]), c["tensors"]
+    w = [math.exp(r.gauss(0, 1.5)) for _ in range(n)]
+    sizes = [max(1, int(c["total"] * x / sum(w))) for x in w]
+    sizes[0] = max(1, c["total"] - sum(sizes[1:]))
+    return sizes
+
+
+def _quantised(x):
+    """8-bit form of a block-padded flat state: (e4m3 values, one scale for each block): the value is their product.  What a block's largest magnitude maps to
+    is 448, the type's largest value; a block below 2^-100 is zero."""
+    x = x.view(-1, BLOCK)
+    top = x.abs().amax(1, keepdim=True)
+    top = torch.where(top < 2.0**-100, 0.0, top)
+    inv = torch.where(top > 0, torch.reciprocal(top) * 448.0, 0.0)
+    return (x * inv).to(torch.float8_e4m3fn).view(-1), (top * (1.0 / 448.0)).view(-1)
+
+
+def _quantised_root(r):
+    """the same for the root of the second moment, whose values above zero stay above zero: the smallest is the type's smallest, 2^-9"""
+    x = r.view(-1, BLOCK)
+    top = x.amax(1, keepdim=True)
+    top = torch.where(top < 2.0**-100, 0.0, top)
+    inv = torch.where(top > 0, torch.reciprocal(top) * 448.0, 0.0)
+    y = x * inv
+    y = torch.where(y > 0, torch.clamp(y, min=2.0**-9), y)
+    return y.to(torch.float8_e4m3fn).view(-1), (top * (1.0 / 448.0)).view(-1)
+
+
+def _prepare_adamw(c, g, dev):
+    sizes = _sizes(c)
+    starts, at = [], 0
+    for z in sizes:
+        starts.append(at)
+        at += -(-z // ALIGN) * ALIGN
+    live = torch.zeros(at, device=dev)
+    for z, o in zip(sizes, starts):
+        live[o:o + z] = 1
+    P, G = TYPES[c["type"]], TYPES[c["grad"]]
+    rnd = lambda: torch.randn(at, device=dev, generator=g) * live  # noqa: E731
+    s = {"c": c, "sizes": sizes, "starts": starts, "step": 10, "param": (rnd() * 0.1).to(P), "grad": (rnd() * 0.02).to(G)}
+    m, r = rnd() * 0.005, (rnd() * 0.02).abs()
+    if c["bits"] == 8:
+        s["m"], s["m_scale"] = _quantised(m)
+        s["v"], s["v_scale"] = _quantised_root(r)
+    else:
+        s["m"], s["v"], s["m_scale"], s["v_scale"] = m, r * r, None, None
+    s["clip"] = torch.rand(1, device=dev, generator=g) * 0.5 + 0.5 if c["clipped"] else None
+    cut = lambda t, per=1: None if t is None else [t[o // per:o // per + -(-z // per)] for z, o in zip(sizes, starts)]  # noqa: E731
+    s["params"], s["grads"], s["ms"], s["vs"] = cut(s["param"]), cut(s["grad"]), cut(s["m"]), cut(s["v"])
+    s["m_scales"], s["v_scales"] = cut(s["m_scale"], BLOCK), cut(s["v_scale"], BLOCK)
+    if own:                 # the list of tensors that an optimizer keeps
+        from marius_amd import hip
+
+        s["tensors"] = hip.AdamWTensors(s["params"], s["ms"], s["vs"], s["m_scales"], s["v_scales"])
+    return s
+
+
+def _outputs_adamw(s):
+    return {"param": s["param"], "m": s["m"], "v": s["v"], "m_scale": s["m_scale"], "v_scale": s["v_scale"]}
+
+
+def _run_adamw_own(s):
+    from marius_amd import hip
+
+    s["step"] += 1
+    hip.adamw_step(s["tensors"], s["grads"], s["step"], LR, BETA1, BETA2, EPS, DECAY, grad_scale=s["clip"])
+    return _outputs_adamw(s)
+
+
+def _blocks(x):
+    """`x` padded with zeros to whole blocks"""
+    return torch.nn.functional.pad(x, (0, -x.numel() % BLOCK))
+
+
+def _update_plain(p, g, m, v, m_scale, v_scale, clip, rate, root):
+    z = p.numel()
+    g = g.float() if clip is None else g.float() * clip
+    w = p.float() * (1.0 - LR * DECAY)
+    if m_scale is None:
+        m0, v0 = m, v
+    else:
+        m0 = (_blocks(m.float()).view(-1, BLOCK) * m_scale.view(-1, 1)).view(-1)[:z]
+        r0 = (_blocks(v.float()).view(-1, BLOCK) * v_scale.view(-1, 1)).view(-1)[:z]
+        v0 = r0 * r0
+    m1 = m0 * BETA1 + g * (1.0 - BETA1)
+    v1 = v0 * BETA2 + (g * (1.0 - BETA2)) * g
+    r1 = torch.sqrt(v1)
+    p.copy_(w - rate * (m1 / (r1 / root + EPS)))
+    if m_scale is None:
+        m.copy_(m1)
+        v.copy_(v1)
+    else:
+        (qm, sm), (qv, sv) = _quantised(_blocks(m1)), _quantised_root(_blocks(r1))
+        m.copy_(qm[:z])
+        v.copy_(qv[:z])
+        m_scale.copy_(sm)
+        v_scale.copy_(sv)
+
+
+def _run_adamw_plain(s):
+    s["step"] += 1
+    rate, root = LR / (1.0 - BETA1 ** s["step"]), math.sqrt(1.0 - BETA2 ** s["step"])
+    none = [None] * len(s["sizes"])
+    for p, g, m, v, ms, vs in zip(s["params"], s["grads"], s["ms"], s["vs"], s["m_scales"] or none, s["v_scales"] or none):
+        _update_plain(p, g, m, v, ms, vs, s["clip"], rate, root)
+    return _outputs_adamw(s)
+
+
+def _exact_adamw(s):
+    """all tensors as one flat vector (they start on whole blocks; what lies between them is zero and stays so)"""
+    t = s["step"] + 1
+    g = s["grad"].double() * (1.0 if s["clip"] is None else s["clip"].double())
+    if s["m_scale"] is None:
+        m, v = s["m"].double(), s["v"].double()
+    else:
+        m = s["m"].double() * s["m_scale"].double().repeat_interleave(BLOCK)
+        v = (s["v"].double() * s["v_scale"].double().repeat_interleave(BLOCK)) ** 2
+    m, v = BETA1 * m + (1 - BETA1) * g, BETA2 * v + (1 - BETA2) * g ** 2
+    w = s["param"].double()
+    w = w - LR * DECAY * w - LR * (m / (1 - BETA1 ** t)) / ((v / (1 - BETA2 ** t)).sqrt() + EPS)
+    if s["m_scale"] is None:
+        return {"param": w, "m": m, "v": v, "m_scale": None, "v_scale": None}
+    out = {"param": w}
+    for name, x in (("m", m), ("v", v.sqrt())):
+        step = x.abs().view(-1, BLOCK).max(1)[0] / 448
+        y = x / torch.where(step > 0, step, 1.0).repeat_interleave(BLOCK)
+        if name == "v":
+            y = torch.where((y > 0) & (y < 2.0**-9), 2.0**-9, y)
+        out[name], out[name + "_scale"] = y.to(torch.float8_e4m3fn).double(), step
+    return out
+
+
+def _work_adamw(c):
+    state = 16 if c["bits"] == 32 else 4 + 16 / BLOCK    # both moments in and out
+    return {"bytes": c["total"] * (2 * BYTES[c["type"]] + BYTES[c["grad"]] + state), "flops": 15.0 * c["total"]}
+
+
+# ---------------------------------------------------------------------------------------------------------------- what the tools call
+def prepare(case, seed):
+    dev = torch.device("cuda:0")
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return {"attention": _prepare_attention, "norm": _prepare_norm, "adamw": _prepare_adamw}[case["op"]](case, g, dev)
+
+
+def run(state):
+    op = state["c"]["op"]
+    if own:
+        return {"attention": _run_attention_own, "norm": _run_norm_own, "adamw": _run_adamw_own}[op](state)
+    return {"attention": _run_attention_plain, "norm": _run_norm_plain, "adamw": _run_adamw_plain}[op](state)
+
+
+def work(case):
+    return {"attention": _work_attention, "norm": _work_norm, "adamw": _work_adamw}[case["op"]](case)
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    return {"attention": _exact_attention, "norm": _exact_norm, "adamw": _exact_adamw}[case["op"]](s)
