@@ -14,7 +14,10 @@ name, defs = sys.argv[1], sys.argv[2:]
 kdir = os.path.join(ROOT, "marius_amd", "csrc", "kernels")
 out = os.path.join(ROOT, "build_abl", name)
 os.makedirs(out, exist_ok=True)
-flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-I" + os.path.join(ROOT, "include"), "-I" + kdir] + defs
+sys.path.insert(0, ROOT)
+from marius_amd.build import KERNEL_FLAGS  # noqa: E402
+
+flags = KERNEL_FLAGS + ["-I" + os.path.join(ROOT, "include"), "-I" + kdir] + defs
 procs, objs = [], []
 for f in sorted(os.listdir(kdir)):
     if f.endswith(".hip"):
