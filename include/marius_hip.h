@@ -49,16 +49,17 @@ enum {
  * marius_table_absmax_counted; marius_lp_layout lost the operand planes of the removed bf16x6 kernels and the stream-K partials; 8:
  * marius_lp_desc.upd_*, marius_segment_update.fused_below, marius_lp_fuses_endpoint_update, marius_segment_plan_occ_single; 9: the
  * fixed-capacity exchange entry points marius_a2a_capacity / marius_a2a_rows_post / marius_a2a_rows_wait, negative ids = padding slots in
- * marius_merge_unique_runs / marius_segment_plan; 10: marius_a2a_publish / marius_a2a_record_* / marius_owner_offsets_counts, marius_layer_post_hook*, marius_prepare_maps; 11: marius_lp_layout.flash_cfg, marius_prepare_maps_preferred, the neighbour-sampling / GraphSage entry points marius_nbr_* and marius_segment_gather_sum).  Every binder
+ * marius_merge_unique_runs / marius_segment_plan; 10: marius_a2a_publish / marius_a2a_record_* / marius_owner_offsets_counts, marius_layer_post_hook*, marius_prepare_maps; 11: marius_lp_layout.flash_cfg, marius_prepare_maps_preferred, the neighbour-sampling / GraphSage entry points marius_nbr_* and marius_segment_gather_sum; 12: marius_residual_norm_*, marius_nbr_plan_* / marius_neighbor_attention_*, marius_adamw_step).  Every binder
  * compares the value it was built against with what the loaded library returns and refuses to run on a mismatch: marius_amd/hip.py lib(),
  * the host module's init (bindings.cpp), and the plug-in recipe of INTEGRATION.md. */
-#define MARIUS_HIP_ABI_VERSION 11
+#define MARIUS_HIP_ABI_VERSION 12
 int marius_hip_abi_version(void);
 /* The MARIUS_* environment switches of the kernel library (test / A-B selectors; a production run sets none) are read ONCE, when the
  * library is loaded.  A process that changes one afterwards (the parity tests do, to reach a non-default kernel) calls this to re-read them. */
 int marius_config_reload(void);
 /* sizeof(marius_lp_desc) / sizeof(marius_lp_layout) as the library was compiled: a second line of defence for ctypes mirrors */
-int marius_hip_struct_bytes(int which /* 0: marius_lp_desc, 1: marius_lp_layout, 2: marius_segment_update */);
+int marius_hip_struct_bytes(int which /* 0: marius_lp_desc, 1: marius_lp_layout, 2: marius_segment_update, 3: marius_residual_norm, 4: marius_residual_norm_grads,
+                                         5: marius_neighbor_plan, 6: marius_neighbor_attention, 7: marius_adamw_tensor */);
 const char* marius_hip_last_error(void);
 
 /* Optional HIP-event profiler (bench.py's roofline): when enabled, the library records hipEvents on the launch stream
@@ -557,6 +558,103 @@ int marius_nbr_positions(const int64_t* node_ids, int64_t n, const int64_t* edge
 int marius_segment_gather_sum(const float* rows, int64_t rows_ld, int32_t d, const int64_t* index_a, const int64_t* offsets_a, int64_t T_a,
                               const int64_t* index_b, const int64_t* offsets_b, int64_t T_b, int64_t n, const int64_t* pre_div, const int64_t* deg_a,
                               const int64_t* deg_b, int32_t mode, const float* self_rows, int64_t self_ld, float* out, int64_t out_ld, marius_stream_t stream);
+
+/* ---- the training block of an attention encoder: element types of the entry points below (statistics and sums are fp32 throughout) ----------- */
+enum { MARIUS_F32 = 0, MARIUS_BF16 = 1, MARIUS_F16 = 2 };
+
+/* The norms before and after a block, fused with the block's gate and the scaled residual (norm.hip):
+ *   u = post_norm ? norm(block) : block;   y = residual_scale * x + act(gate) * u;   h = norm(y)  (pre_norm: the next block's input)
+ *   RMS: norm(v) = v / sqrt(mean v^2 + eps) * w + b;  LAYER: the same of v - mean v.
+ * x / y are rows of stream_type (fp32, or `type`), block / h / element gates of `type`, weights, biases and channel gates of param_type (NULL weight: ones, NULL
+ * bias: zeros).  Rows of 1 to 8192 elements, any row stride >= d and any alignment of the element type.  y and h are rounded once each; h comes from the
+ * unrounded y.  Without a block (has_block = 0) h = norm(x) and y is not written.
+ * The backward pass takes the gradients of y and h (either may be NULL: zero), the STORED y and the block, and takes the statistics again.  dx (NULL: not wanted),
+ * dblock, dgate ([n, d] of `type`, or [d] of param_type: the sum over rows), weight and bias gradients of param_type (NULL: not wanted); sums over rows go
+ * through `workspace` in a fixed order: the same bits on every run.  dx = residual_scale * (grad_y + what comes back through the pre norm). */
+enum { MARIUS_NORM_RMS = 0, MARIUS_NORM_LAYER = 1 };
+enum { MARIUS_GATE_NONE = 0, MARIUS_GATE_CHANNEL = 1 /* [d] */, MARIUS_GATE_ELEMENT = 2 /* [n, d] */ };
+typedef struct marius_residual_norm {
+    int64_t n;
+    int32_t d, stream_type, type, param_type;
+    int32_t kind, post_norm, pre_norm, has_block, gate_mode, gate_activation /* MARIUS_ACT_* */;
+    float eps, residual_scale;
+    const void* gate;
+    int64_t gate_ld; /* element gates */
+    const void *post_weight, *post_bias, *pre_weight, *pre_bias;
+} marius_residual_norm;
+typedef struct marius_residual_norm_grads {
+    const void *grad_y, *grad_h;
+    int64_t grad_y_ld, grad_h_ld;
+    void *dx, *dblock, *dgate;
+    int64_t dx_ld, dblock_ld, dgate_ld;
+    void *dpost_weight, *dpost_bias, *dpre_weight, *dpre_bias;
+} marius_residual_norm_grads;
+int marius_residual_norm_forward(const marius_residual_norm* desc, const void* x, int64_t x_ld, const void* block, int64_t block_ld, void* y, int64_t y_ld, void* h,
+                                 int64_t h_ld, marius_stream_t stream);
+size_t marius_residual_norm_workspace_bytes(int64_t n, int32_t d);
+int marius_residual_norm_backward(const marius_residual_norm* desc, const marius_residual_norm_grads* grads, const void* y, int64_t y_ld, const void* block, int64_t block_ld,
+                                  void* workspace, size_t workspace_bytes, marius_stream_t stream);
+
+/* Neighbour lists in both directions, made once for a sampled batch or a graph and used by every pass over it (nbr_plan.hip).
+ * marius_nbr_plan_lists: the list of target i is its part of list a (entries offsets_a[i] .. offsets_a[i + 1), the last one ends at T_a), then of list b (T_b = 0:
+ *   none), then its own row self_offset + i (self_offset < 0: none).  T = T_a + T_b (+ n).  Out: offsets [n + 1], index / owner [T] (row and target of every
+ *   entry), keys [T] (the rows once more, for marius_sort_unique), status [4] (ZEROED by the caller): bit 0: offsets that do not ascend from 0 and cover
+ *   their list, bit 1: a row outside [0, rows).  A caller reads status before it goes on: the calls below and the attention take the lists as they are.
+ * marius_nbr_plan_reverse: the entries grouped by row, in list order: r_offsets [rows + 1], r_owner [T]; perm of marius_sort_unique = r_entry.
+ * marius_nbr_plan_items: lists cut into work items of at most `chunk` entries: items {list, first, end, slot or -1} (at most n + T / chunk), splits {list, first
+ *   slot, parts, 0} of the lists that were cut (at most T / chunk), totals [3] = items, slots, splits. */
+size_t marius_nbr_plan_workspace_bytes(int64_t n);
+int marius_nbr_plan_lists(const int64_t* index_a, const int64_t* offsets_a, int64_t T_a, const int64_t* index_b, const int64_t* offsets_b, int64_t T_b, int64_t n, int64_t rows,
+                          int64_t self_offset, int32_t* offsets, int32_t* index, int32_t* owner, int64_t* keys, int32_t* status, void* workspace, size_t workspace_bytes,
+                          marius_stream_t stream);
+int marius_nbr_plan_reverse(const int64_t* uniq, const int32_t* seg_offsets, const int64_t* num_unique_dev, const int32_t* perm, const int32_t* owner, int64_t T, int64_t rows,
+                            int32_t* r_offsets, int32_t* r_owner, marius_stream_t stream);
+int marius_nbr_plan_items(const int32_t* offsets, int64_t n, int32_t chunk, int32_t* items, int32_t max_items, int32_t* splits, int32_t max_splits, int32_t* totals,
+                          void* workspace, size_t workspace_bytes, marius_stream_t stream);
+typedef struct marius_neighbor_plan {
+    int64_t n, rows, T;
+    const int32_t* index;                                    /* [T] */
+    const int32_t *items, *splits;                           /* of the targets' lists */
+    int32_t n_items, n_slots, n_splits, reserved_;
+    const int32_t *r_owner, *r_entry, *r_items, *r_splits;   /* of the rows' lists */
+    int32_t r_n_items, r_n_slots, r_n_splits, r_reserved_;
+} marius_neighbor_plan;
+
+/* Attention of the targets over their lists (nbr_attention.hip): s_e = scale * q_i . k_j + bias_e per query head, o_i = sum softmax(s)_e v_j; heads is a multiple
+ * of kv_heads (query heads h and key head h / (heads / kv_heads)), heads of 1 to 256 elements, contiguous; row and head strides in elements are the caller's.
+ * bias [T, heads] fp32 or NULL, in the plan's entry order; -inf masks an entry: its key and value are not used.  A list without a live entry gives o = 0.
+ * stats [n, heads, 2] fp32, written by the forward and read by the backward pass: largest score (-inf: none) and the log of the sum of exp(score - largest).
+ * Forward: out [n, heads, dim].  Backward: dq [n, heads, dim], dk / dv [rows, kv_heads, dim] (contiguous; rows that no list names get zero), dbias [T, heads] or NULL.
+ * No atomics: the same bits on every run.  Workspace: marius_neighbor_attention_workspace_bytes. */
+typedef struct marius_neighbor_attention {
+    int32_t heads, kv_heads, dim, type;
+    float scale;
+    int32_t reserved_;
+    const void *q, *k, *v;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    const float* bias;
+    float* stats;
+} marius_neighbor_attention;
+size_t marius_neighbor_attention_workspace_bytes(const marius_neighbor_plan* plan, int32_t heads, int32_t kv_heads, int32_t dim, int32_t backward);
+int marius_neighbor_attention_forward(const marius_neighbor_plan* plan, const marius_neighbor_attention* desc, void* out, void* workspace, size_t workspace_bytes,
+                                      marius_stream_t stream);
+int marius_neighbor_attention_backward(const marius_neighbor_plan* plan, const marius_neighbor_attention* desc, const void* grad_out, int64_t grad_row, int64_t grad_head,
+                                       void* dq, void* dk, void* dv, float* dbias, void* workspace, size_t workspace_bytes, marius_stream_t stream);
+
+/* AdamW over many tensors (adamw.hip): p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps), moments m and v updated first; t = step (from 1),
+ * or *step_dev (a captured call replays with the step it finds there).  Every gradient is multiplied by *grad_scale (NULL: 1).  All tensors of a call have
+ * parameters of param_type and gradients of grad_type; a launch takes 64 tensors.  state_bits 32: exp_avg / exp_avg_sq fp32 [n].  state_bits 8: e4m3 codes [n] and one
+ * fp32 scale for every 256 elements [ceil(n / 256)]; exp_avg_sq then holds the ROOT of the second moment (value = code * scale in both), and a root above zero stays
+ * above zero. */
+typedef struct marius_adamw_tensor {
+    void* param;
+    const void* grad;
+    void *exp_avg, *exp_avg_sq;
+    float *exp_avg_scale, *exp_avg_sq_scale;
+    int64_t n;
+} marius_adamw_tensor;
+int marius_adamw_step(const marius_adamw_tensor* tensors, int32_t count, int32_t param_type, int32_t grad_type, int32_t state_bits, int64_t step, const int64_t* step_dev,
+                      double lr, double beta1, double beta2, double eps, double weight_decay, const float* grad_scale, marius_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,245 @@
+// AdamW over many tensors in one launch, its two moments in fp32 or in 8 bits.
+//
+//     g = gradient (* *grad_scale)            m = beta1 m + (1 - beta1) g            v = beta2 v + (1 - beta2) g g
+//     p = p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+//
+// 8-bit states: blocks of 256 elements with one fp32 scale each.  m is held as e4m3 times its block's scale; of v the ROOT is held (what the step divides
+// by), e4m3 times its scale: e4m3 reaches 2^18 down from a block's largest value, which for the root is 2^36 of v.  A root above zero never becomes zero (it
+// stays at the type's smallest value): a weight whose gradients are tiny beside its block's would otherwise be divided by eps alone.  scale = largest / 448,
+// the type's largest value; a block whose largest magnitude is below 2^-100 is zero (its reciprocal would leave fp32).  The step itself uses the new
+// moments before they are rounded.  All of it is single fp32 operations in the order written (no contraction): the same bits from any other
+// program that does them in this order.
+//
+// Bound by HBM: 28 bytes an element with fp32 states, 16.1 with 8-bit ones (fp32 parameters and gradients).  A workgroup takes tiles of 2048 elements, eight
+// per lane (16-byte loads of every stream; the 32 lanes of a block share its scale by shuffles), and finds its tensor by binary search in the launch's own
+// arguments: no table in memory to build, to keep or to go stale.
+#include "row_types.h"
+
+namespace marius {
+
+constexpr int AW_T = 256, AW_EPT = 8, AW_TILE = AW_T * AW_EPT, AW_TENSORS = 64, AW_BLOCK = 256;
+
+struct AwTensor {
+    void* p;
+    const void* g;
+    void *m, *v;
+    float *ms, *vs;
+    int64_t n;
+};
+struct AwArgs {
+    AwTensor t[AW_TENSORS];
+    int first[AW_TENSORS + 1];  // first tile of every tensor
+    int count;
+    float decay, rate, beta1, omb1, beta2, omb2, inv_root, eps;
+    const float* grad_scale;
+    const int64_t* step_dev;    // the step's number on the device: rate and inv_root are taken from it
+    double lr, beta1_d, beta2_d;
+};
+static_assert(sizeof(AwArgs) <= 4096, "kernel arguments");
+
+template <typename X>
+__device__ __forceinline__ void aw_load(const X* p, int64_t i, int left, float (&v)[AW_EPT]) {
+    if (left >= AW_EPT) {
+        X t[AW_EPT];
+        __builtin_memcpy(t, p + i, sizeof(t));
+#pragma unroll
+        for (int e = 0; e < AW_EPT; ++e) v[e] = (float)t[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < AW_EPT; ++e) v[e] = e < left ? (float)p[i + e] : 0.f;
+    }
+}
+template <typename X>
+__device__ __forceinline__ void aw_store(X* p, int64_t i, int left, const float (&v)[AW_EPT]) {
+    if (left >= AW_EPT) {
+        X t[AW_EPT];
+#pragma unroll
+        for (int e = 0; e < AW_EPT; ++e) t[e] = (X)v[e];
+        __builtin_memcpy(p + i, t, sizeof(t));
+    } else {
+#pragma unroll
+        for (int e = 0; e < AW_EPT; ++e)
+            if (e < left) p[i + e] = (X)v[e];
+    }
+}
+// eight e4m3 codes <-> floats (the conversions round to nearest even)
+__device__ __forceinline__ void aw_load8(const uint8_t* p, int64_t i, int left, float (&v)[AW_EPT]) {
+    uint8_t c[AW_EPT] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (left >= AW_EPT) __builtin_memcpy(c, p + i, sizeof(c));
+    else
+#pragma unroll
+        for (int e = 0; e < AW_EPT; ++e)
+            if (e < left) c[e] = p[i + e];
+    int w[2];
+    __builtin_memcpy(w, c, sizeof(w));
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w[q], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w[q], true);
+        v[4 * q] = a[0];
+        v[4 * q + 1] = a[1];
+        v[4 * q + 2] = b[0];
+        v[4 * q + 3] = b[1];
+    }
+}
+__device__ __forceinline__ void aw_store8(uint8_t* p, int64_t i, int left, const float (&v)[AW_EPT]) {
+    int w[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        w[q] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * q], v[4 * q + 1], 0, false);
+        w[q] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * q + 2], v[4 * q + 3], w[q], true);
+    }
+    uint8_t c[AW_EPT];
+    __builtin_memcpy(c, w, sizeof(c));
+    if (left >= AW_EPT) __builtin_memcpy(p + i, c, sizeof(c));
+    else
+#pragma unroll
+        for (int e = 0; e < AW_EPT; ++e)
+            if (e < left) p[i + e] = c[e];
+}
+// a block's 32 lanes: largest |x| -> the scale to keep and the factor that takes x to e4m3's range
+__device__ __forceinline__ void aw_scale(const float (&x)[AW_EPT], float& scale, float& inv) {
+#pragma clang fp contract(off)
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < AW_EPT; ++e) top = fmaxf(top, fabsf(x[e]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if (top < 0x1p-100f) top = 0.f;
+    scale = top * (1.f / 448.f);
+    inv = top > 0.f ? (1.f / top) * 448.f : 0.f;
+}
+
+template <typename P, typename G, bool BITS8>
+__global__ __launch_bounds__(AW_T) void adamw_kernel(AwArgs A) {
+#pragma clang fp contract(off)
+    int lo = 0, hi = A.count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (A.first[mid] <= (int)blockIdx.x) lo = mid;
+        else hi = mid;
+    }
+    const AwTensor t = A.t[lo];
+    const int64_t i = (int64_t)((int)blockIdx.x - A.first[lo]) * AW_TILE + (int)threadIdx.x * AW_EPT;
+    const int left = t.n - i >= AW_EPT ? AW_EPT : t.n > i ? (int)(t.n - i) : 0;
+    float rate = A.rate, inv_root = A.inv_root;
+    if (A.step_dev) {
+        const double step = (double)*A.step_dev;
+        rate = (float)(A.lr / (1.0 - pow(A.beta1_d, step)));
+        inv_root = (float)(1.0 / sqrt(1.0 - pow(A.beta2_d, step)));
+    }
+    const float gs = A.grad_scale ? *A.grad_scale : 1.f;
+    float p[AW_EPT], g[AW_EPT], m[AW_EPT], v[AW_EPT], r[AW_EPT];
+    aw_load<P>((const P*)t.p, i, left, p);
+    aw_load<G>((const G*)t.g, i, left, g);
+    if (BITS8) {
+        aw_load8((const uint8_t*)t.m, i, left, m);
+        aw_load8((const uint8_t*)t.v, i, left, v);
+        const float sm = left > 0 ? t.ms[i / AW_BLOCK] : 0.f, sv = left > 0 ? t.vs[i / AW_BLOCK] : 0.f;
+#pragma unroll
+        for (int e = 0; e < AW_EPT; ++e) {
+            m[e] = m[e] * sm;
+            v[e] = v[e] * sv;
+            v[e] = v[e] * v[e];
+        }
+    } else {
+        aw_load<float>((const float*)t.m, i, left, m);
+        aw_load<float>((const float*)t.v, i, left, v);
+    }
+#pragma unroll
+    for (int e = 0; e < AW_EPT; ++e) {
+        if (A.grad_scale) g[e] = g[e] * gs;
+        m[e] = m[e] * A.beta1 + g[e] * A.omb1;
+        v[e] = v[e] * A.beta2 + (g[e] * A.omb2) * g[e];
+        r[e] = sqrtf(v[e]);
+        p[e] = p[e] * A.decay - rate * (m[e] / (r[e] * inv_root + A.eps));
+    }
+    aw_store<P>((P*)t.p, i, left, p);
+    if (BITS8) {
+        float scale, inv;
+        aw_scale(m, scale, inv);  // (every lane takes part: elements behind the tensor are zero)
+        float rscale, rinv;
+        aw_scale(r, rscale, rinv);
+        if (left > 0 && (threadIdx.x & 31) == 0) {
+            t.ms[i / AW_BLOCK] = scale;
+            t.vs[i / AW_BLOCK] = rscale;
+        }
+#pragma unroll
+        for (int e = 0; e < AW_EPT; ++e) {
+            m[e] = m[e] * inv;
+            r[e] = r[e] * rinv;
+            if (r[e] > 0.f && r[e] < 0x1p-9f) r[e] = 0x1p-9f;
+        }
+        aw_store8((uint8_t*)t.m, i, left, m);
+        aw_store8((uint8_t*)t.v, i, left, r);
+    } else {
+        aw_store<float>((float*)t.m, i, left, m);
+        aw_store<float>((float*)t.v, i, left, v);
+    }
+}
+
+template <typename P, typename G>
+static void launch_adamw(const AwArgs& A, bool bits8, unsigned tiles, hipStream_t st) {
+    if (bits8) adamw_kernel<P, G, true><<<dim3(tiles), dim3(AW_T), 0, st>>>(A);
+    else adamw_kernel<P, G, false><<<dim3(tiles), dim3(AW_T), 0, st>>>(A);
+}
+template <typename P>
+static void launch_adamw_grad(const AwArgs& A, int grad_type, bool bits8, unsigned tiles, hipStream_t st) {
+    if (grad_type == MARIUS_F32) launch_adamw<P, float>(A, bits8, tiles, st);
+    else if (grad_type == MARIUS_BF16) launch_adamw<P, __bf16>(A, bits8, tiles, st);
+    else launch_adamw<P, _Float16>(A, bits8, tiles, st);
+}
+
+}  // namespace marius
+
+using namespace marius;
+
+extern "C" int marius_adamw_step(const marius_adamw_tensor* tensors, int32_t count, int32_t param_type, int32_t grad_type, int32_t state_bits, int64_t step,
+                                 const int64_t* step_dev, double lr, double beta1, double beta2, double eps, double weight_decay, const float* grad_scale,
+                                 marius_stream_t stream) {
+    MARIUS_REQUIRE(count >= 0 && (count == 0 || tensors), "adamw_step: bad tensor list");
+    MARIUS_REQUIRE(float_type_ok(param_type) && float_type_ok(grad_type), "adamw_step: types are MARIUS_F32 / BF16 / F16");
+    MARIUS_REQUIRE(state_bits == 32 || state_bits == 8, "adamw_step: states are held in 32 or in 8 bits");
+    MARIUS_REQUIRE(step_dev || step >= 1, "adamw_step: steps are counted from 1");
+    MARIUS_REQUIRE(lr >= 0 && beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0 && weight_decay >= 0, "adamw_step: lr, eps, weight_decay >= 0, betas in [0, 1)");
+    for (int k = 0; k < count; ++k) {  // before anything is launched: a refused list leaves every tensor as it was
+        const marius_adamw_tensor& s = tensors[k];
+        MARIUS_REQUIRE(s.n >= 0 && cdiv(s.n, AW_TILE) < (1ll << 30), "adamw_step: bad size of tensor %d", k);
+        MARIUS_REQUIRE(s.n == 0 || (s.param && s.grad && s.exp_avg && s.exp_avg_sq && (state_bits == 32 || (s.exp_avg_scale && s.exp_avg_sq_scale))),
+                       "adamw_step: null pointer in tensor %d", k);
+    }
+    AwArgs A;
+    A.decay = (float)(1.0 - lr * weight_decay);
+    A.rate = step_dev ? 0.f : (float)(lr / (1.0 - std::pow(beta1, (double)step)));
+    A.inv_root = step_dev ? 0.f : (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
+    A.beta1 = (float)beta1;
+    A.omb1 = (float)(1.0 - beta1);
+    A.beta2 = (float)beta2;
+    A.omb2 = (float)(1.0 - beta2);
+    A.eps = (float)eps;
+    A.grad_scale = grad_scale;
+    A.step_dev = step_dev;
+    A.lr = lr;
+    A.beta1_d = beta1;
+    A.beta2_d = beta2;
+    for (int k = 0; k < count;) {
+        A.count = 0;
+        int64_t tiles = 0;
+        for (; k < count && A.count < AW_TENSORS; ++k) {
+            const marius_adamw_tensor& s = tensors[k];
+            if (s.n == 0) continue;
+            const int64_t more = cdiv(s.n, AW_TILE);
+            if (A.count > 0 && tiles + more >= (1ll << 30)) break;  // (a grid's size)
+            A.t[A.count] = AwTensor{s.param, s.grad, s.exp_avg, s.exp_avg_sq, s.exp_avg_scale, s.exp_avg_sq_scale, s.n};
+            A.first[A.count++] = (int)tiles;
+            tiles += more;
+        }
+        if (A.count == 0) break;
+        A.first[A.count] = (int)tiles;
+        if (param_type == MARIUS_F32) launch_adamw_grad<float>(A, grad_type, state_bits == 8, (unsigned)tiles, as_stream(stream));
+        else if (param_type == MARIUS_BF16) launch_adamw_grad<__bf16>(A, grad_type, state_bits == 8, (unsigned)tiles, as_stream(stream));
+        else launch_adamw_grad<_Float16>(A, grad_type, state_bits == 8, (unsigned)tiles, as_stream(stream));
+        const int rc = check_launch("adamw_step");
+        if (rc) return rc;
+    }
+    return MARIUS_OK;
+}

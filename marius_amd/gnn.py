@@ -86,6 +86,18 @@ class DENSEGraph:
         self.in_neighbors_mapping_ = self.out_neighbors_mapping_ = None
         self.src_sorted_edges_ = self.dst_sorted_edges_ = None
         self.in_num_neighbors_ = self.out_num_neighbors_ = None
+        self.plan_ = None
+
+    def neighborPlan(self):
+        """the attention's plan of this layer's lists (outgoing, incoming neighbours, the target's own row), made once between two prepareForNextLayer calls"""
+        if self.plan_ is None:
+            lists = [(m.contiguous(), o.contiguous()) for m, o in ((self.out_neighbors_mapping_, self.out_offsets_), (self.in_neighbors_mapping_, self.in_offsets_)) if m is not None]
+            first = self.getLayerOffset()
+            rows = self.node_ids_.numel()
+            if not lists:  # (a graph without sampled neighbours: every target attends to itself)
+                lists = [(torch.zeros(0, **_i64(self.node_ids_.device)), torch.zeros(rows - first, **_i64(self.node_ids_.device)))]
+            self.plan_ = H.NeighborPlan(*lists[0], rows, *(lists[1] if len(lists) > 1 else (None, None)), self_offset=first)
+        return self.plan_
 
     def performMap(self):
         """graph.cpp:361-398"""
@@ -125,6 +137,7 @@ class DENSEGraph:
 
     def prepareForNextLayer(self):
         """graph.cpp:290-325 (views only)"""
+        self.plan_ = None
         rm = int(self.hop_offsets_[1] - self.hop_offsets_[0])
         fin_nodes = int(self.hop_offsets_[2] - self.hop_offsets_[1])
         if self.src_sorted_edges_.size(0) > 0:
@@ -332,15 +345,140 @@ class GraphSageEncoder(torch.nn.Module):
         return out
 
 
-def node_classification_step(encoder, features, dense_graph, labels, lr, reduction="sum"):
+class _NeighborAttention(torch.autograd.Function):
+    """softmax attention of the targets over their lists (nbr_attention.hip); the backward pass recomputes the probabilities"""
+
+    @staticmethod
+    def forward(ctx, q, k, v, bias, plan, scale):
+        out, stats = H.neighbor_attention(q, k, v, plan, scale, bias)
+        ctx.plan, ctx.scale = plan, scale
+        ctx.save_for_backward(q, k, v, bias, stats)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        q, k, v, bias, stats = ctx.saved_tensors
+        dq, dk, dv, dbias = H.neighbor_attention_backward(grad_out, q, k, v, stats, ctx.plan, ctx.scale, bias, need_dbias=ctx.needs_input_grad[3])
+        return dq, dk, dv, dbias, None, None
+
+
+class _ResidualNorm(torch.autograd.Function):
+    """the norms before and after a block with its gate and residual scale (norm.hip); returns (y, h) without what is not there: (y,), (h,) or both"""
+
+    @staticmethod
+    def forward(ctx, x, block, gate, post_weight, post_bias, pre_weight, pre_bias, how):
+        y, h = H.residual_norm(x, block, gate, post_weight, post_bias, pre_weight, pre_bias, **how)
+        ctx.how, ctx.with_y, ctx.with_h = how, block is not None, h is not None
+        ctx.save_for_backward(y, block, gate, post_weight, post_bias, pre_weight, pre_bias)
+        return tuple(t for t, there in ((y, ctx.with_y), (h, ctx.with_h)) if there)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        grads = list(grads)
+        grad_y = grads.pop(0) if ctx.with_y else None
+        grad_h = grads.pop(0) if ctx.with_h else None
+        got = H.residual_norm_backward(grad_y, grad_h, *ctx.saved_tensors, need_dx=ctx.needs_input_grad[0], **ctx.how)
+        return tuple(got[k] for k in ("dx", "dblock", "dgate", "dpost_weight", "dpost_bias", "dpre_weight", "dpre_bias")) + (None,)
+
+
+def neighbor_attention(q, k, v, plan, scale=None, bias=None):
+    """differentiable H.neighbor_attention: out [n, heads, dim]"""
+    return _NeighborAttention.apply(q, k, v, bias, plan, scale)
+
+
+class ResidualNorm(torch.nn.Module):
+    """The norms around a block: forward(x, block) -> (y, h), y = residual_scale * x + act(gate) * (post norm of the block), h = (pre norm of y), the next
+    block's input; forward(x) -> (x, h) in front of the first block.  gate: "NONE", "CHANNEL" (a learned [dim] vector, from `gate_init`) or "ELEMENT" (given with every call)."""
+
+    def __init__(self, dim, post_norm=False, pre_norm=True, kind="RMS", eps=1e-6, bias=False, gate="NONE", gate_activation="NONE", gate_init=1.0, residual_scale=1.0, device="cuda:0"):
+        super().__init__()
+        vec = lambda there, value: torch.nn.Parameter(torch.full((dim,), value, device=device)) if there else None  # noqa: E731
+        self.gate_kind = gate
+        self.post_weight, self.post_bias = vec(post_norm, 1.0), vec(post_norm and bias, 0.0)
+        self.pre_weight, self.pre_bias = vec(pre_norm, 1.0), vec(pre_norm and bias, 0.0)
+        self.gate = vec(gate == "CHANNEL", gate_init)
+        self.how = dict(post_norm=post_norm, pre_norm=pre_norm, kind=kind, eps=eps, residual_scale=residual_scale, gate_activation=gate_activation)
+
+    def forward(self, x, block=None, gate=None):
+        if block is None:
+            how = dict(self.how, post_norm=False, residual_scale=1.0, gate_activation="NONE")
+            return x, _ResidualNorm.apply(x, None, None, None, None, self.pre_weight, self.pre_bias, how)[0]
+        if (self.gate_kind == "ELEMENT") != (gate is not None):
+            raise H.MariusHipError("ResidualNorm: a gate comes with the call where the module's gate is ELEMENT, and only there")
+        out = _ResidualNorm.apply(x, block, self.gate if gate is None else gate, self.post_weight, self.post_bias, self.pre_weight, self.pre_bias, self.how)
+        return out if len(out) == 2 else (out[0], None)
+
+
+class GraphAttentionLayer(torch.nn.Module):
+    """Dot-product attention of a layer's target nodes over their sampled neighbours (outgoing, then incoming) and themselves: the softmax aggregation beside
+    GraphSageLayer's mean.  kv_heads < heads: heads share keys and values.  num_relations > 0: a learned bias for each relation and head on the edges' scores (3-column
+    edges), and one for the own row."""
+
+    def __init__(self, input_dim, output_dim, heads, kv_heads=None, num_relations=0, device="cuda:0"):
+        super().__init__()
+        if output_dim % heads != 0:
+            raise H.MariusHipError("GraphAttentionLayer: output_dim is a multiple of the number of heads")
+        self.heads, self.kv_heads, self.dim = heads, kv_heads or heads, output_dim // heads
+        glorot = lambda o, i: torch.nn.Parameter(torch.nn.init.xavier_uniform_(torch.empty(o, i, device=device)))  # noqa: E731
+        self.wq, self.wo = glorot(output_dim, input_dim), glorot(output_dim, output_dim)
+        self.wkv = glorot(2 * self.kv_heads * self.dim, input_dim)
+        self.relation_bias = torch.nn.Parameter(torch.zeros(num_relations + 1, heads, device=device)) if num_relations > 0 else None
+
+    def entryBias(self, dense_graph, plan):
+        """the scores' bias, entry by entry in the plan's order: the relation's row of the table, its last row for a target's own entry"""
+        relation = torch.full((plan.num_entries,), self.relation_bias.size(0) - 1, **_i64(plan.device))
+        edges = [e for m, e in ((dense_graph.out_neighbors_mapping_, dense_graph.src_sorted_edges_), (dense_graph.in_neighbors_mapping_, dense_graph.dst_sorted_edges_)) if m is not None]
+        for part, e in enumerate(edges):
+            if e.size(1) != 3:
+                raise H.MariusHipError("GraphAttentionLayer: relation biases need edges of three columns")
+            relation[plan.places(part)] = e.select(1, 1)
+        return self.relation_bias.index_select(0, relation)
+
+    def forward(self, inputs, dense_graph, train=True):
+        plan = dense_graph.neighborPlan()
+        n = plan.n
+        q = torch.matmul(inputs.narrow(0, inputs.size(0) - n, n), self.wq.t()).view(n, self.heads, self.dim)
+        kv = torch.matmul(inputs, self.wkv.t()).view(inputs.size(0), 2, self.kv_heads, self.dim)
+        bias = None if self.relation_bias is None else self.entryBias(dense_graph, plan)
+        out = neighbor_attention(q, kv[:, 0], kv[:, 1], plan, None, bias)
+        return torch.matmul(out.view(n, self.heads * self.dim), self.wo.t())
+
+
+class GraphAttentionEncoder(torch.nn.Module):
+    """An encoder of attention blocks over a sampled DENSE graph, beside GraphSageEncoder and with its call: the features are projected to `dim`, every layer is
+    y = residual_scale x + gate * norm(attention(norm(x))) with the norms of ResidualNorm, the last one's output goes through `classes` linear outputs."""
+
+    def __init__(self, input_dim, dim, classes, layers, heads, kv_heads=None, num_relations=0, kind="RMS", post_norm=True, gate="CHANNEL", residual_scale=1.0, device="cuda:0"):
+        super().__init__()
+        glorot = lambda o, i: torch.nn.Parameter(torch.nn.init.xavier_uniform_(torch.empty(o, i, device=device)))  # noqa: E731
+        self.project, self.classify = glorot(dim, input_dim), glorot(classes, dim)
+        self.first = ResidualNorm(dim, kind=kind, device=device)
+        self.layers = torch.nn.ModuleList([GraphAttentionLayer(dim, dim, heads, kv_heads, num_relations, device) for _ in range(layers)])
+        self.norms = torch.nn.ModuleList([ResidualNorm(dim, post_norm=post_norm, kind=kind, gate=gate, residual_scale=residual_scale, device=device) for _ in range(layers)])
+
+    def forward(self, features, dense_graph, train=True):
+        dense_graph.performMap()
+        x, h = self.first(torch.matmul(features, self.project.t()))
+        for i, (layer, norm) in enumerate(zip(self.layers, self.norms)):
+            block = layer(h, dense_graph, train)
+            x, h = norm(x.narrow(0, x.size(0) - block.size(0), block.size(0)), block)
+            if i < len(self.layers) - 1:
+                dense_graph.prepareForNextLayer()
+        return torch.matmul(h, self.classify.t())
+
+
+def node_classification_step(encoder, features, dense_graph, labels, lr, reduction="sum", optimizer=None):
     """Model::train_batch, NODE_CLASSIFICATION branch (src/cpp/src/nn/model.cpp:317-328): y_pred for the batch's target nodes, CrossEntropyLoss
     (src/cpp/src/nn/loss.cpp:88-102), backward, the dense Adagrad step of every layer parameter (marius_dense_adagrad_step: optim.cpp:114-145;
-    the sums live in `.adagrad_sum` of the parameters).  Returns (loss, y_pred)."""
+    the sums live in `.adagrad_sum` of the parameters), or optimizer.step() where one is given (marius_amd.optim.AdamW; lr is its own then).  Returns (loss, y_pred)."""
     for p in encoder.parameters():
         p.grad = None
     y = encoder(features, dense_graph, True)
     loss = torch.nn.functional.cross_entropy(y, labels.to(torch.int64), reduction=reduction)
     loss.backward()
+    if optimizer is not None:
+        optimizer.step()
+        return loss.detach(), y.detach()
     with torch.no_grad():
         for p in encoder.parameters():
             if p.grad is None:

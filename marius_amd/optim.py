@@ -1,0 +1,63 @@
+"""AdamW over all parameters of a model in one launch per 64 tensors (marius_adamw_step), beside the dense Adagrad / Adam steps of marius_amd.hip."""
+import torch
+
+from . import hip as H
+
+
+class AdamW:
+    """AdamW with decoupled weight decay over device tensors, their states in 32 bits or in 8 (state_bits=8: e4m3 codes and a float32 scale for every 256 elements, the
+    second moment as its root; 2 instead of 8 bytes a parameter).  step() takes the gradients from `.grad`; a parameter without one is left as it is.
+    capturable=True: the step's number lives on the device and step() may be captured into a graph and replayed (the gradients then are the captured tensors)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, capturable=False):
+        self.params = [p for p in params]
+        if state_bits not in (32, 8):
+            raise H.MariusHipError("AdamW: states are held in 32 or in 8 bits")
+        if not self.params:
+            raise H.MariusHipError("AdamW: no parameters")
+        self.lr, self.betas, self.eps, self.weight_decay, self.state_bits, self.capturable = lr, tuple(betas), eps, weight_decay, state_bits, capturable
+        kind = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
+        self.exp_avg, self.exp_avg_sq = ([torch.zeros(p.shape, dtype=torch.float32, device=p.device).to(kind) for p in self.params] for _ in range(2))
+        blocks = lambda p: torch.zeros(-(-p.numel() // H.ADAMW_BLOCK), dtype=torch.float32, device=p.device)  # noqa: E731
+        self.exp_avg_scale, self.exp_avg_sq_scale = (None if state_bits == 32 else [blocks(p) for p in self.params] for _ in range(2))
+        self.num_steps = 0
+        groups = {}
+        for i, p in enumerate(self.params):
+            groups.setdefault((p.device, p.dtype), []).append(i)
+        of = lambda ts, at: None if ts is None else [ts[i] for i in at]  # noqa: E731
+        self._groups = [(at, H.AdamWTensors(of(self.params, at), of(self.exp_avg, at), of(self.exp_avg_sq, at), of(self.exp_avg_scale, at), of(self.exp_avg_sq_scale, at)))
+                        for at in groups.values()]
+        self._step_dev = {dev: torch.zeros(1, dtype=torch.int64, device=dev) for dev in {p.device for p in self.params}} if capturable else None
+
+    def zero_grad(self):
+        for p in self.params:
+            p.grad = None
+
+    @torch.no_grad()
+    def step(self, grad_scale=None):
+        """one step; grad_scale: float32 device tensor of one element that multiplies every gradient (a clipping factor, the inverse of a loss scale)"""
+        if self.capturable:
+            for t in self._step_dev.values():
+                t.add_(1)
+        else:
+            self.num_steps += 1
+        for at, tensors in self._groups:
+            grads = [self.params[i].grad for i in at]
+            for kind in {g.dtype for g in grads if g is not None}:   # (one kind of gradient in every program we know of)
+                H.adamw_step(tensors, [g if g is not None and g.dtype == kind else None for g in grads], self._step_dev[tensors.device] if self.capturable else self.num_steps,
+                             self.lr, *self.betas, self.eps, self.weight_decay, grad_scale)
+
+    def state_dict(self):
+        steps = int(next(iter(self._step_dev.values()))) if self.capturable else self.num_steps
+        return {"num_steps": steps, "state_bits": self.state_bits, "lr": self.lr, "betas": self.betas, "eps": self.eps, "weight_decay": self.weight_decay,
+                "exp_avg": self.exp_avg, "exp_avg_sq": self.exp_avg_sq, "exp_avg_scale": self.exp_avg_scale, "exp_avg_sq_scale": self.exp_avg_sq_scale}
+
+    def load_state_dict(self, state):
+        if state["state_bits"] != self.state_bits or [t.shape for t in state["exp_avg"]] != [t.shape for t in self.exp_avg]:
+            raise H.MariusHipError("AdamW: the state is of other parameters, or held in other bits")
+        self.num_steps, self.lr, self.betas, self.eps, self.weight_decay = state["num_steps"], state["lr"], tuple(state["betas"]), state["eps"], state["weight_decay"]
+        for name in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
+            for mine, theirs in zip(getattr(self, name) or [], state[name] or []):
+                mine.copy_(theirs)
+        for t in (self._step_dev or {}).values():
+            t.fill_(state["num_steps"])

@@ -3,6 +3,7 @@ the harness with its `kernel<<<grid, block, shmem, stream>>>(args);` launches re
 compiled by g++ against the shim tests/emul/common.h (HIP's execution model on host threads; the copies' `#include "common.h"` resolves to the
 shim, not to the hipcc header of the same name).  The product sources are not touched and nothing under marius_amd/ can reach this library.
 python tests/emul/build_emul.py"""
+import concurrent.futures as cf
 import os
 import re
 import subprocess
@@ -10,8 +11,9 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 KDIR = os.path.join(ROOT, "marius_amd", "csrc", "kernels")
-FILES = ["neighbor.hip", "rows.hip", "rng.hip", "encoder.hip", "segreduce.hip", "sort_unique.hip", "exchange.hip", "lp_decoder.hip", "eval_filter.hip"]
-HEADERS = ["seg_plan.h", "lp_common.h"]  # kernel-side headers the files include by name: copied next to them (their own `#include "common.h"` then finds the shim)
+FILES = ["neighbor.hip", "rows.hip", "rng.hip", "encoder.hip", "segreduce.hip", "sort_unique.hip", "exchange.hip", "lp_decoder.hip", "eval_filter.hip",
+         "norm.hip", "adamw.hip", "nbr_plan.hip", "nbr_attention.hip"]
+HEADERS = ["seg_plan.h", "lp_common.h", "row_types.h"]  # kernel-side headers the files include by name: copied next to them (their own `#include "common.h"` then finds the shim)
 
 
 def _match(s, i, open_ch, close_ch):
@@ -82,6 +84,13 @@ def transform(src):
         i = a1 + 1
 
 
+def _compile(cmd):
+    """None, or the end of what a failing compiler said (the compilers run without a preloaded sanitizer runtime: it slows them to a crawl)"""
+    env = {k: v for k, v in os.environ.items() if k != "LD_PRELOAD"}
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, env=env)
+    return r.stdout[-6000:] if r.returncode != 0 else None
+
+
 def build(force=False, sanitize=False):
     """sanitize: -fsanitize=address,undefined (load it into a python started with LD_PRELOAD=libasan.so: tests/test_kernels_emul_cpu.py does)"""
     out_dir = os.path.join(HERE, "_build")
@@ -94,23 +103,32 @@ def build(force=False, sanitize=False):
     for h in HEADERS:
         with open(os.path.join(KDIR, h)) as fh, open(os.path.join(out_dir, h), "w") as oh:
             oh.write(transform(fh.read()))
-    for f in FILES:
-        with open(os.path.join(KDIR, f)) as fh:
-            text = transform(fh.read())
-        with open(os.path.join(out_dir, f + ".inc"), "w") as fh:
+    # one translation unit per kernel file, compiled side by side (the shim's state is inline variables: one copy in the library)
+    units = [("kernels_emul.cpp", None)] + [(f + ".cpp", f) for f in FILES]
+    jobs, objects = [], []
+    for unit, f in units:
+        if f is None:
+            with open(os.path.join(HERE, unit)) as fh:
+                text = fh.read()
+        else:
+            with open(os.path.join(KDIR, f)) as fh:
+                text = "#include <algorithm>\n#include <numeric>\n\n#include \"common.h\"\n" + transform(fh.read())
+        with open(os.path.join(out_dir, unit), "w") as fh:
             fh.write(text)
-    with open(os.path.join(HERE, "kernels_emul.cpp")) as fh:
-        harness = fh.read()
-    with open(os.path.join(out_dir, "kernels_emul.cpp"), "w") as fh:
-        fh.write(harness + "".join('#include "%s.inc"\n' % f for f in FILES))
-    cmd = ["g++", "-std=c++20", "-O1", "-g", "-fPIC", "-shared", "-pthread", "-ffp-contract=off", "-Wno-unknown-pragmas",
-           # -Bsymbolic: the emulated library defines the SAME symbols as libmarius_hip.so (entry points, and the kernels' names, which are host-side launch
-           # stubs there); a process that has the HIP library loaded globally (marius_amd.host() does) must not get them interposed into this one
-           "-Wl,-Bsymbolic", "-I" + HERE, "-I" + os.path.join(ROOT, "include"), os.path.join(out_dir, "kernels_emul.cpp"), "-o", lib]
-    cmd += ["-fsanitize=address,undefined", "-fno-omit-frame-pointer"] if sanitize else []
-    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("emulation build failed:\n" + r.stdout[-6000:])
+        obj = os.path.join(out_dir, unit + (".asan.o" if sanitize else ".o"))
+        objects.append(obj)
+        jobs.append(["g++", "-std=c++20", "-O1", "-g", "-fPIC", "-pthread", "-ffp-contract=off", "-Wno-unknown-pragmas", "-I" + HERE, "-I" + os.path.join(ROOT, "include"),
+                     "-c", os.path.join(out_dir, unit), "-o", obj] + (["-fsanitize=address,undefined", "-fno-omit-frame-pointer"] if sanitize else []))
+    # -Bsymbolic: the emulated library defines the SAME symbols as libmarius_hip.so (entry points, and the kernels' names, which are host-side launch
+    # stubs there); a process that has the HIP library loaded globally (marius_amd.host() does) must not get them interposed into this one
+    link = ["g++", "-shared", "-pthread", "-Wl,-Bsymbolic"] + objects + ["-o", lib] + (["-fsanitize=address,undefined"] if sanitize else [])
+    with cf.ThreadPoolExecutor(max_workers=8) as ex:
+        for r in ex.map(_compile, jobs):
+            if r is not None:
+                raise RuntimeError("emulation build failed:\n" + r)
+    r = _compile(link)
+    if r is not None:
+        raise RuntimeError("emulation build failed:\n" + r)
     return lib
 
 

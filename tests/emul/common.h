@@ -368,6 +368,30 @@ inline emul::vec<float, 16> __builtin_amdgcn_mfma_f32_32x32x2f32(float a, float 
     emul::wave_barrier();
     return c;
 }
+// e4m3 (OCP): v_cvt_pk_f32_fp8 / v_cvt_pk_fp8_f32 on two of a word's four codes; to nearest even, values the type does not reach become NaN
+inline float emul_fp8_to_f32(uint8_t c) {
+    const int e = (c >> 3) & 15, m = c & 7;
+    const float v = e == 15 && m == 7 ? NAN : e ? std::ldexp(1.f + m / 8.f, e - 7) : std::ldexp((float)m, -9);
+    return c & 0x80 ? -v : v;
+}
+inline uint8_t emul_f32_to_fp8(float f) {
+    const uint8_t sign = std::signbit(f) ? 0x80 : 0;
+    const float a = std::fabs(f);
+    if (std::isnan(f) || a >= 480.f) return sign | 0x7f;
+    if (a == 0.f) return sign;
+    const int e = std::max(-6, std::ilogb(a));
+    int q = (int)std::nearbyint(std::ldexp(a, 3 - e));  // eighths of 2^e, 16 where it rounds up to the next power of two
+    const int code = (e == -6 && q < 8) ? q : ((e + 7) << 3) + (q - 8);
+    return code >= 0x7f ? (uint8_t)(sign | 0x7f) : (uint8_t)(sign | code);
+}
+inline emul::vec<float, 2> __builtin_amdgcn_cvt_pk_f32_fp8(int w, bool hi) {
+    const uint32_t u = (uint32_t)w >> (hi ? 16 : 0);
+    return emul::vec<float, 2>{{emul_fp8_to_f32((uint8_t)u), emul_fp8_to_f32((uint8_t)(u >> 8))}};
+}
+inline int __builtin_amdgcn_cvt_pk_fp8_f32(float a, float b, int old, bool hi) {
+    const uint32_t two = emul_f32_to_fp8(a) | (uint32_t)emul_f32_to_fp8(b) << 8;
+    return (int)(hi ? ((uint32_t)old & 0xffffu) | two << 16 : ((uint32_t)old & 0xffff0000u) | two);
+}
 inline unsigned long long __builtin_amdgcn_ballot_w64(bool pred) { return __ballot(pred ? 1 : 0); }
 inline void __builtin_amdgcn_wave_barrier() { emul::wave_barrier(); }
 inline void __builtin_amdgcn_s_sleep(int) {}  // (workgroups run one after another: what a spin waits for has already happened)
