@@ -11,115 +11,185 @@
 //
 // (m, log l) are kept apart because their sum can lose log l: a list whose entries all carry the type's lowest value as bias has m = -3.4e38.
 //
-// One wave per work item (a list, or 256 entries of a long one).  A head's row is spread over LPH lanes, 16 bytes each; the wave's 64 / LPH lane groups
-// are hp heads (the power of two that covers them) times as many entries in flight side by side as are left, each lane group with its own running maximum, sum
-// and accumulator, joined by shuffles at the end.  Parts of a long list are written as partial results and joined by a second launch in order.
+// A work item is a list, or a part of a long one.  A head's row is spread over LPH lanes, 16 bytes each; hp heads (the power of two that covers them, or
+// what a wave holds) make a slot, and every slot of a wave walks an item of its own: most lists have a handful of entries, and what bounds
+// them is how many dependent loads (item -> row number -> row) are in flight.  UN entries are loaded at a time, the next ones' numbers while these are
+// computed.  Parts of a long list are written as partial results and joined by a second launch in order.
 // Bound by the gather of rows: 2 rows per entry in each of the three sweeps.
 #include "row_types.h"
 
 namespace marius {
 
-constexpr float LOG2E = 1.4426950408889634f, NA_INF = __builtin_inff();
+constexpr float NA_INF = __builtin_inff();
 constexpr int NA_WAVES = 4;
 
 struct NaArgs {
     const void *q, *k, *v, *go;
     int64_t q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, go_ld, go_hd;   // row and head strides, elements
     const float* bias;                                          // [T, H] or NULL
-    float *out_bias, *stats, *delta, *part;
+    float *out_bias, *stats, *part;
+    float4* rowstats;                                           // [n, H]: m, log l, delta of a target's list, for the sweep over the rows' lists
     void *out, *dk, *dv;                                        // contiguous [n, H, D], [rows, Hkv, D]
     const int32_t *index, *owner, *entry;                       // forward lists: index; reverse lists: owner, entry (position in the forward lists)
     const int4 *items, *splits;
-    int n_items, n_splits, H, Hkv, D, hp;                       // hp: heads per wave
+    int n_items, n_splits, H, Hkv, D, hp;                       // hp: heads per slot
     float scale;
 };
 
+// sum over the LPH lanes of a head: neighbours within a row of 16 lanes by data-parallel moves, further ones by shuffles
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+    int w;
+    __builtin_memcpy(&w, &v, 4);
+    w = __builtin_amdgcn_update_dpp(0, w, CTRL, 0xf, 0xf, true);
+    float o;
+    __builtin_memcpy(&o, &w, 4);
+    return v + o;
+}
 template <int LPH>
 __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-    for (int o = LPH >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if (LPH >= 2) v = dpp_add<0xB1>(v);    // lane ^ 1
+    if (LPH >= 4) v = dpp_add<0x4E>(v);    // lane ^ 2
+    if (LPH >= 8) v = dpp_add<0x141>(v);   // the other half of 8 lanes (mirrored: its four lanes hold one value)
+    if (LPH >= 16) v = dpp_add<0x140>(v);  // the other half of 16 lanes
+    if (LPH >= 32) v += __shfl_xor(v, 16, 64);
+    if (LPH >= 64) v += __shfl_xor(v, 32, 64);
     return v;
 }
-// `cur` and `other`: running (maximum, sum) pairs and their weights to a common maximum; a maximum of -inf has weight zero
-__device__ __forceinline__ float weight_to(float m, float top) { return m == -NA_INF ? 0.f : __expf(m - top); }
+
+// A lane's piece of a head's row: VEC elements from `at`.  Where the row is no multiple of VEC, the last lane's piece ends with the row and overlaps its
+// neighbour's (both compute and store the same there); lanes behind the row repeat the last piece.  `first` is the first element that is the lane's own
+// (VEC: none); leave_own keeps the others out of the sums over the row, both factors zero, so that no infinity of a neighbour's element turns into NaN.
+template <typename T, int VEC>
+struct Piece {
+    T t[VEC];
+    __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(t, p, sizeof(t)); }
+    __device__ __forceinline__ void get(float (&v)[VEC]) const {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = (float)t[e];
+    }
+};
+template <int VEC, int LPH>
+struct Place {
+    int at, first;
+    bool tail;  // (uniform: the row does not fill its lanes' pieces)
+    __device__ __forceinline__ Place(int l, int D) : at(l * VEC < D - VEC ? l * VEC : D - VEC), tail(D != LPH * VEC) {
+        first = l * VEC - at;
+        first = first > VEC ? VEC : first;
+    }
+    __device__ __forceinline__ void leave_own(float (&v)[VEC]) const {
+        if (!tail) return;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = e >= first ? v[e] : 0.f;
+    }
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void put(T* p, const float (&v)[VEC]) {
+    T t[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) t[e] = (T)v[e];
+    __builtin_memcpy(p, t, sizeof(t));
+}
+// weight of a running sum that goes from maximum m to `ref`; a maximum of -inf has weight zero
+__device__ __forceinline__ float weight_to(float m, float ref) { return m == -NA_INF ? 0.f : __expf(m - ref); }
+__device__ __forceinline__ float finite_ref(float m) { return m == -NA_INF ? 0.f : m; }
+
+// which item, head and piece a lane works on
+template <int VEC, int LPH>
+struct Lane {
+    int l, h, slot;
+    bool head;
+    __device__ __forceinline__ Lane(const NaArgs& A, int heads) {
+        const int lane = threadIdx.x & 63, g = lane / LPH, slots = 64 / (LPH * A.hp);
+        l = lane & (LPH - 1);
+        h = blockIdx.y * A.hp + (g & (A.hp - 1));
+        head = h < heads;
+        h = head ? h : heads - 1;
+        slot = (blockIdx.x * NA_WAVES + (threadIdx.x >> 6)) * slots + g / A.hp;
+    }
+};
+template <int UN>
+__device__ __forceinline__ void load_numbers(const int32_t* p, int (&v)[UN]) { __builtin_memcpy(v, p, sizeof(v)); }  // (lists end with UN spare entries)
 
 // ---------------------------------------------------------------------------------------------------------------- forward
-template <typename T, int LPH, bool BIAS>
+template <typename T, int VEC, int LPH, bool BIAS>
 __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_kernel(NaArgs A) {
-    constexpr int VEC = 16 / sizeof(T), UN = 4;
-    const int lane = threadIdx.x & 63, item = blockIdx.x * NA_WAVES + (threadIdx.x >> 6);
-    if (item >= A.n_items) return;
-    const int4 it = A.items[item];
-    const int l = lane & (LPH - 1), g = lane / LPH, hp = A.hp, ES = 64 / (LPH * hp), es = g / hp, h = blockIdx.y * hp + (g & (hp - 1));
-    const bool head = h < A.H;
-    const int hc = head ? h : A.H - 1, kv = hc / (A.H / A.Hkv), c = l * VEC;
-    float q[VEC], acc[VEC], m = -NA_INF, sum = 0.f;
-    piece_load<T, VEC>((const T*)A.q + (int64_t)it.x * A.q_ld + hc * A.q_hd, c, A.D, q);
+    constexpr int UN = 4;
+    const Lane<VEC, LPH> w(A, A.H);
+    if (w.slot >= A.n_items || !w.head) return;
+    const int4 it = A.items[w.slot];
+    const Place<VEC, LPH> at(w.l, A.D);
+    const int kv = w.h / (A.H / A.Hkv);
+    float q[VEC], acc[VEC], m = -NA_INF, sum = 0.f, bias[UN];
+    Piece<T, VEC> raw;
+    raw.load((const T*)A.q + (int64_t)it.x * A.q_ld + w.h * A.q_hd + at.at);
+    raw.get(q);
+    at.leave_own(q);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
         q[e] *= A.scale;
         acc[e] = 0.f;
     }
-    const T *kp = (const T*)A.k + kv * A.k_hd, *vp = (const T*)A.v + kv * A.v_hd;
-    for (int b = it.y; b < it.z; b += 64) {
-        const int mine = b + lane < it.z ? A.index[b + lane] : 0;
-        const int end = it.z - b < 64 ? it.z - b : 64;
-        for (int t = 0; t < end; t += ES * UN) {
-            float kk[UN][VEC], vv[UN][VEC], s[UN];
-            bool ok[UN];
+    const T *kp = (const T*)A.k + kv * A.k_hd + at.at, *vp = (const T*)A.v + kv * A.v_hd + at.at;
+    int next[UN];
+    load_numbers<UN>(A.index + it.y, next);
+    if (BIAS)
 #pragma unroll
-            for (int u = 0; u < UN; ++u) {
-                const int at = t + u * ES + es;
-                const int64_t j = __shfl(mine, at & 63, 64);
-                ok[u] = at < end;
-                float bias = 0.f;
-                if (BIAS && ok[u]) bias = A.bias[(int64_t)(b + at) * A.H + hc];
-                if (BIAS && bias == -NA_INF) ok[u] = false;
-                s[u] = bias;
+        for (int u = 0; u < UN; ++u) bias[u] = it.y + u < it.z ? A.bias[(int64_t)(it.y + u) * A.H + w.h] : -NA_INF;
+    for (int t = it.y; t < it.z; t += UN) {
+        Piece<T, VEC> kk[UN], vv[UN];
+        float s[UN];
+        bool ok[UN];
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) kk[u][e] = vv[u][e] = 0.f;
-                if (ok[u]) {
-                    piece_load<T, VEC>(kp + j * A.k_ld, c, A.D, kk[u]);
-                    piece_load<T, VEC>(vp + j * A.v_ld, c, A.D, vv[u]);
-                }
-            }
-            float top = m;
-#pragma unroll
-            for (int u = 0; u < UN; ++u) {
-                float d = 0.f;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) d += q[e] * kk[u][e];
-                d = group_sum<LPH>(d);
-                s[u] = ok[u] ? d + s[u] : -NA_INF;
-                top = fmaxf(top, s[u]);
-            }
-            const float ref = top == -NA_INF ? 0.f : top, w = weight_to(m, ref);
-            m = top;
-            sum *= w;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] *= w;
-#pragma unroll
-            for (int u = 0; u < UN; ++u) {
-                const float p = __expf(s[u] - ref);
-                sum += p;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) acc[e] += p * vv[u][e];
+        for (int u = 0; u < UN; ++u) {
+            ok[u] = t + u < it.z;
+            const int64_t j = ok[u] ? next[u] : next[0];  // (behind the list: its last rows once more, computed on by nobody)
+            kk[u].load(kp + j * A.k_ld);
+            vv[u].load(vp + j * A.v_ld);
+            s[u] = 0.f;
+            if (BIAS) {
+                s[u] = bias[u];
+                ok[u] = bias[u] != -NA_INF;
             }
         }
-    }
-    for (int o = LPH * hp; o < 64; o <<= 1) {  // the entries side by side
-        const float om = __shfl_xor(m, o, 64), os = __shfl_xor(sum, o, 64), top = fmaxf(m, om), ref = top == -NA_INF ? 0.f : top;
-        const float w = weight_to(m, ref), ow = weight_to(om, ref);
-        sum = sum * w + os * ow;
+        if (t + UN < it.z) {
+            load_numbers<UN>(A.index + t + UN, next);
+            if (BIAS)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] = acc[e] * w + __shfl_xor(acc[e], o, 64) * ow;
+                for (int u = 0; u < UN; ++u) bias[u] = t + UN + u < it.z ? A.bias[(int64_t)(t + UN + u) * A.H + w.h] : -NA_INF;
+        }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            float k[VEC], d = 0.f;
+            kk[u].get(k);
+            at.leave_own(k);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) d += q[e] * k[e];
+            d = group_sum<LPH>(d);
+            s[u] = ok[u] ? d + s[u] : -NA_INF;
+            top = fmaxf(top, s[u]);
+        }
+        const float ref = finite_ref(top), scale = weight_to(m, ref);
         m = top;
+        sum *= scale;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] *= scale;
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            if (!ok[u]) continue;
+            const float p = __expf(s[u] - ref);
+            sum += p;
+            float v[VEC];
+            vv[u].get(v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] += p * v[e];
+        }
     }
-    if (es != 0 || !head) return;
     if (it.w >= 0) {
-        float* part = A.part + (int64_t)it.w * A.H * (A.D + 2) + (int64_t)h * (A.D + 2);
-        piece_store<float, VEC>(part + 2, c, A.D, acc);
-        if (l == 0) {
+        float* part = A.part + ((int64_t)it.w * A.H + w.h) * (A.D + 2);
+        put<float, VEC>(part + 2 + at.at, acc);
+        if (w.l == 0) {
             part[0] = m;
             part[1] = sum;
         }
@@ -127,30 +197,31 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_kernel(NaArgs A) 
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // (NaN stays)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] *= inv;
-        piece_store<T, VEC>((T*)A.out + ((int64_t)it.x * A.H + h) * A.D, c, A.D, acc);
-        if (l == 0) {
-            A.stats[((int64_t)it.x * A.H + h) * 2] = m;
-            A.stats[((int64_t)it.x * A.H + h) * 2 + 1] = sum == 0.f ? 0.f : logf(sum);
+        const int64_t o = (int64_t)it.x * A.H + w.h;
+        put<T, VEC>((T*)A.out + o * A.D + at.at, acc);
+        if (w.l == 0) {
+            A.stats[o * 2] = m;
+            A.stats[o * 2 + 1] = sum == 0.f ? 0.f : logf(sum);
         }
     }
 }
 
 // the parts of a long list, in order
-template <typename T, int LPH>
+template <typename T, int VEC, int LPH>
 __global__ __launch_bounds__(64) void nbr_attention_join_kernel(NaArgs A) {
-    constexpr int VEC = 16 / sizeof(T);
     const int4 sp = A.splits[blockIdx.x];
-    const int l = threadIdx.x & (LPH - 1), h = blockIdx.y * (64 / LPH) + threadIdx.x / LPH, c = l * VEC;
+    const int h = blockIdx.y * (64 / LPH) + threadIdx.x / LPH;
+    const Place<VEC, LPH> at(threadIdx.x & (LPH - 1), A.D);
     if (h >= A.H) return;
     float acc[VEC], m = -NA_INF, sum = 0.f;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
     for (int s = 0; s < sp.z; ++s) {
-        const float* part = A.part + (int64_t)(sp.y + s) * A.H * (A.D + 2) + (int64_t)h * (A.D + 2);
+        const float* part = A.part + ((int64_t)(sp.y + s) * A.H + h) * (A.D + 2);
         float v[VEC];
-        const float om = part[0], os = part[1], top = fmaxf(m, om), ref = top == -NA_INF ? 0.f : top;
+        const float om = part[0], os = part[1], top = fmaxf(m, om), ref = finite_ref(top);
         const float w = weight_to(m, ref), ow = weight_to(om, ref);
-        piece_load<float, VEC>(part + 2, c, A.D, v);
+        __builtin_memcpy(v, part + 2 + at.at, sizeof(v));
         sum = sum * w + os * ow;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] = acc[e] * w + v[e] * ow;
@@ -159,107 +230,119 @@ __global__ __launch_bounds__(64) void nbr_attention_join_kernel(NaArgs A) {
     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] *= inv;
-    piece_store<T, VEC>((T*)A.out + ((int64_t)sp.x * A.H + h) * A.D, c, A.D, acc);
-    if (l == 0) {
-        A.stats[((int64_t)sp.x * A.H + h) * 2] = m;
-        A.stats[((int64_t)sp.x * A.H + h) * 2 + 1] = sum == 0.f ? 0.f : logf(sum);
+    const int64_t o = (int64_t)sp.x * A.H + h;
+    put<T, VEC>((T*)A.out + o * A.D + at.at, acc);
+    if ((threadIdx.x & (LPH - 1)) == 0) {
+        A.stats[o * 2] = m;
+        A.stats[o * 2 + 1] = sum == 0.f ? 0.f : logf(sum);
     }
 }
 
 // p from a score and its list's (m, log l); a list without a live entry has m = -inf
-__device__ __forceinline__ float probability(float s, float m, float logl) { return __expf((s - (m == -NA_INF ? 0.f : m)) - logl); }
+__device__ __forceinline__ float probability(float s, float m, float logl) { return __expf((s - finite_ref(m)) - logl); }
+
+// dq = scale (sum p d k - delta sum p k): two roundings, not a fused one, so that a list of one entry gives exactly zero
+template <int VEC>
+__device__ __forceinline__ void dq_of(float (&pdk)[VEC], const float (&pk)[VEC], float delta, float scale) {
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) pdk[e] = scale * (pdk[e] - delta * pk[e]);
+}
 
 // ---------------------------------------------------------------------------------------------------------------- backward over the targets' lists: dq, delta
-template <typename T, int LPH, bool BIAS>
+template <typename T, int VEC, int LPH, bool BIAS>
 __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dq_kernel(NaArgs A) {
-    constexpr int VEC = 16 / sizeof(T), UN = 4;
-    const int lane = threadIdx.x & 63, item = blockIdx.x * NA_WAVES + (threadIdx.x >> 6);
-    if (item >= A.n_items) return;
-    const int4 it = A.items[item];
-    const int l = lane & (LPH - 1), g = lane / LPH, hp = A.hp, ES = 64 / (LPH * hp), es = g / hp, h = blockIdx.y * hp + (g & (hp - 1));
-    const bool head = h < A.H;
-    const int hc = head ? h : A.H - 1, kv = hc / (A.H / A.Hkv), c = l * VEC;
-    float q[VEC], go[VEC], pdk[VEC], pk[VEC], delta = 0.f;
-    piece_load<T, VEC>((const T*)A.q + (int64_t)it.x * A.q_ld + hc * A.q_hd, c, A.D, q);
-    piece_load<T, VEC>((const T*)A.go + (int64_t)it.x * A.go_ld + hc * A.go_hd, c, A.D, go);
-    const float m = A.stats[((int64_t)it.x * A.H + hc) * 2], logl = A.stats[((int64_t)it.x * A.H + hc) * 2 + 1];
+    constexpr int UN = 4;
+    const Lane<VEC, LPH> w(A, A.H);
+    if (w.slot >= A.n_items || !w.head) return;
+    const int4 it = A.items[w.slot];
+    const Place<VEC, LPH> at(w.l, A.D);
+    const int kv = w.h / (A.H / A.Hkv);
+    const int64_t o = (int64_t)it.x * A.H + w.h;
+    float q[VEC], go[VEC], pdk[VEC], pk[VEC], delta = 0.f, bias[UN];
+    Piece<T, VEC> raw, raw2;
+    raw.load((const T*)A.q + (int64_t)it.x * A.q_ld + w.h * A.q_hd + at.at);
+    raw2.load((const T*)A.go + (int64_t)it.x * A.go_ld + w.h * A.go_hd + at.at);
+    const float m = A.stats[o * 2], logl = A.stats[o * 2 + 1];
+    raw.get(q);
+    raw2.get(go);
+    at.leave_own(q);
+    at.leave_own(go);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
         q[e] *= A.scale;
         pdk[e] = pk[e] = 0.f;
     }
-    const T *kp = (const T*)A.k + kv * A.k_hd, *vp = (const T*)A.v + kv * A.v_hd;
-    for (int b = it.y; b < it.z; b += 64) {
-        const int mine = b + lane < it.z ? A.index[b + lane] : 0;
-        const int end = it.z - b < 64 ? it.z - b : 64;
-        for (int t = 0; t < end; t += ES * UN) {
-            float kk[UN][VEC], vv[UN][VEC], bias[UN];
-            bool ok[UN];
+    const T *kp = (const T*)A.k + kv * A.k_hd + at.at, *vp = (const T*)A.v + kv * A.v_hd + at.at;
+    int next[UN];
+    load_numbers<UN>(A.index + it.y, next);
+    if (BIAS)
 #pragma unroll
-            for (int u = 0; u < UN; ++u) {
-                const int at = t + u * ES + es;
-                const int64_t j = __shfl(mine, at & 63, 64);
-                ok[u] = at < end;
-                bias[u] = 0.f;
-                if (BIAS && ok[u]) bias[u] = A.bias[(int64_t)(b + at) * A.H + hc];
-                if (BIAS && bias[u] == -NA_INF) ok[u] = false;
+        for (int u = 0; u < UN; ++u) bias[u] = it.y + u < it.z ? A.bias[(int64_t)(it.y + u) * A.H + w.h] : -NA_INF;
+    for (int t = it.y; t < it.z; t += UN) {
+        Piece<T, VEC> kk[UN], vv[UN];
+        float b[UN];
+        bool ok[UN];
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) kk[u][e] = vv[u][e] = 0.f;
-                if (ok[u]) {
-                    piece_load<T, VEC>(kp + j * A.k_ld, c, A.D, kk[u]);
-                    piece_load<T, VEC>(vp + j * A.v_ld, c, A.D, vv[u]);
-                }
+        for (int u = 0; u < UN; ++u) {
+            ok[u] = t + u < it.z;
+            const int64_t j = ok[u] ? next[u] : next[0];
+            kk[u].load(kp + j * A.k_ld);
+            vv[u].load(vp + j * A.v_ld);
+            b[u] = 0.f;
+            if (BIAS) {
+                b[u] = bias[u];
+                ok[u] = bias[u] != -NA_INF;
             }
+        }
+        if (t + UN < it.z) {
+            load_numbers<UN>(A.index + t + UN, next);
+            if (BIAS)
 #pragma unroll
-            for (int u = 0; u < UN; ++u) {
-                float s = 0.f, d = 0.f;
+                for (int u = 0; u < UN; ++u) bias[u] = t + UN + u < it.z ? A.bias[(int64_t)(t + UN + u) * A.H + w.h] : -NA_INF;
+        }
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    s += q[e] * kk[u][e];
-                    d += go[e] * vv[u][e];
-                }
-                s = group_sum<LPH>(s) + bias[u];
-                d = group_sum<LPH>(d);
-                const float p = ok[u] ? probability(s, m, logl) : 0.f, pd = ok[u] ? p * d : 0.f;
-                delta += pd;
+        for (int u = 0; u < UN; ++u) {
+            if (!ok[u]) continue;
+            float k[VEC], own[VEC], v[VEC], s = 0.f, d = 0.f;
+            kk[u].get(k);
+            vv[u].get(v);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    pdk[e] += pd * kk[u][e];
-                    pk[e] += p * kk[u][e];
-                }
+            for (int e = 0; e < VEC; ++e) own[e] = k[e];
+            at.leave_own(own);
+            at.leave_own(v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                s += q[e] * own[e];
+                d += go[e] * v[e];
+            }
+            s = group_sum<LPH>(s) + b[u];
+            d = group_sum<LPH>(d);
+            const float p = probability(s, m, logl), pd = p * d;
+            delta += pd;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                pdk[e] += pd * k[e];
+                pk[e] += p * k[e];
             }
         }
     }
-    for (int o = LPH * hp; o < 64; o <<= 1) {
-        delta += __shfl_xor(delta, o, 64);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            pdk[e] += __shfl_xor(pdk[e], o, 64);
-            pk[e] += __shfl_xor(pk[e], o, 64);
-        }
-    }
-    if (es != 0 || !head) return;
     if (it.w >= 0) {
-        float* part = A.part + ((int64_t)it.w * A.H + h) * (2 * A.D + 1);
-        piece_store<float, VEC>(part + 1, c, A.D, pdk);
-        piece_store<float, VEC>(part + 1 + A.D, c, A.D, pk);
-        if (l == 0) part[0] = delta;
+        float* part = A.part + ((int64_t)it.w * A.H + w.h) * (2 * A.D + 1);
+        put<float, VEC>(part + 1 + at.at, pdk);
+        put<float, VEC>(part + 1 + A.D + at.at, pk);
+        if (w.l == 0) part[0] = delta;
     } else {
-        // (two roundings, not a fused one: a list of one entry then gives exactly zero)
-        {
-#pragma clang fp contract(off)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) pdk[e] = A.scale * (pdk[e] - delta * pk[e]);
-        }
-        piece_store<T, VEC>((T*)A.out + ((int64_t)it.x * A.H + h) * A.D, c, A.D, pdk);
-        if (l == 0) A.delta[(int64_t)it.x * A.H + h] = delta;
+        dq_of<VEC>(pdk, pk, delta, A.scale);
+        put<T, VEC>((T*)A.out + o * A.D + at.at, pdk);
+        if (w.l == 0) A.rowstats[o] = make_float4(m, logl, delta, 0.f);
     }
 }
-template <typename T, int LPH>
+template <typename T, int VEC, int LPH>
 __global__ __launch_bounds__(64) void nbr_attention_dq_join_kernel(NaArgs A) {
-    constexpr int VEC = 16 / sizeof(T);
     const int4 sp = A.splits[blockIdx.x];
-    const int l = threadIdx.x & (LPH - 1), h = blockIdx.y * (64 / LPH) + threadIdx.x / LPH, c = l * VEC;
+    const int h = blockIdx.y * (64 / LPH) + threadIdx.x / LPH;
+    const Place<VEC, LPH> at(threadIdx.x & (LPH - 1), A.D);
     if (h >= A.H) return;
     float pdk[VEC], pk[VEC], delta = 0.f;
 #pragma unroll
@@ -267,8 +350,8 @@ __global__ __launch_bounds__(64) void nbr_attention_dq_join_kernel(NaArgs A) {
     for (int s = 0; s < sp.z; ++s) {
         const float* part = A.part + ((int64_t)(sp.y + s) * A.H + h) * (2 * A.D + 1);
         float a[VEC], b[VEC];
-        piece_load<float, VEC>(part + 1, c, A.D, a);
-        piece_load<float, VEC>(part + 1 + A.D, c, A.D, b);
+        __builtin_memcpy(a, part + 1 + at.at, sizeof(a));
+        __builtin_memcpy(b, part + 1 + A.D + at.at, sizeof(b));
         delta += part[0];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
@@ -276,105 +359,111 @@ __global__ __launch_bounds__(64) void nbr_attention_dq_join_kernel(NaArgs A) {
             pk[e] += b[e];
         }
     }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) pdk[e] = A.scale * (pdk[e] - delta * pk[e]);
-    piece_store<T, VEC>((T*)A.out + ((int64_t)sp.x * A.H + h) * A.D, c, A.D, pdk);
-    if (l == 0) A.delta[(int64_t)sp.x * A.H + h] = delta;
+    dq_of<VEC>(pdk, pk, delta, A.scale);
+    const int64_t o = (int64_t)sp.x * A.H + h;
+    put<T, VEC>((T*)A.out + o * A.D + at.at, pdk);
+    if ((threadIdx.x & (LPH - 1)) == 0) A.rowstats[o] = make_float4(A.stats[o * 2], A.stats[o * 2 + 1], delta, 0.f);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- backward over the rows' lists: dk, dv, db
-template <typename T, int LPH, bool BIAS>
+template <typename T, int VEC, int LPH, bool BIAS>
 __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dkv_kernel(NaArgs A) {
-    constexpr int VEC = 16 / sizeof(T), UN = 4;
-    const int lane = threadIdx.x & 63, item = blockIdx.x * NA_WAVES + (threadIdx.x >> 6);
-    if (item >= A.n_items) return;
-    const int4 it = A.items[item];
-    const int l = lane & (LPH - 1), g = lane / LPH, hp = A.hp, ES = 64 / (LPH * hp), es = g / hp, kv = blockIdx.y * hp + (g & (hp - 1)), R = A.H / A.Hkv;
-    const bool head = kv < A.Hkv;
-    const int kc = head ? kv : A.Hkv - 1, c = l * VEC;
+    constexpr int UN = 2;
+    const Lane<VEC, LPH> w(A, A.Hkv);
+    if (w.slot >= A.n_items || !w.head) return;
+    const int4 it = A.items[w.slot];
+    const Place<VEC, LPH> at(w.l, A.D);
+    const int R = A.H / A.Hkv;
     float k[VEC], v[VEC], dk[VEC], dv[VEC];
-    piece_load<T, VEC>((const T*)A.k + (int64_t)it.x * A.k_ld + kc * A.k_hd, c, A.D, k);
-    piece_load<T, VEC>((const T*)A.v + (int64_t)it.x * A.v_ld + kc * A.v_hd, c, A.D, v);
+    Piece<T, VEC> raw, raw2;
+    raw.load((const T*)A.k + (int64_t)it.x * A.k_ld + w.h * A.k_hd + at.at);
+    raw2.load((const T*)A.v + (int64_t)it.x * A.v_ld + w.h * A.v_hd + at.at);
+    int next[UN], next_e[UN];
+    load_numbers<UN>(A.owner + it.y, next);
+    if (BIAS) load_numbers<UN>(A.entry + it.y, next_e);
+    raw.get(k);
+    raw2.get(v);
+    at.leave_own(k);
+    at.leave_own(v);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
         k[e] *= A.scale;
         dk[e] = dv[e] = 0.f;
     }
-    for (int b = it.y; b < it.z; b += 64) {
-        const int mine = b + lane < it.z ? A.owner[b + lane] : 0, mine_e = BIAS && b + lane < it.z ? A.entry[b + lane] : 0;
-        const int end = it.z - b < 64 ? it.z - b : 64;
-        for (int t = 0; t < end; t += ES * UN) {
-            for (int r = 0; r < R; ++r) {
-                const int h = kc * R + r;
-                float qq[UN][VEC], go[UN][VEC], m[UN], logl[UN], delta[UN], bias[UN];
-                bool ok[UN];
+    for (int t = it.y; t < it.z; t += UN) {
+        int64_t i[UN], e_at[UN];
+        bool in[UN];
 #pragma unroll
-                for (int u = 0; u < UN; ++u) {
-                    const int at = t + u * ES + es;
-                    const int64_t i = __shfl(mine, at & 63, 64), e_at = BIAS ? __shfl(mine_e, at & 63, 64) : 0;
-                    ok[u] = at < end;
-                    bias[u] = 0.f;
-                    if (BIAS && ok[u]) bias[u] = A.bias[e_at * A.H + h];
-                    if (BIAS && bias[u] == -NA_INF) ok[u] = false;
-                    m[u] = logl[u] = delta[u] = 0.f;
+        for (int u = 0; u < UN; ++u) {
+            in[u] = t + u < it.z;
+            i[u] = in[u] ? next[u] : next[0];
+            e_at[u] = BIAS ? (in[u] ? next_e[u] : next_e[0]) : 0;
+        }
+        if (t + UN < it.z) {
+            load_numbers<UN>(A.owner + t + UN, next);
+            if (BIAS) load_numbers<UN>(A.entry + t + UN, next_e);
+        }
+        for (int r = 0; r < R; ++r) {
+            const int h = w.h * R + r;
+            Piece<T, VEC> qq[UN], gg[UN];
+            float4 st[UN];
+            float bias[UN];
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) qq[u][e] = go[u][e] = 0.f;
-                    if (ok[u]) {
-                        piece_load<T, VEC>((const T*)A.q + i * A.q_ld + h * A.q_hd, c, A.D, qq[u]);
-                        piece_load<T, VEC>((const T*)A.go + i * A.go_ld + h * A.go_hd, c, A.D, go[u]);
-                        m[u] = A.stats[(i * A.H + h) * 2];
-                        logl[u] = A.stats[(i * A.H + h) * 2 + 1];
-                        delta[u] = A.delta[i * A.H + h];
-                    }
+            for (int u = 0; u < UN; ++u) {
+                st[u] = A.rowstats[i[u] * A.H + h];
+                bias[u] = BIAS ? A.bias[e_at[u] * A.H + h] : 0.f;
+                qq[u].load((const T*)A.q + i[u] * A.q_ld + h * A.q_hd + at.at);
+                gg[u].load((const T*)A.go + i[u] * A.go_ld + h * A.go_hd + at.at);
+            }
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                if (!in[u]) continue;
+                float q[VEC], g[VEC], oq[VEC], og[VEC], s = 0.f, d = 0.f;
+                qq[u].get(q);
+                gg[u].get(g);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    oq[e] = q[e];
+                    og[e] = g[e];
                 }
+                at.leave_own(oq);
+                at.leave_own(og);
+                const bool live = !BIAS || bias[u] != -NA_INF;
 #pragma unroll
-                for (int u = 0; u < UN; ++u) {
-                    float s = 0.f, d = 0.f;
+                for (int e = 0; e < VEC; ++e) {
+                    s += oq[e] * k[e];
+                    d += og[e] * v[e];
+                }
+                s = group_sum<LPH>(s) + bias[u];
+                d = group_sum<LPH>(d);
+                const float p = live ? probability(s, st[u].x, st[u].y) : 0.f, ds = live ? p * (d - st[u].z) : 0.f;
+                if (BIAS && A.out_bias && w.l == 0) A.out_bias[e_at[u] * A.H + h] = ds;
+                if (!live) continue;
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        s += qq[u][e] * k[e];
-                        d += go[u][e] * v[e];
-                    }
-                    s = group_sum<LPH>(s) + bias[u];
-                    d = group_sum<LPH>(d);
-                    const float p = ok[u] ? probability(s, m[u], logl[u]) : 0.f, ds = ok[u] ? p * (d - delta[u]) : 0.f;
-                    if (BIAS) {
-                        const int at = t + u * ES + es;
-                        const int64_t e_at = __shfl(mine_e, at & 63, 64);
-                        if (A.out_bias && l == 0 && head && at < end) A.out_bias[e_at * A.H + h] = ds;
-                    }
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        dk[e] += ds * qq[u][e];
-                        dv[e] += p * go[u][e];
-                    }
+                for (int e = 0; e < VEC; ++e) {
+                    dk[e] += ds * q[e];
+                    dv[e] += p * g[e];
                 }
             }
         }
     }
-    for (int o = LPH * hp; o < 64; o <<= 1)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            dk[e] += __shfl_xor(dk[e], o, 64);
-            dv[e] += __shfl_xor(dv[e], o, 64);
-        }
-    if (es != 0 || !head) return;
     if (it.w >= 0) {
-        float* part = A.part + ((int64_t)it.w * A.Hkv + kv) * 2 * A.D;
-        piece_store<float, VEC>(part, c, A.D, dk);
-        piece_store<float, VEC>(part + A.D, c, A.D, dv);
+        float* part = A.part + ((int64_t)it.w * A.Hkv + w.h) * 2 * A.D;
+        put<float, VEC>(part + at.at, dk);
+        put<float, VEC>(part + A.D + at.at, dv);
     } else {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) dk[e] *= A.scale;
-        piece_store<T, VEC>((T*)A.dk + ((int64_t)it.x * A.Hkv + kv) * A.D, c, A.D, dk);
-        piece_store<T, VEC>((T*)A.dv + ((int64_t)it.x * A.Hkv + kv) * A.D, c, A.D, dv);
+        const int64_t o = ((int64_t)it.x * A.Hkv + w.h) * A.D + at.at;
+        put<T, VEC>((T*)A.dk + o, dk);
+        put<T, VEC>((T*)A.dv + o, dv);
     }
 }
-template <typename T, int LPH>
+template <typename T, int VEC, int LPH>
 __global__ __launch_bounds__(64) void nbr_attention_dkv_join_kernel(NaArgs A) {
-    constexpr int VEC = 16 / sizeof(T);
     const int4 sp = A.splits[blockIdx.x];
-    const int l = threadIdx.x & (LPH - 1), h = blockIdx.y * (64 / LPH) + threadIdx.x / LPH, c = l * VEC;
+    const int h = blockIdx.y * (64 / LPH) + threadIdx.x / LPH;
+    const Place<VEC, LPH> at(threadIdx.x & (LPH - 1), A.D);
     if (h >= A.Hkv) return;
     float dk[VEC], dv[VEC];
 #pragma unroll
@@ -382,8 +471,8 @@ __global__ __launch_bounds__(64) void nbr_attention_dkv_join_kernel(NaArgs A) {
     for (int s = 0; s < sp.z; ++s) {
         const float* part = A.part + ((int64_t)(sp.y + s) * A.Hkv + h) * 2 * A.D;
         float a[VEC], b[VEC];
-        piece_load<float, VEC>(part, c, A.D, a);
-        piece_load<float, VEC>(part + A.D, c, A.D, b);
+        __builtin_memcpy(a, part + at.at, sizeof(a));
+        __builtin_memcpy(b, part + A.D + at.at, sizeof(b));
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             dk[e] += a[e];
@@ -392,43 +481,48 @@ __global__ __launch_bounds__(64) void nbr_attention_dkv_join_kernel(NaArgs A) {
     }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) dk[e] *= A.scale;
-    piece_store<T, VEC>((T*)A.dk + ((int64_t)sp.x * A.Hkv + h) * A.D, c, A.D, dk);
-    piece_store<T, VEC>((T*)A.dv + ((int64_t)sp.x * A.Hkv + h) * A.D, c, A.D, dv);
+    const int64_t o = ((int64_t)sp.x * A.Hkv + h) * A.D + at.at;
+    put<T, VEC>((T*)A.dk + o, dk);
+    put<T, VEC>((T*)A.dv + o, dv);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- launches
 enum NaPass { NA_FWD = 0, NA_DQ, NA_DKV };
 
-template <typename T, int LPH>
+template <typename T, int VEC, int LPH>
 static void na_launch(NaArgs A, NaPass pass, hipStream_t st) {
     const int heads = pass == NA_DKV ? A.Hkv : A.H, groups = 64 / LPH;
     A.hp = 1;
     while (A.hp < groups && A.hp < heads) A.hp <<= 1;
-    const dim3 grid((unsigned)cdiv(A.n_items, NA_WAVES), (unsigned)cdiv(heads, A.hp)), jgrid((unsigned)A.n_splits, (unsigned)cdiv(heads, groups));
+    const dim3 grid((unsigned)cdiv(A.n_items, NA_WAVES * (groups / A.hp)), (unsigned)cdiv(heads, A.hp)), jgrid((unsigned)A.n_splits, (unsigned)cdiv(heads, groups));
+    const dim3 block(64 * NA_WAVES);
     if (pass == NA_FWD) {
-        if (A.bias) nbr_attention_kernel<T, LPH, true><<<grid, dim3(64 * NA_WAVES), 0, st>>>(A);
-        else nbr_attention_kernel<T, LPH, false><<<grid, dim3(64 * NA_WAVES), 0, st>>>(A);
-        if (A.n_splits > 0) nbr_attention_join_kernel<T, LPH><<<jgrid, dim3(64), 0, st>>>(A);
+        if (A.bias) nbr_attention_kernel<T, VEC, LPH, true><<<grid, block, 0, st>>>(A);
+        else nbr_attention_kernel<T, VEC, LPH, false><<<grid, block, 0, st>>>(A);
+        if (A.n_splits > 0) nbr_attention_join_kernel<T, VEC, LPH><<<jgrid, dim3(64), 0, st>>>(A);
     } else if (pass == NA_DQ) {
-        if (A.bias) nbr_attention_dq_kernel<T, LPH, true><<<grid, dim3(64 * NA_WAVES), 0, st>>>(A);
-        else nbr_attention_dq_kernel<T, LPH, false><<<grid, dim3(64 * NA_WAVES), 0, st>>>(A);
-        if (A.n_splits > 0) nbr_attention_dq_join_kernel<T, LPH><<<jgrid, dim3(64), 0, st>>>(A);
+        if (A.bias) nbr_attention_dq_kernel<T, VEC, LPH, true><<<grid, block, 0, st>>>(A);
+        else nbr_attention_dq_kernel<T, VEC, LPH, false><<<grid, block, 0, st>>>(A);
+        if (A.n_splits > 0) nbr_attention_dq_join_kernel<T, VEC, LPH><<<jgrid, dim3(64), 0, st>>>(A);
     } else {
-        if (A.bias) nbr_attention_dkv_kernel<T, LPH, true><<<grid, dim3(64 * NA_WAVES), 0, st>>>(A);
-        else nbr_attention_dkv_kernel<T, LPH, false><<<grid, dim3(64 * NA_WAVES), 0, st>>>(A);
-        if (A.n_splits > 0) nbr_attention_dkv_join_kernel<T, LPH><<<jgrid, dim3(64), 0, st>>>(A);
+        if (A.bias) nbr_attention_dkv_kernel<T, VEC, LPH, true><<<grid, block, 0, st>>>(A);
+        else nbr_attention_dkv_kernel<T, VEC, LPH, false><<<grid, block, 0, st>>>(A);
+        if (A.n_splits > 0) nbr_attention_dkv_join_kernel<T, VEC, LPH><<<jgrid, dim3(64), 0, st>>>(A);
     }
 }
+// lanes per head: the power of two that covers its pieces of 16 bytes (heads shorter than one piece: an element per lane)
 template <typename T>
 static void na_launch_width(const NaArgs& A, NaPass pass, hipStream_t st) {
-    const int pieces = (int)cdiv(A.D, 16 / (int)sizeof(T));
-    if (pieces <= 1) na_launch<T, 1>(A, pass, st);
-    else if (pieces <= 2) na_launch<T, 2>(A, pass, st);
-    else if (pieces <= 4) na_launch<T, 4>(A, pass, st);
-    else if (pieces <= 8) na_launch<T, 8>(A, pass, st);
-    else if (pieces <= 16) na_launch<T, 16>(A, pass, st);
-    else if (pieces <= 32) na_launch<T, 32>(A, pass, st);
-    else na_launch<T, 64>(A, pass, st);
+    constexpr int VEC = 16 / (int)sizeof(T);
+    const int pieces = (int)cdiv(A.D, VEC);
+    if (A.D < VEC) na_launch<T, 1, VEC>(A, pass, st);
+    else if (pieces <= 1) na_launch<T, VEC, 1>(A, pass, st);
+    else if (pieces <= 2) na_launch<T, VEC, 2>(A, pass, st);
+    else if (pieces <= 4) na_launch<T, VEC, 4>(A, pass, st);
+    else if (pieces <= 8) na_launch<T, VEC, 8>(A, pass, st);
+    else if (pieces <= 16) na_launch<T, VEC, 16>(A, pass, st);
+    else if (pieces <= 32) na_launch<T, VEC, 32>(A, pass, st);
+    else na_launch<T, VEC, VEC == 4 ? 64 : 32>(A, pass, st);  // (256 elements of 16 bits are 32 pieces)
 }
 static void na_launch_typed(const NaArgs& A, int type, NaPass pass, hipStream_t st) {
     if (A.n_items == 0) return;
@@ -477,7 +571,7 @@ extern "C" size_t marius_neighbor_attention_workspace_bytes(const marius_neighbo
     if (!P || heads <= 0 || kv_heads <= 0 || dim <= 0) return 0;
     if (!backward) return (size_t)P->n_slots * heads * (dim + 2) * sizeof(float);
     const size_t dq = (size_t)P->n_slots * heads * (2 * dim + 1), dkv = (size_t)P->r_n_slots * kv_heads * 2 * dim;
-    return ((size_t)P->n * heads + (dq > dkv ? dq : dkv)) * sizeof(float);
+    return (size_t)P->n * heads * sizeof(float4) + (dq > dkv ? dq : dkv) * sizeof(float);
 }
 
 extern "C" int marius_neighbor_attention_forward(const marius_neighbor_plan* P, const marius_neighbor_attention* m, void* out, void* workspace, size_t workspace_bytes,
@@ -510,8 +604,8 @@ extern "C" int marius_neighbor_attention_backward(const marius_neighbor_plan* P,
     A.go = grad_out;
     A.go_ld = grad_row;
     A.go_hd = grad_head;
-    A.delta = (float*)workspace;
-    A.part = A.delta + (size_t)P->n * A.H;
+    A.rowstats = (float4*)workspace;
+    A.part = (float*)(A.rowstats + (size_t)P->n * A.H);
     A.out = dq;
     na_launch_typed(A, m->type, NA_DQ, st);
     A.dk = dk;

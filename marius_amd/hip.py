@@ -855,7 +855,10 @@ def residual_norm_backward(grad_y, grad_h, y, block=None, gate=None, post_weight
     return got
 
 
-PLAN_CHUNK = 256  # entries of a work item
+def plan_chunk(entries):
+    """entries of a work item: 256 (few partial results), down to 32 where a plan has few entries (a served request with long lists: 4096 items fill the card)"""
+    return min(256, max(32, entries // 4096))
+
 
 
 class NeighborPlan:
@@ -878,37 +881,40 @@ class NeighborPlan:
         total = ta + tb + (n if own >= 0 else 0)
         lists = [t.contiguous() for t in lists] + [None] * (4 - len(lists))
         i32 = dict(dtype=torch.int32, device=dev)
-        offs, self.index, owner = torch.zeros(n + 1, **i32), torch.empty(total, **i32), torch.empty(total, **i32)
+        spare = 4  # (the attention reads the lists four entries at a time)
+        offs, self._index, owner = torch.zeros(n + 1, **i32), torch.empty(total + spare, **i32), torch.empty(total, **i32)
         keys, status = torch.empty(total, dtype=torch.int64, device=dev), torch.zeros(4, **i32)
         L = lib()
         with _on(index):
             wsb = max(L.marius_nbr_plan_workspace_bytes(n), L.marius_nbr_plan_workspace_bytes(num_rows))
             ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-            check(L.marius_nbr_plan_lists(ptr(lists[0]), ptr(lists[1]), ta, ptr(lists[2]), ptr(lists[3]), tb, n, num_rows, own, ptr(offs), ptr(self.index), ptr(owner),
+            check(L.marius_nbr_plan_lists(ptr(lists[0]), ptr(lists[1]), ta, ptr(lists[2]), ptr(lists[3]), tb, n, num_rows, own, ptr(offs), ptr(self._index), ptr(owner),
                                           ptr(keys), ptr(status), ptr(ws), wsb, stream_ptr()), "nbr_plan_lists")
             bad = int(status[0])
             _require(not bad & 1, "NeighborPlan: offsets have to ascend from 0 to the end of their list")
             _require(not bad & 2, "NeighborPlan: an index lies outside the %d rows", num_rows)
-            r_offs, self._r_owner, self._r_entry = torch.empty(num_rows + 1, **i32), torch.empty(total, **i32), torch.empty(0, **i32)
-            um = UniqueMap(max(total, 1), dev)
+            r_offs, self._r_owner, self._r_entry = torch.empty(num_rows + 1, **i32), torch.empty(total + spare, **i32), None
+            um = UniqueMap(total + spare, dev)
             if total > 0:
                 um.run(keys, max(1, (num_rows - 1).bit_length()))
-                self._r_entry = um.perm
+            self._r_entry = um.perm
             check(L.marius_nbr_plan_reverse(ptr(um.uniq), ptr(um.seg), ptr(um.count), ptr(um.perm), ptr(owner), total, num_rows, ptr(r_offs), ptr(self._r_owner), stream_ptr()),
                   "nbr_plan_reverse")
-            more = total // PLAN_CHUNK
+            chunk = plan_chunk(total)
+            more = total // chunk
             totals = torch.zeros(2, 4, **i32)
             made = []
             for k, (o, m) in enumerate(((offs, n), (r_offs, num_rows))):
                 items, splits = torch.empty((m + more, 4), **i32), torch.empty((more, 4), **i32)
-                check(L.marius_nbr_plan_items(ptr(o), m, PLAN_CHUNK, ptr(items), m + more, ptr(splits), more, ptr(totals[k]), ptr(ws), wsb, stream_ptr()), "nbr_plan_items")
+                check(L.marius_nbr_plan_items(ptr(o), m, chunk, ptr(items), m + more, ptr(splits), more, ptr(totals[k]), ptr(ws), wsb, stream_ptr()), "nbr_plan_items")
                 made += [items, splits]
             counts = totals.tolist()
         self._items, self._splits, self._r_items, self._r_splits = made
         self.n, self.num_rows, self.num_entries, self.device, self.owner, self.offsets = n, num_rows, total, dev, owner, offs
+        self.index = self._index[:total]
         self.desc = NeighborPlanDesc(n=n, rows=num_rows, T=total)
         d = self.desc
-        d.index, d.items, d.splits, d.r_owner, d.r_entry, d.r_items, d.r_splits = (t.data_ptr() for t in (self.index, self._items, self._splits, self._r_owner, self._r_entry,
+        d.index, d.items, d.splits, d.r_owner, d.r_entry, d.r_items, d.r_splits = (t.data_ptr() for t in (self._index, self._items, self._splits, self._r_owner, self._r_entry,
                                                                                                         self._r_items, self._r_splits))
         (d.n_items, d.n_slots, d.n_splits, _), (d.r_n_items, d.r_n_slots, d.r_n_splits, _) = counts
         self._starts, self._ends, self._own = (lists[1], lists[3]), (ta, tb), own >= 0

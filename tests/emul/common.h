@@ -368,6 +368,13 @@ inline emul::vec<float, 16> __builtin_amdgcn_mfma_f32_32x32x2f32(float a, float 
     emul::wave_barrier();
     return c;
 }
+// data-parallel moves within a row of 16 lanes: quad permutations, mirrors of 8 and of 16 lanes
+inline int __builtin_amdgcn_update_dpp(int, int v, int ctrl, int, int, bool) {
+    return emul::exchange<int>(v, [](int lane, int c) {
+        if (c < 0x100) return (lane & ~3) | ((c >> (2 * (lane & 3))) & 3);
+        return c == 0x141 ? (lane & ~7) | (7 - (lane & 7)) : (lane & ~15) | (15 - (lane & 15));
+    }, ctrl);
+}
 // e4m3 (OCP): v_cvt_pk_f32_fp8 / v_cvt_pk_fp8_f32 on two of a word's four codes; to nearest even, values the type does not reach become NaN
 inline float emul_fp8_to_f32(uint8_t c) {
     const int e = (c >> 3) & 15, m = c & 7;
