@@ -28,68 +28,16 @@ struct NaArgs {
     int64_t q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, go_ld, go_hd;   // row and head strides, elements
     const float* bias;                                          // [T, H] or NULL
     float *out_bias, *stats, *part;
+    float2* part2;                                              // a part's (m, sum), or its delta
     float4* rowstats;                                           // [n, H]: m, log l, delta of a target's list, for the sweep over the rows' lists
     void *out, *dk, *dv;                                        // contiguous [n, H, D], [rows, Hkv, D]
     const int32_t *index, *owner, *entry;                       // forward lists: index; reverse lists: owner, entry (position in the forward lists)
     const int4 *items, *splits;
     int n_items, n_splits, H, Hkv, D, hp;                       // hp: heads per slot
+    bool dense;                                                 // items of more than two entries on average
     float scale;
 };
 
-// sum over the LPH lanes of a head: neighbours within a row of 16 lanes by data-parallel moves, further ones by shuffles
-template <int CTRL>
-__device__ __forceinline__ float dpp_add(float v) {
-    int w;
-    __builtin_memcpy(&w, &v, 4);
-    w = __builtin_amdgcn_update_dpp(0, w, CTRL, 0xf, 0xf, true);
-    float o;
-    __builtin_memcpy(&o, &w, 4);
-    return v + o;
-}
-template <int LPH>
-__device__ __forceinline__ float group_sum(float v) {
-    if (LPH >= 2) v = dpp_add<0xB1>(v);    // lane ^ 1
-    if (LPH >= 4) v = dpp_add<0x4E>(v);    // lane ^ 2
-    if (LPH >= 8) v = dpp_add<0x141>(v);   // the other half of 8 lanes (mirrored: its four lanes hold one value)
-    if (LPH >= 16) v = dpp_add<0x140>(v);  // the other half of 16 lanes
-    if (LPH >= 32) v += __shfl_xor(v, 16, 64);
-    if (LPH >= 64) v += __shfl_xor(v, 32, 64);
-    return v;
-}
-
-// A lane's piece of a head's row: VEC elements from `at`.  Where the row is no multiple of VEC, the last lane's piece ends with the row and overlaps its
-// neighbour's (both compute and store the same there); lanes behind the row repeat the last piece.  `first` is the first element that is the lane's own
-// (VEC: none); leave_own keeps the others out of the sums over the row, both factors zero, so that no infinity of a neighbour's element turns into NaN.
-template <typename T, int VEC>
-struct Piece {
-    T t[VEC];
-    __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(t, p, sizeof(t)); }
-    __device__ __forceinline__ void get(float (&v)[VEC]) const {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = (float)t[e];
-    }
-};
-template <int VEC, int LPH>
-struct Place {
-    int at, first;
-    bool tail;  // (uniform: the row does not fill its lanes' pieces)
-    __device__ __forceinline__ Place(int l, int D) : at(l * VEC < D - VEC ? l * VEC : D - VEC), tail(D != LPH * VEC) {
-        first = l * VEC - at;
-        first = first > VEC ? VEC : first;
-    }
-    __device__ __forceinline__ void leave_own(float (&v)[VEC]) const {
-        if (!tail) return;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = e >= first ? v[e] : 0.f;
-    }
-};
-template <typename T, int VEC>
-__device__ __forceinline__ void put(T* p, const float (&v)[VEC]) {
-    T t[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) t[e] = (T)v[e];
-    __builtin_memcpy(p, t, sizeof(t));
-}
 // weight of a running sum that goes from maximum m to `ref`; a maximum of -inf has weight zero
 __device__ __forceinline__ float weight_to(float m, float ref) { return m == -NA_INF ? 0.f : __expf(m - ref); }
 __device__ __forceinline__ float finite_ref(float m) { return m == -NA_INF ? 0.f : m; }
@@ -118,7 +66,7 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_kernel(NaArgs A) 
     const Lane<VEC, LPH> w(A, A.H);
     if (w.slot >= A.n_items || !w.head) return;
     const int4 it = A.items[w.slot];
-    const Place<VEC, LPH> at(w.l, A.D);
+    const Place<VEC> at(w.l, A.D, A.D != LPH * VEC);
     const int kv = w.h / (A.H / A.Hkv);
     float q[VEC], acc[VEC], m = -NA_INF, sum = 0.f, bias[UN];
     Piece<T, VEC> raw;
@@ -187,12 +135,9 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_kernel(NaArgs A) 
         }
     }
     if (it.w >= 0) {
-        float* part = A.part + ((int64_t)it.w * A.H + w.h) * (A.D + 2);
-        put<float, VEC>(part + 2 + at.at, acc);
-        if (w.l == 0) {
-            part[0] = m;
-            part[1] = sum;
-        }
+        const int64_t o = (int64_t)it.w * A.H + w.h;
+        put<float, VEC>(A.part + o * A.D + at.at, acc);
+        if (w.l == 0) A.part2[o] = make_float2(m, sum);
     } else {
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // (NaN stays)
 #pragma unroll
@@ -206,36 +151,93 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_kernel(NaArgs A) 
     }
 }
 
-// the parts of a long list, in order
+// The parts of a long list: wave w takes parts w, w + NA_JOIN, ... in order, then the waves' results are joined in order.
+constexpr int NA_JOIN = 8;
 template <typename T, int VEC, int LPH>
-__global__ __launch_bounds__(64) void nbr_attention_join_kernel(NaArgs A) {
+__global__ __launch_bounds__(64 * NA_JOIN) void nbr_attention_join_kernel(NaArgs A) {
+    __shared__ float red[NA_JOIN][VEC + 2][64];
     const int4 sp = A.splits[blockIdx.x];
-    const int h = blockIdx.y * (64 / LPH) + threadIdx.x / LPH;
-    const Place<VEC, LPH> at(threadIdx.x & (LPH - 1), A.D);
-    if (h >= A.H) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = blockIdx.y * (64 / LPH) + lane / LPH, hc = h < A.H ? h : A.H - 1;
+    const Place<VEC> at(lane & (LPH - 1), A.D, A.D != LPH * VEC);
     float acc[VEC], m = -NA_INF, sum = 0.f;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
-    for (int s = 0; s < sp.z; ++s) {
-        const float* part = A.part + ((int64_t)(sp.y + s) * A.H + h) * (A.D + 2);
-        float v[VEC];
-        const float om = part[0], os = part[1], top = fmaxf(m, om), ref = finite_ref(top);
-        const float w = weight_to(m, ref), ow = weight_to(om, ref);
-        __builtin_memcpy(v, part + 2 + at.at, sizeof(v));
+    auto join = [&](float om, float os, const float(&v)[VEC]) {
+        const float top = fmaxf(m, om), ref = finite_ref(top), w = weight_to(m, ref), ow = weight_to(om, ref);
         sum = sum * w + os * ow;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] = acc[e] * w + v[e] * ow;
         m = top;
+    };
+#pragma unroll 4
+    for (int s = wave; s < sp.z; s += NA_JOIN) {
+        const int64_t o = (int64_t)(sp.y + s) * A.H + hc;
+        float v[VEC];
+        __builtin_memcpy(v, A.part + o * A.D + at.at, sizeof(v));
+        const float2 ms = A.part2[o];
+        join(ms.x, ms.y, v);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) red[wave][e][lane] = acc[e];
+    red[wave][VEC][lane] = m;
+    red[wave][VEC + 1][lane] = sum;
+    __syncthreads();
+    if (wave != 0 || h >= A.H) return;
+    for (int s = 1; s < NA_JOIN; ++s) {
+        float v[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = red[s][e][lane];
+        join(red[s][VEC][lane], red[s][VEC + 1][lane], v);
     }
     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] *= inv;
     const int64_t o = (int64_t)sp.x * A.H + h;
     put<T, VEC>((T*)A.out + o * A.D + at.at, acc);
-    if ((threadIdx.x & (LPH - 1)) == 0) {
+    if ((lane & (LPH - 1)) == 0) {
         A.stats[o * 2] = m;
         A.stats[o * 2 + 1] = sum == 0.f ? 0.f : logf(sum);
     }
+}
+// the same for sums: two rows of D, and (`more`) a number of their own; true for the lanes that hold the result
+template <int VEC, int LPH>
+__device__ __forceinline__ bool join_sums(const NaArgs& A, int heads, bool more, const Place<VEC>& at, int h, float (&a)[VEC], float (&b)[VEC], float& first) {
+    __shared__ float red[NA_JOIN][2 * VEC + 1][64];
+    const int4 sp = A.splits[blockIdx.x];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hc = h < heads ? h : heads - 1;
+    first = 0.f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) a[e] = b[e] = 0.f;
+#pragma unroll 4
+    for (int s = wave; s < sp.z; s += NA_JOIN) {
+        const int64_t o = (int64_t)(sp.y + s) * heads + hc;
+        float x[VEC], y[VEC];
+        __builtin_memcpy(x, A.part + o * 2 * A.D + at.at, sizeof(x));
+        __builtin_memcpy(y, A.part + o * 2 * A.D + A.D + at.at, sizeof(y));
+        if (more) first += A.part2[o].x;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            a[e] += x[e];
+            b[e] += y[e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        red[wave][e][lane] = a[e];
+        red[wave][VEC + e][lane] = b[e];
+    }
+    red[wave][2 * VEC][lane] = first;
+    __syncthreads();
+    if (wave != 0 || h >= heads) return false;
+    for (int s = 1; s < NA_JOIN; ++s) {
+        first += red[s][2 * VEC][lane];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            a[e] += red[s][e][lane];
+            b[e] += red[s][VEC + e][lane];
+        }
+    }
+    return true;
 }
 
 // p from a score and its list's (m, log l); a list without a live entry has m = -inf
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dq_kernel(NaArgs 
     const Lane<VEC, LPH> w(A, A.H);
     if (w.slot >= A.n_items || !w.head) return;
     const int4 it = A.items[w.slot];
-    const Place<VEC, LPH> at(w.l, A.D);
+    const Place<VEC> at(w.l, A.D, A.D != LPH * VEC);
     const int kv = w.h / (A.H / A.Hkv);
     const int64_t o = (int64_t)it.x * A.H + w.h;
     float q[VEC], go[VEC], pdk[VEC], pk[VEC], delta = 0.f, bias[UN];
@@ -328,10 +330,10 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dq_kernel(NaArgs 
         }
     }
     if (it.w >= 0) {
-        float* part = A.part + ((int64_t)it.w * A.H + w.h) * (2 * A.D + 1);
-        put<float, VEC>(part + 1 + at.at, pdk);
-        put<float, VEC>(part + 1 + A.D + at.at, pk);
-        if (w.l == 0) part[0] = delta;
+        const int64_t p = (int64_t)it.w * A.H + w.h;
+        put<float, VEC>(A.part + p * 2 * A.D + at.at, pdk);
+        put<float, VEC>(A.part + p * 2 * A.D + A.D + at.at, pk);
+        if (w.l == 0) A.part2[p] = make_float2(delta, 0.f);
     } else {
         dq_of<VEC>(pdk, pk, delta, A.scale);
         put<T, VEC>((T*)A.out + o * A.D + at.at, pdk);
@@ -339,40 +341,24 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dq_kernel(NaArgs 
     }
 }
 template <typename T, int VEC, int LPH>
-__global__ __launch_bounds__(64) void nbr_attention_dq_join_kernel(NaArgs A) {
-    const int4 sp = A.splits[blockIdx.x];
-    const int h = blockIdx.y * (64 / LPH) + threadIdx.x / LPH;
-    const Place<VEC, LPH> at(threadIdx.x & (LPH - 1), A.D);
-    if (h >= A.H) return;
-    float pdk[VEC], pk[VEC], delta = 0.f;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) pdk[e] = pk[e] = 0.f;
-    for (int s = 0; s < sp.z; ++s) {
-        const float* part = A.part + ((int64_t)(sp.y + s) * A.H + h) * (2 * A.D + 1);
-        float a[VEC], b[VEC];
-        __builtin_memcpy(a, part + 1 + at.at, sizeof(a));
-        __builtin_memcpy(b, part + 1 + A.D + at.at, sizeof(b));
-        delta += part[0];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            pdk[e] += a[e];
-            pk[e] += b[e];
-        }
-    }
+__global__ __launch_bounds__(64 * NA_JOIN) void nbr_attention_dq_join_kernel(NaArgs A) {
+    const int lane = threadIdx.x & 63, h = blockIdx.y * (64 / LPH) + lane / LPH;
+    const Place<VEC> at(lane & (LPH - 1), A.D, A.D != LPH * VEC);
+    float pdk[VEC], pk[VEC], delta;
+    if (!join_sums<VEC, LPH>(A, A.H, true, at, h, pdk, pk, delta)) return;
     dq_of<VEC>(pdk, pk, delta, A.scale);
-    const int64_t o = (int64_t)sp.x * A.H + h;
+    const int64_t o = (int64_t)A.splits[blockIdx.x].x * A.H + h;
     put<T, VEC>((T*)A.out + o * A.D + at.at, pdk);
-    if ((threadIdx.x & (LPH - 1)) == 0) A.rowstats[o] = make_float4(A.stats[o * 2], A.stats[o * 2 + 1], delta, 0.f);
+    if ((lane & (LPH - 1)) == 0) A.rowstats[o] = make_float4(A.stats[o * 2], A.stats[o * 2 + 1], delta, 0.f);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- backward over the rows' lists: dk, dv, db
-template <typename T, int VEC, int LPH, bool BIAS>
+template <typename T, int VEC, int LPH, bool BIAS, int UN>
 __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dkv_kernel(NaArgs A) {
-    constexpr int UN = 2;
     const Lane<VEC, LPH> w(A, A.Hkv);
     if (w.slot >= A.n_items || !w.head) return;
     const int4 it = A.items[w.slot];
-    const Place<VEC, LPH> at(w.l, A.D);
+    const Place<VEC> at(w.l, A.D, A.D != LPH * VEC);
     const int R = A.H / A.Hkv;
     float k[VEC], v[VEC], dk[VEC], dv[VEC];
     Piece<T, VEC> raw, raw2;
@@ -460,28 +446,14 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dkv_kernel(NaArgs
     }
 }
 template <typename T, int VEC, int LPH>
-__global__ __launch_bounds__(64) void nbr_attention_dkv_join_kernel(NaArgs A) {
-    const int4 sp = A.splits[blockIdx.x];
-    const int h = blockIdx.y * (64 / LPH) + threadIdx.x / LPH;
-    const Place<VEC, LPH> at(threadIdx.x & (LPH - 1), A.D);
-    if (h >= A.Hkv) return;
-    float dk[VEC], dv[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) dk[e] = dv[e] = 0.f;
-    for (int s = 0; s < sp.z; ++s) {
-        const float* part = A.part + ((int64_t)(sp.y + s) * A.Hkv + h) * 2 * A.D;
-        float a[VEC], b[VEC];
-        __builtin_memcpy(a, part + at.at, sizeof(a));
-        __builtin_memcpy(b, part + A.D + at.at, sizeof(b));
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            dk[e] += a[e];
-            dv[e] += b[e];
-        }
-    }
+__global__ __launch_bounds__(64 * NA_JOIN) void nbr_attention_dkv_join_kernel(NaArgs A) {
+    const int lane = threadIdx.x & 63, h = blockIdx.y * (64 / LPH) + lane / LPH;
+    const Place<VEC> at(lane & (LPH - 1), A.D, A.D != LPH * VEC);
+    float dk[VEC], dv[VEC], none;
+    if (!join_sums<VEC, LPH>(A, A.Hkv, false, at, h, dk, dv, none)) return;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) dk[e] *= A.scale;
-    const int64_t o = ((int64_t)sp.x * A.Hkv + h) * A.D + at.at;
+    const int64_t o = ((int64_t)A.splits[blockIdx.x].x * A.Hkv + h) * A.D + at.at;
     put<T, VEC>((T*)A.dk + o, dk);
     put<T, VEC>((T*)A.dv + o, dv);
 }
@@ -499,15 +471,17 @@ static void na_launch(NaArgs A, NaPass pass, hipStream_t st) {
     if (pass == NA_FWD) {
         if (A.bias) nbr_attention_kernel<T, VEC, LPH, true><<<grid, block, 0, st>>>(A);
         else nbr_attention_kernel<T, VEC, LPH, false><<<grid, block, 0, st>>>(A);
-        if (A.n_splits > 0) nbr_attention_join_kernel<T, VEC, LPH><<<jgrid, dim3(64), 0, st>>>(A);
+        if (A.n_splits > 0) nbr_attention_join_kernel<T, VEC, LPH><<<jgrid, dim3(64 * NA_JOIN), 0, st>>>(A);
     } else if (pass == NA_DQ) {
         if (A.bias) nbr_attention_dq_kernel<T, VEC, LPH, true><<<grid, block, 0, st>>>(A);
         else nbr_attention_dq_kernel<T, VEC, LPH, false><<<grid, block, 0, st>>>(A);
-        if (A.n_splits > 0) nbr_attention_dq_join_kernel<T, VEC, LPH><<<jgrid, dim3(64), 0, st>>>(A);
+        if (A.n_splits > 0) nbr_attention_dq_join_kernel<T, VEC, LPH><<<jgrid, dim3(64 * NA_JOIN), 0, st>>>(A);
     } else {
-        if (A.bias) nbr_attention_dkv_kernel<T, VEC, LPH, true><<<grid, block, 0, st>>>(A);
-        else nbr_attention_dkv_kernel<T, VEC, LPH, false><<<grid, block, 0, st>>>(A);
-        if (A.n_splits > 0) nbr_attention_dkv_join_kernel<T, VEC, LPH><<<jgrid, dim3(64), 0, st>>>(A);
+        if (A.bias && A.dense) nbr_attention_dkv_kernel<T, VEC, LPH, true, 4><<<grid, block, 0, st>>>(A);
+        else if (A.bias) nbr_attention_dkv_kernel<T, VEC, LPH, true, 2><<<grid, block, 0, st>>>(A);
+        else if (A.dense) nbr_attention_dkv_kernel<T, VEC, LPH, false, 4><<<grid, block, 0, st>>>(A);
+        else nbr_attention_dkv_kernel<T, VEC, LPH, false, 2><<<grid, block, 0, st>>>(A);
+        if (A.n_splits > 0) nbr_attention_dkv_join_kernel<T, VEC, LPH><<<jgrid, dim3(64 * NA_JOIN), 0, st>>>(A);
     }
 }
 // lanes per head: the power of two that covers its pieces of 16 bytes (heads shorter than one piece: an element per lane)
@@ -530,6 +504,9 @@ static void na_launch_typed(const NaArgs& A, int type, NaPass pass, hipStream_t 
     else if (type == MARIUS_BF16) na_launch_width<__bf16>(A, pass, st);
     else na_launch_width<_Float16>(A, pass, st);
 }
+
+// the workspace: (backward: row statistics,) the parts' small numbers, the parts' rows, each at a multiple of 16 bytes
+static size_t na_small_bytes(const marius_neighbor_plan* P, int heads) { return ((size_t)P->n_slots * heads * sizeof(float2) + 15) & ~(size_t)15; }
 
 static int na_args(const marius_neighbor_plan* P, const marius_neighbor_attention* m, const char* what, NaArgs& A) {
     MARIUS_REQUIRE(P && m, "%s: null descriptor", what);
@@ -569,9 +546,10 @@ using namespace marius;
 
 extern "C" size_t marius_neighbor_attention_workspace_bytes(const marius_neighbor_plan* P, int32_t heads, int32_t kv_heads, int32_t dim, int32_t backward) {
     if (!P || heads <= 0 || kv_heads <= 0 || dim <= 0) return 0;
-    if (!backward) return (size_t)P->n_slots * heads * (dim + 2) * sizeof(float);
-    const size_t dq = (size_t)P->n_slots * heads * (2 * dim + 1), dkv = (size_t)P->r_n_slots * kv_heads * 2 * dim;
-    return (size_t)P->n * heads * sizeof(float4) + (dq > dkv ? dq : dkv) * sizeof(float);
+    const size_t small = na_small_bytes(P, heads);
+    if (!backward) return small + (size_t)P->n_slots * heads * dim * sizeof(float);
+    const size_t dq = (size_t)P->n_slots * heads * 2 * dim, dkv = (size_t)P->r_n_slots * kv_heads * 2 * dim;
+    return (size_t)P->n * heads * sizeof(float4) + small + (dq > dkv ? dq : dkv) * sizeof(float);
 }
 
 extern "C" int marius_neighbor_attention_forward(const marius_neighbor_plan* P, const marius_neighbor_attention* m, void* out, void* workspace, size_t workspace_bytes,
@@ -584,7 +562,8 @@ extern "C" int marius_neighbor_attention_forward(const marius_neighbor_plan* P, 
     MARIUS_REQUIRE(P->n_slots == 0 || (workspace && P->splits && workspace_bytes >= marius_neighbor_attention_workspace_bytes(P, m->heads, m->kv_heads, m->dim, 0)),
                    "neighbor_attention_forward: workspace too small");
     A.out = out;
-    A.part = (float*)workspace;
+    A.part2 = (float2*)workspace;
+    A.part = (float*)((char*)workspace + na_small_bytes(P, A.H));
     na_launch_typed(A, m->type, NA_FWD, as_stream(stream));
     return check_launch("neighbor_attention_forward");
 }
@@ -605,7 +584,8 @@ extern "C" int marius_neighbor_attention_backward(const marius_neighbor_plan* P,
     A.go_ld = grad_row;
     A.go_hd = grad_head;
     A.rowstats = (float4*)workspace;
-    A.part = (float*)(A.rowstats + (size_t)P->n * A.H);
+    A.part2 = (float2*)(A.rowstats + (size_t)P->n * A.H);
+    A.part = (float*)((char*)A.part2 + na_small_bytes(P, A.H));
     A.out = dq;
     na_launch_typed(A, m->type, NA_DQ, st);
     A.dk = dk;
@@ -616,6 +596,7 @@ extern "C" int marius_neighbor_attention_backward(const marius_neighbor_plan* P,
     A.items = (const int4*)P->r_items;
     A.splits = (const int4*)P->r_splits;
     A.n_items = P->r_n_items;
+    A.dense = P->T > 2 * (int64_t)P->r_n_items;
     A.n_splits = P->r_n_splits;
     na_launch_typed(A, m->type, NA_DKV, st);
     return check_launch("neighbor_attention_backward");

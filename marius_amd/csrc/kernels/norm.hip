@@ -14,15 +14,17 @@
 //     dx = s dt,   dg = dt u act'(g),   du = act(g) dt,   dz = the same norm gradient of du w_post at z
 //     dw = sum over rows of (gradient of the norm's output) times (normalised row),   db = sum over rows of that gradient
 //
-// Bound by HBM: every element is read once and written once, about ten operations each.  A row lives in the registers of 2 to 64 lanes of one wave (several
-// rows per wave where they are short) or of a whole workgroup (long rows), so the two statistics cost shuffles, not passes over memory.  Sums over rows are
-// deterministic: a workgroup adds its rows in order in registers, its lanes in a fixed order in LDS, and a second launch adds the workgroups' partials in
-// order.  Statistics, sums and the residual are fp32; y and h are rounded once each, at their stores (h comes from the unrounded y).
+// Bound by HBM: every element is read once and written once, about ten operations each.  A row lives in registers, four elements a lane: in 1 to 64 lanes of one wave
+// (several rows per wave where they are short) or, longer than 256 elements, in a workgroup, so the statistics cost lane moves (and a barrier), not passes over memory.
+// Four elements, not eight, for the 16-bit types too: the backward pass holds five rows and five sums a lane, and with eight elements one wave per SIMD was
+// left (50,000 rows of 1024 in bf16: 579 us, against FILL_BWD us).
+// Sums over rows are deterministic: a workgroup adds its rows in order in registers, its lanes in a fixed order in LDS, and a second launch adds the
+// workgroups' partials in order.  Statistics, sums and the residual are fp32; y and h are rounded once each, at their stores (h comes from the unrounded y).
 #include "row_types.h"
 
 namespace marius {
 
-constexpr int NORM_T = 256, NORM_MAX_D = 8192, NORM_MAX_WG = 1024;
+constexpr int NORM_T = 256, NORM_MAX_T = 1024, NORM_MAX_D = 8192, NORM_MAX_WG = 1024;
 
 struct NormArgs {
     const void *x, *z, *gate, *post_w, *post_b, *pre_w, *pre_b, *dy, *dh;  // forward: x; backward: x = the stored y
@@ -47,159 +49,188 @@ __device__ __forceinline__ float gate_slope(float g, float a, int act) {
     return 1.f;
 }
 
-// sums over a row's lanes, the same bits on all of them
-template <int N, bool BLK>
-__device__ __forceinline__ void row_sums(float (&v)[N], int tpr, float* red) {
-    for (int o = BLK ? 32 : tpr >> 1; o > 0; o >>= 1)
+// A row's lanes: tpr lanes of a wave (a power of two), or, BLK, the workgroup.  Every lane holds NCH pieces of VEC elements.
+template <int VEC, int NCH, bool BLK>
+struct Row {
+    int tpr, lane, rows, mine;  // lanes of a row, this one's number, rows a workgroup holds, this one's
+    int at[NCH], first[NCH];
+    bool tail;
+    float inv_d, *red;          // red: LDS of two reductions, used in turn
+    int turn;
+    __device__ __forceinline__ Row(const NormArgs& A, float* red_) : red(red_), turn(0) {
+        tpr = BLK ? (int)blockDim.x : A.tpr;
+        lane = BLK ? (int)threadIdx.x : (int)threadIdx.x & (tpr - 1);
+        rows = BLK ? 1 : NORM_T / tpr;
+        mine = BLK ? 0 : (int)threadIdx.x / tpr;
+        tail = A.d != tpr * NCH * VEC;
+        inv_d = 1.f / (float)A.d;
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
-    if (BLK) {
-        const int nw = blockDim.x >> 6, w = threadIdx.x >> 6;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0)
-#pragma unroll
-            for (int i = 0; i < N; ++i) red[w * N + i] = v[i];
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            v[i] = 0.f;
-            for (int k = 0; k < nw; ++k) v[i] += red[k * N + i];
+        for (int j = 0; j < NCH; ++j) {
+            const Place<VEC> p(j * tpr + lane, A.d, tail);
+            at[j] = p.at;
+            first[j] = p.first;
         }
     }
-}
-
-// mean (LAYER) and 1 / sqrt(mean square deviation + eps) of a row in registers; elements behind the row are zero on entry
-template <int NCH, int VEC, bool BLK>
-__device__ __forceinline__ void row_stats(const float (&v)[NCH][VEC], const NormArgs& A, int lane, float* red, float& mean, float& r) {
-    const float inv = 1.f / (float)A.d;
-    mean = 0.f;
-    if (A.layer) {
+    template <typename T>
+    __device__ __forceinline__ void load(Piece<T, VEC> (&p)[NCH], const void* base, int64_t row, int64_t ld) const {
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) p[j].load((const T*)base + row * ld + at[j]);
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(void* base, int64_t row, int64_t ld, const float (&v)[NCH][VEC]) const {
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) put<T, VEC>((T*)base + row * ld + at[j], v[j]);
+    }
+    // sums over the row of what every element contributes; elements that are a neighbour's have to be zero
+    template <int N>
+    __device__ __forceinline__ void sums(float (&v)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (BLK || tpr >= 2) v[i] = add_half<2>(v[i]);
+            if (BLK || tpr >= 4) v[i] = add_half<4>(v[i]);
+            if (BLK || tpr >= 8) v[i] = add_half<8>(v[i]);
+            if (BLK || tpr >= 16) v[i] = add_half<16>(v[i]);
+            if (BLK || tpr >= 32) v[i] = add_half<32>(v[i]);
+            if (BLK || tpr >= 64) v[i] = add_half<64>(v[i]);
+        }
+        if (BLK) {
+            // (one barrier: what the next reduction writes is the other half, and the one after that is behind the next barrier)
+            const int nw = (int)blockDim.x >> 6, w = (int)threadIdx.x >> 6;
+            float* r = red + turn * (NORM_MAX_T / 64) * 2;
+            turn ^= 1;
+            if ((threadIdx.x & 63) == 0)
+#pragma unroll
+                for (int i = 0; i < N; ++i) r[w * 2 + i] = v[i];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                v[i] = 0.f;
+                for (int k = 0; k < nw; ++k) v[i] += r[k * 2 + i];
+            }
+        }
+    }
+    __device__ __forceinline__ float own(float v, int j, int e) const { return tail && e < first[j] ? 0.f : v; }
+    // v -> the normalised row (v - mean) r; r = 1 / sqrt(mean square deviation + eps)
+    __device__ __forceinline__ float normalise(float (&v)[NCH][VEC], const NormArgs& A) {
+        if (A.layer) {
+            float s[1] = {0.f};
+#pragma unroll
+            for (int j = 0; j < NCH; ++j)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s[0] += own(v[j][e], j, e);
+            sums<1>(s);
+            const float mean = s[0] * inv_d;
+#pragma unroll
+            for (int j = 0; j < NCH; ++j)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[j][e] -= mean;
+        }
         float s[1] = {0.f};
 #pragma unroll
         for (int j = 0; j < NCH; ++j)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) s[0] += v[j][e];
-        row_sums<1, BLK>(s, A.tpr, red);
-        mean = s[0] * inv;
+            for (int e = 0; e < VEC; ++e) s[0] += own(v[j][e] * v[j][e], j, e);
+        sums<1>(s);
+        const float r = 1.f / sqrtf(s[0] * inv_d + A.eps);
+#pragma unroll
+        for (int j = 0; j < NCH; ++j)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[j][e] *= r;
+        return r;
     }
-    float s[1] = {0.f};
+    // a: gradient of the normalised row vn -> of what was normalised: r (a - [mean a] - vn mean(a vn))
+    __device__ __forceinline__ void gradient(float (&a)[NCH][VEC], const float (&vn)[NCH][VEC], const NormArgs& A, float r) {
+        float s[2] = {0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < NCH; ++j)
+        for (int j = 0; j < NCH; ++j)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float t = (j * A.tpr + lane) * VEC + e < A.d ? v[j][e] - mean : 0.f;
-            s[0] += t * t;
+            for (int e = 0; e < VEC; ++e) {
+                s[0] += own(a[j][e] * vn[j][e], j, e);
+                s[1] += own(a[j][e], j, e);
+            }
+        sums<2>(s);
+        const float ma = A.layer ? s[1] * inv_d : 0.f, mv = s[0] * inv_d;
+#pragma unroll
+        for (int j = 0; j < NCH; ++j)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) a[j][e] = r * (a[j][e] - ma - vn[j][e] * mv);
+    }
+    __device__ __forceinline__ void param(const void* p, int type, float missing, float (&v)[NCH][VEC]) const {
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            if (p) piece_any<VEC>(p, type, at[j], v[j]);
+            else
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[j][e] = missing;
         }
-    row_sums<1, BLK>(s, A.tpr, red);
-    r = 1.f / sqrtf(s[0] * inv + A.eps);
-}
-
-template <int NCH, int VEC>
-__device__ __forceinline__ void load_param(const void* p, int type, int tpr, int lane, int d, float missing, float (&v)[NCH][VEC]) {
-#pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-        if (p) piece_load_any<VEC>(p, type, (j * tpr + lane) * VEC, d, v[j]);
-        else
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[j][e] = missing;
     }
-}
+    template <typename T>
+    __device__ __forceinline__ void get(const Piece<T, VEC> (&p)[NCH], float (&v)[NCH][VEC]) const {
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) p[j].get(v[j]);
+    }
+};
 
-template <typename S, typename T, int NCH, bool BLK>
-__global__ __launch_bounds__(BLK ? 512 : NORM_T) void residual_norm_kernel(NormArgs A) {
-    constexpr int VEC = 16 / sizeof(T);
-    __shared__ float red[8];
-    const int tpr = BLK ? (int)blockDim.x : A.tpr, lane = BLK ? (int)threadIdx.x : (int)threadIdx.x & (tpr - 1);
-    const int rpw = BLK ? 1 : NORM_T / tpr, mine = BLK ? 0 : (int)threadIdx.x / tpr;
+template <typename S, typename T, int VEC, int NCH, bool BLK>
+__global__ __launch_bounds__(BLK ? NORM_MAX_T : NORM_T) void residual_norm_kernel(NormArgs A) {
+    __shared__ float red[BLK ? 4 * NORM_MAX_T / 64 : 1];
+    Row<VEC, NCH, BLK> R(A, red);
     float w2[NCH][VEC], b2[NCH][VEC], w1[NCH][VEC], b1[NCH][VEC], gc[NCH][VEC];
-    load_param<NCH, VEC>(A.post ? A.post_w : nullptr, A.param_type, tpr, lane, A.d, 1.f, w1);
-    load_param<NCH, VEC>(A.post ? A.post_b : nullptr, A.param_type, tpr, lane, A.d, 0.f, b1);
-    load_param<NCH, VEC>(A.pre ? A.pre_w : nullptr, A.param_type, tpr, lane, A.d, 1.f, w2);
-    load_param<NCH, VEC>(A.pre ? A.pre_b : nullptr, A.param_type, tpr, lane, A.d, 0.f, b2);
-    load_param<NCH, VEC>(A.gate_mode == 1 ? A.gate : nullptr, A.param_type, tpr, lane, A.d, 1.f, gc);
+    R.param(A.post ? A.post_w : nullptr, A.param_type, 1.f, w1);
+    R.param(A.post ? A.post_b : nullptr, A.param_type, 0.f, b1);
+    R.param(A.pre ? A.pre_w : nullptr, A.param_type, 1.f, w2);
+    R.param(A.pre ? A.pre_b : nullptr, A.param_type, 0.f, b2);
+    R.param(A.gate_mode == 1 ? A.gate : nullptr, A.param_type, 1.f, gc);
     if (A.gate_mode == 1)
 #pragma unroll
         for (int j = 0; j < NCH; ++j)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) gc[j][e] = gate_act(gc[j][e], A.act);
-    for (int64_t base = (int64_t)blockIdx.x * rpw; base < A.n; base += (int64_t)gridDim.x * rpw) {
-        const bool live = base + mine < A.n;
-        const int64_t row = live ? base + mine : A.n - 1;  // (lanes behind the last row take part in the shuffles with its values and store nothing)
+    for (int64_t base = (int64_t)blockIdx.x * R.rows; base < A.n; base += (int64_t)gridDim.x * R.rows) {
+        const bool live = base + R.mine < A.n;
+        const int64_t row = live ? base + R.mine : A.n - 1;  // (lanes behind the last row take part in the sums with its values and store nothing)
+        Piece<S, VEC> xp[NCH];
+        Piece<T, VEC> zp[NCH], gp[NCH];
         float y[NCH][VEC];
-#pragma unroll
-        for (int j = 0; j < NCH; ++j) piece_load<S, VEC>((const S*)A.x + row * A.x_ld, (j * tpr + lane) * VEC, A.d, y[j]);
+        R.load(xp, A.x, row, A.x_ld);
+        if (A.z) R.load(zp, A.z, row, A.z_ld);
+        if (A.gate_mode == 2) R.load(gp, A.gate, row, A.gate_ld);
+        R.get(xp, y);
         if (A.z) {
-            float z[NCH][VEC], g[NCH][VEC];
-#pragma unroll
-            for (int j = 0; j < NCH; ++j) {
-                piece_load<T, VEC>((const T*)A.z + row * A.z_ld, (j * tpr + lane) * VEC, A.d, z[j]);
-                if (A.gate_mode == 2) piece_load<T, VEC>((const T*)A.gate + row * A.gate_ld, (j * tpr + lane) * VEC, A.d, g[j]);
-            }
-            float mean = 0.f, r = 1.f;
-            if (A.post) row_stats<NCH, VEC, BLK>(z, A, lane, red, mean, r);
+            float u[NCH][VEC], open[NCH][VEC];
+            R.get(zp, u);
+            if (A.gate_mode == 2) R.get(gp, open);
+            if (A.post) R.normalise(u, A);
 #pragma unroll
             for (int j = 0; j < NCH; ++j)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    const float u = A.post ? (z[j][e] - mean) * r * w1[j][e] + b1[j][e] : z[j][e];
-                    const float open = A.gate_mode == 2 ? gate_act(g[j][e], A.act) : gc[j][e];
-                    y[j][e] = A.scale * y[j][e] + open * u;
+                    if (A.post) u[j][e] = u[j][e] * w1[j][e] + b1[j][e];
+                    y[j][e] = A.scale * y[j][e] + (A.gate_mode == 2 ? gate_act(open[j][e], A.act) : gc[j][e]) * u[j][e];
                 }
-            if (live)
-#pragma unroll
-                for (int j = 0; j < NCH; ++j) piece_store<S, VEC>((S*)A.y + row * A.y_ld, (j * tpr + lane) * VEC, A.d, y[j]);
+            if (live) R.template store<S>(A.y, row, A.y_ld, y);
         }
         if (A.pre) {
-            float mean, r;
-            // (elements behind the row: gate, weights and z are zero or one there, so y may not be zero: clear it for the statistics)
+            R.normalise(y, A);
 #pragma unroll
             for (int j = 0; j < NCH; ++j)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e)
-                    if ((j * tpr + lane) * VEC + e >= A.d) y[j][e] = 0.f;
-            row_stats<NCH, VEC, BLK>(y, A, lane, red, mean, r);
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) y[j][e] = (y[j][e] - mean) * r * w2[j][e] + b2[j][e];
-            if (live)
-#pragma unroll
-                for (int j = 0; j < NCH; ++j) piece_store<T, VEC>((T*)A.h + row * A.h_ld, (j * tpr + lane) * VEC, A.d, y[j]);
+                for (int e = 0; e < VEC; ++e) y[j][e] = y[j][e] * w2[j][e] + b2[j][e];
+            if (live) R.template store<T>(A.h, row, A.h_ld, y);
         }
     }
 }
 
-// gradient of the norm's input from a = (gradient of its output) times w, at v: r (a - [mean a] - vn mean(a vn)).  v becomes the normalised row.
-template <int NCH, int VEC, bool BLK>
-__device__ __forceinline__ void norm_gradient(float (&v)[NCH][VEC], float (&a)[NCH][VEC], const NormArgs& A, float mean, float r, float* red) {
-    float s[2] = {0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < NCH; ++j)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            s[0] += a[j][e] * v[j][e];
-            s[1] += a[j][e];
-        }
-    row_sums<2, BLK>(s, A.tpr, red);
-    const float inv = 1.f / (float)A.d, ma = A.layer ? s[1] * inv : 0.f, mv = s[0] * inv;
-#pragma unroll
-    for (int j = 0; j < NCH; ++j)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) a[j][e] = r * (a[j][e] - ma - v[j][e] * mv);
-}
-
-template <typename S, typename T, int NCH, bool BLK>
-__global__ __launch_bounds__(BLK ? 512 : NORM_T) void residual_norm_backward_kernel(NormArgs A) {
-    constexpr int VEC = 16 / sizeof(T);
-    __shared__ float red[16];
+template <typename S, typename T, int VEC, int NCH, bool BLK>
+__global__ __launch_bounds__(BLK ? NORM_MAX_T : NORM_T) void residual_norm_backward_kernel(NormArgs A) {
+    __shared__ float red[BLK ? 4 * NORM_MAX_T / 64 : 1];
     __shared__ float fold[BLK ? 1 : NORM_T * VEC];
-    const int tpr = BLK ? (int)blockDim.x : A.tpr, lane = BLK ? (int)threadIdx.x : (int)threadIdx.x & (tpr - 1);
-    const int rpw = BLK ? 1 : NORM_T / tpr, mine = BLK ? 0 : (int)threadIdx.x / tpr;
+    Row<VEC, NCH, BLK> R(A, red);
     float w2[NCH][VEC], w1[NCH][VEC], b1[NCH][VEC], gc[NCH][VEC], acc[SUMS][NCH][VEC];
-    load_param<NCH, VEC>(A.post ? A.post_w : nullptr, A.param_type, tpr, lane, A.d, 1.f, w1);
-    load_param<NCH, VEC>(A.post ? A.post_b : nullptr, A.param_type, tpr, lane, A.d, 0.f, b1);
-    load_param<NCH, VEC>(A.pre ? A.pre_w : nullptr, A.param_type, tpr, lane, A.d, 1.f, w2);
-    load_param<NCH, VEC>(A.gate_mode == 1 ? A.gate : nullptr, A.param_type, tpr, lane, A.d, 1.f, gc);
+    R.param(A.post ? A.post_w : nullptr, A.param_type, 1.f, w1);
+    R.param(A.post ? A.post_b : nullptr, A.param_type, 0.f, b1);
+    R.param(A.pre ? A.pre_w : nullptr, A.param_type, 1.f, w2);
+    R.param(A.gate_mode == 1 ? A.gate : nullptr, A.param_type, 1.f, gc);
     if (A.gate_mode == 1)
 #pragma unroll
         for (int j = 0; j < NCH; ++j)
@@ -211,105 +242,94 @@ __global__ __launch_bounds__(BLK ? 512 : NORM_T) void residual_norm_backward_ker
         for (int j = 0; j < NCH; ++j)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) acc[k][j][e] = 0.f;
-    for (int64_t base = (int64_t)blockIdx.x * rpw; base < A.n; base += (int64_t)gridDim.x * rpw) {
-        const bool live = base + mine < A.n;
-        const int64_t row = live ? base + mine : A.n - 1;
+    const bool pre = A.pre && A.dh, reads_z = A.z && (A.post || A.gate_mode);
+    for (int64_t base = (int64_t)blockIdx.x * R.rows; base < A.n; base += (int64_t)gridDim.x * R.rows) {
+        const bool live = base + R.mine < A.n;
+        const int64_t row = live ? base + R.mine : A.n - 1;
+        Piece<S, VEC> dyp[NCH], yp[NCH];
+        Piece<T, VEC> dhp[NCH], zp[NCH], gp[NCH];
         float dt[NCH][VEC];
-#pragma unroll
-        for (int j = 0; j < NCH; ++j) {
-            if (A.dy) piece_load<S, VEC>((const S*)A.dy + row * A.dy_ld, (j * tpr + lane) * VEC, A.d, dt[j]);
-            else
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) dt[j][e] = 0.f;
+        if (pre) {
+            R.load(yp, A.x, row, A.x_ld);
+            R.load(dhp, A.dh, row, A.dh_ld);
         }
-        if (A.pre && A.dh) {
-            float y[NCH][VEC], a[NCH][VEC], mean, r;
+        if (A.dy) R.load(dyp, A.dy, row, A.dy_ld);
+        if (reads_z) R.load(zp, A.z, row, A.z_ld);
+        if (A.gate_mode == 2) R.load(gp, A.gate, row, A.gate_ld);
 #pragma unroll
-            for (int j = 0; j < NCH; ++j) {
-                piece_load<S, VEC>((const S*)A.x + row * A.x_ld, (j * tpr + lane) * VEC, A.d, y[j]);
-                piece_load<T, VEC>((const T*)A.dh + row * A.dh_ld, (j * tpr + lane) * VEC, A.d, a[j]);
-            }
-            row_stats<NCH, VEC, BLK>(y, A, lane, red, mean, r);
+        for (int j = 0; j < NCH; ++j)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) dt[j][e] = 0.f;
+        if (pre) {
+            float y[NCH][VEC];
+            R.get(yp, y);
+            R.get(dhp, dt);
+            const float r = R.normalise(y, A);
 #pragma unroll
             for (int j = 0; j < NCH; ++j)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    y[j][e] = (y[j][e] - mean) * r;
                     if (live) {
-                        acc[SUM_PRE_W][j][e] += a[j][e] * y[j][e];
-                        acc[SUM_PRE_B][j][e] += a[j][e];
+                        acc[SUM_PRE_W][j][e] += dt[j][e] * y[j][e];
+                        acc[SUM_PRE_B][j][e] += dt[j][e];
                     }
-                    a[j][e] *= w2[j][e];
+                    dt[j][e] *= w2[j][e];
                 }
-            norm_gradient<NCH, VEC, BLK>(y, a, A, mean, r, red);
+            R.gradient(dt, y, A, r);
+        }
+        if (A.dy) {
+            float dy[NCH][VEC];
+            R.get(dyp, dy);
 #pragma unroll
             for (int j = 0; j < NCH; ++j)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) dt[j][e] += a[j][e];
+                for (int e = 0; e < VEC; ++e) dt[j][e] += dy[j][e];
         }
         if (A.dx && live) {
-            float o[VEC];
+            float dx[NCH][VEC];
 #pragma unroll
-            for (int j = 0; j < NCH; ++j) {
+            for (int j = 0; j < NCH; ++j)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) o[e] = A.scale * dt[j][e];
-                piece_store<S, VEC>((S*)A.dx + row * A.dx_ld, (j * tpr + lane) * VEC, A.d, o);
-            }
+                for (int e = 0; e < VEC; ++e) dx[j][e] = A.scale * dt[j][e];
+            R.template store<S>(A.dx, row, A.dx_ld, dx);
         }
         if (!A.z) continue;
-        float z[NCH][VEC], g[NCH][VEC], mean = 0.f, r = 1.f;
-        if (A.post || A.gate_mode) {
-#pragma unroll
-            for (int j = 0; j < NCH; ++j) piece_load<T, VEC>((const T*)A.z + row * A.z_ld, (j * tpr + lane) * VEC, A.d, z[j]);
-            if (A.post) {
-                row_stats<NCH, VEC, BLK>(z, A, lane, red, mean, r);
-#pragma unroll
-                for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) z[j][e] = (z[j][e] - mean) * r;
-            }
-        }
-        if (A.gate_mode == 2)
-#pragma unroll
-            for (int j = 0; j < NCH; ++j) piece_load<T, VEC>((const T*)A.gate + row * A.gate_ld, (j * tpr + lane) * VEC, A.d, g[j]);
+        float z[NCH][VEC], r = 1.f;
+        if (reads_z) R.get(zp, z);
+        if (A.post) r = R.normalise(z, A);
         if (A.gate_mode) {
+            float g[NCH][VEC], dg[NCH][VEC];
+            if (A.gate_mode == 2) R.get(gp, g);
 #pragma unroll
-            for (int j = 0; j < NCH; ++j) {
-                float o[VEC];
+            for (int j = 0; j < NCH; ++j)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    const float u = A.post ? z[j][e] * w1[j][e] + b1[j][e] : z[j][e];
-                    const float du = dt[j][e] * u;
+                    const float u = A.post ? z[j][e] * w1[j][e] + b1[j][e] : z[j][e], du = dt[j][e] * u;
                     if (A.gate_mode == 2) {
                         const float open = gate_act(g[j][e], A.act);
-                        o[e] = du * gate_slope(g[j][e], open, A.act);
+                        dg[j][e] = du * gate_slope(g[j][e], open, A.act);
                         dt[j][e] *= open;
                     } else {
                         if (live) acc[SUM_GATE][j][e] += du;
                         dt[j][e] *= gc[j][e];
                     }
                 }
-                if (A.gate_mode == 2 && live) piece_store<T, VEC>((T*)A.dgate + row * A.dgate_ld, (j * tpr + lane) * VEC, A.d, o);
-            }
+            if (A.gate_mode == 2 && live) R.template store<T>(A.dgate, row, A.dgate_ld, dg);
         }
         if (A.post) {
 #pragma unroll
             for (int j = 0; j < NCH; ++j)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    const bool in = (j * tpr + lane) * VEC + e < A.d;  // (behind the row z is -mean r: keep it out of the sums)
-                    if (!in) z[j][e] = 0.f;
                     if (live) {
                         acc[SUM_POST_W][j][e] += dt[j][e] * z[j][e];
                         acc[SUM_POST_B][j][e] += dt[j][e];
                     }
-                    dt[j][e] = in ? dt[j][e] * w1[j][e] : 0.f;
+                    dt[j][e] *= w1[j][e];
                 }
-            norm_gradient<NCH, VEC, BLK>(z, dt, A, mean, r, red);
+            R.gradient(dt, z, A, r);
         }
-        if (live)
-#pragma unroll
-            for (int j = 0; j < NCH; ++j) piece_store<T, VEC>((T*)A.dz + row * A.dz_ld, (j * tpr + lane) * VEC, A.d, dt[j]);
+        if (live) R.template store<T>(A.dz, row, A.dz_ld, dt);
     }
     // this workgroup's sums: lanes that own the same columns are added in a fixed order
 #pragma unroll
@@ -318,22 +338,21 @@ __global__ __launch_bounds__(BLK ? 512 : NORM_T) void residual_norm_backward_ker
         float* out = A.partial + ((int64_t)blockIdx.x * SUMS + k) * A.d;
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            const int c = (j * tpr + lane) * VEC;
             if (BLK) {
-                piece_store<float, VEC>(out, c, A.d, acc[k][j]);
+                put<float, VEC>(out + R.at[j], acc[k][j]);
             } else {
                 __syncthreads();
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) fold[threadIdx.x * VEC + e] = acc[k][j][e];
                 __syncthreads();
-                if (mine == 0) {
+                if (R.mine == 0) {
                     float s[VEC];
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) s[e] = 0.f;
-                    for (int q = 0; q < rpw; ++q)
+                    for (int q = 0; q < R.rows; ++q)
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) s[e] += fold[(q * tpr + lane) * VEC + e];
-                    piece_store<float, VEC>(out, c, A.d, s);
+                        for (int e = 0; e < VEC; ++e) s[e] += fold[(q * R.tpr + R.lane) * VEC + e];
+                    put<float, VEC>(out + R.at[j], s);
                 }
             }
         }
@@ -346,20 +365,21 @@ struct NormSumArgs {
     const void* gate;      // channel gate: its sum is multiplied by act'
     void* out[SUMS];
 };
-// 32 columns x 8 slices of the workgroups: a slice adds its workgroups in order, the slices are added in order
-__global__ __launch_bounds__(256) void residual_norm_sums_kernel(NormSumArgs A) {
-    __shared__ float red[256];
+// 32 columns x 32 slices of the workgroups: a slice adds its workgroups in order, the slices are added in order
+__global__ __launch_bounds__(1024) void residual_norm_sums_kernel(NormSumArgs A) {
+    __shared__ float red[1024];
     const int k = blockIdx.y, c = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
     if (!(A.want >> k & 1)) return;  // (uniform)
     float s = 0.f;
     if (c < A.d)
-        for (int w = slice; w < A.nwg; w += 8) s += A.partial[((int64_t)w * SUMS + k) * A.d + c];
+#pragma unroll 8
+        for (int w = slice; w < A.nwg; w += 32) s += A.partial[((int64_t)w * SUMS + k) * A.d + c];
     red[threadIdx.x] = s;
     __syncthreads();
     if (slice == 0 && c < A.d) {
         float t = 0.f;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) t += red[q * 32 + threadIdx.x];
+        for (int q = 0; q < 32; ++q) t += red[q * 32 + threadIdx.x];
         if (k == SUM_GATE) {
             const float g = element_any(A.gate, A.type, c);
             t *= gate_slope(g, gate_act(g, A.act), A.act);
@@ -368,39 +388,41 @@ __global__ __launch_bounds__(256) void residual_norm_sums_kernel(NormSumArgs A) 
     }
 }
 
-// lanes per row and pieces per lane: a row of up to 128 pieces stays in one wave (two pieces a lane at most), a longer one takes a workgroup
+// a row of up to 64 pieces of four elements stays in one wave, a longer one takes a workgroup of as many waves as hold it (two pieces a lane beyond 4096 elements)
 struct NormShape {
-    int tpr, nch;
+    int vec, tpr, nch, threads;
     bool blk;
 };
-static NormShape norm_shape(int d, int vec) {
-    const int units = (int)cdiv(d, vec);
-    NormShape s{1, 1, units > 128};
-    if (!s.blk) {
-        while (s.tpr < 64 && s.tpr < units) s.tpr <<= 1;
-        s.nch = units > 64 ? 2 : 1;
+static NormShape norm_shape(int d) {
+    NormShape s{d < 4 ? 1 : 4, 1, 1, NORM_T, false};
+    const int units = (int)cdiv(d, s.vec);
+    s.blk = units > 64;
+    if (s.blk) {
+        s.nch = units > NORM_MAX_T ? 2 : 1;
+        s.threads = s.tpr = (int)cdiv(cdiv(units, s.nch), 64) * 64;
     } else {
-        s.tpr = units > 1024 ? 512 : 256;
-        s.nch = (int)cdiv(units, s.tpr) <= 1 ? 1 : cdiv(units, s.tpr) <= 2 ? 2 : 4;
+        while (s.tpr < units) s.tpr <<= 1;
     }
     return s;
+}
+static unsigned norm_groups(const NormShape& s, int64_t n, int most) {
+    const int64_t groups = cdiv(n, s.blk ? 1 : NORM_T / s.tpr);
+    return (unsigned)(groups < most ? groups : most);
 }
 
 template <typename S, typename T>
 static void launch_norm(const NormArgs& A, const NormShape& s, bool backward, unsigned grid, hipStream_t st) {
-    const dim3 g(grid), b(s.blk ? s.tpr : NORM_T);
+    const dim3 g(grid), b(s.threads);
     if (backward) {
-        if (!s.blk && s.nch == 1) residual_norm_backward_kernel<S, T, 1, false><<<g, b, 0, st>>>(A);
-        else if (!s.blk) residual_norm_backward_kernel<S, T, 2, false><<<g, b, 0, st>>>(A);
-        else if (s.nch == 1) residual_norm_backward_kernel<S, T, 1, true><<<g, b, 0, st>>>(A);
-        else if (s.nch == 2) residual_norm_backward_kernel<S, T, 2, true><<<g, b, 0, st>>>(A);
-        else residual_norm_backward_kernel<S, T, 4, true><<<g, b, 0, st>>>(A);
+        if (s.vec == 1) residual_norm_backward_kernel<S, T, 1, 1, false><<<g, b, 0, st>>>(A);
+        else if (!s.blk) residual_norm_backward_kernel<S, T, 4, 1, false><<<g, b, 0, st>>>(A);
+        else if (s.nch == 1) residual_norm_backward_kernel<S, T, 4, 1, true><<<g, b, 0, st>>>(A);
+        else residual_norm_backward_kernel<S, T, 4, 2, true><<<g, b, 0, st>>>(A);
     } else {
-        if (!s.blk && s.nch == 1) residual_norm_kernel<S, T, 1, false><<<g, b, 0, st>>>(A);
-        else if (!s.blk) residual_norm_kernel<S, T, 2, false><<<g, b, 0, st>>>(A);
-        else if (s.nch == 1) residual_norm_kernel<S, T, 1, true><<<g, b, 0, st>>>(A);
-        else if (s.nch == 2) residual_norm_kernel<S, T, 2, true><<<g, b, 0, st>>>(A);
-        else residual_norm_kernel<S, T, 4, true><<<g, b, 0, st>>>(A);
+        if (s.vec == 1) residual_norm_kernel<S, T, 1, 1, false><<<g, b, 0, st>>>(A);
+        else if (!s.blk) residual_norm_kernel<S, T, 4, 1, false><<<g, b, 0, st>>>(A);
+        else if (s.nch == 1) residual_norm_kernel<S, T, 4, 1, true><<<g, b, 0, st>>>(A);
+        else residual_norm_kernel<S, T, 4, 2, true><<<g, b, 0, st>>>(A);
     }
 }
 static void launch_norm_typed(const NormArgs& A, const NormShape& s, int stream_type, int type, bool backward, unsigned grid, hipStream_t st) {
@@ -465,10 +487,9 @@ extern "C" int marius_residual_norm_forward(const marius_residual_norm* m, const
     A.y_ld = y_ld;
     A.h = h;
     A.h_ld = h_ld;
-    const NormShape s = norm_shape(A.d, m->type == MARIUS_F32 ? 4 : 8);
+    const NormShape s = norm_shape(A.d);
     A.tpr = s.tpr;
-    const int64_t groups = cdiv(A.n, s.blk ? 1 : NORM_T / s.tpr);
-    launch_norm_typed(A, s, m->stream_type, m->type, false, (unsigned)(groups < 2048 ? groups : 2048), as_stream(stream));
+    launch_norm_typed(A, s, m->stream_type, m->type, false, norm_groups(s, A.n, 2048), as_stream(stream));
     return check_launch("residual_norm_forward");
 }
 
@@ -511,10 +532,9 @@ extern "C" int marius_residual_norm_backward(const marius_residual_norm* m, cons
         A.dgate = A.gate_mode == MARIUS_GATE_ELEMENT ? g->dgate : nullptr;
         A.dgate_ld = g->dgate_ld;
         A.partial = (float*)workspace;
-        const NormShape s = norm_shape(A.d, m->type == MARIUS_F32 ? 4 : 8);
+        const NormShape s = norm_shape(A.d);
         A.tpr = s.tpr;
-        const int64_t groups = cdiv(A.n, s.blk ? 1 : NORM_T / s.tpr);
-        nwg = (int)(groups < NORM_MAX_WG ? groups : NORM_MAX_WG);
+        nwg = (int)norm_groups(s, A.n, NORM_MAX_WG);
         launch_norm_typed(A, s, m->stream_type, m->type, true, (unsigned)nwg, st);
     }
     if (A.want) {  // (no rows: the sums are zero)
@@ -527,7 +547,7 @@ extern "C" int marius_residual_norm_backward(const marius_residual_norm* m, cons
         S.act = A.act;
         S.gate = A.gate;
         for (int k = 0; k < SUMS; ++k) S.out[k] = sums[k];
-        residual_norm_sums_kernel<<<dim3((unsigned)cdiv(A.d, 32), SUMS), dim3(256), 0, st>>>(S);
+        residual_norm_sums_kernel<<<dim3((unsigned)cdiv(A.d, 32), SUMS), dim3(1024), 0, st>>>(S);
     }
     return check_launch("residual_norm_backward");
 }

@@ -375,6 +375,13 @@ inline int __builtin_amdgcn_update_dpp(int, int v, int ctrl, int, int, bool) {
         return c == 0x141 ? (lane & ~7) | (7 - (lane & 7)) : (lane & ~15) | (15 - (lane & 15));
     }, ctrl);
 }
+// v_permlane16_swap / v_permlane32_swap of a register with itself: (the lower, the upper) of each pair of rows of 16 lanes / of the wave's halves
+inline emul::vec<unsigned, 2> emul_lane_pair(unsigned v, int bit) {
+    const unsigned lo = emul::exchange<unsigned>(v, [](int lane, int b) { return lane & ~b; }, bit), hi = emul::exchange<unsigned>(v, [](int lane, int b) { return lane | b; }, bit);
+    return emul::vec<unsigned, 2>{{lo, hi}};
+}
+inline emul::vec<unsigned, 2> __builtin_amdgcn_permlane16_swap(unsigned a, unsigned, bool, bool) { return emul_lane_pair(a, 16); }
+inline emul::vec<unsigned, 2> __builtin_amdgcn_permlane32_swap(unsigned a, unsigned, bool, bool) { return emul_lane_pair(a, 32); }
 // e4m3 (OCP): v_cvt_pk_f32_fp8 / v_cvt_pk_fp8_f32 on two of a word's four codes; to nearest even, values the type does not reach become NaN
 inline float emul_fp8_to_f32(uint8_t c) {
     const int e = (c >> 3) & 15, m = c & 7;
