@@ -17,7 +17,7 @@
 // Bound by HBM: every element is read once and written once, about ten operations each.  A row lives in registers, four elements a lane: in 1 to 64 lanes of one wave
 // (several rows per wave where they are short) or, longer than 256 elements, in a workgroup, so the statistics cost lane moves (and a barrier), not passes over memory.
 // Four elements, not eight, for the 16-bit types too: the backward pass holds five rows and five sums a lane, and with eight elements one wave per SIMD was
-// left (50,000 rows of 1024 in bf16: 579 us, against FILL_BWD us).
+// left (50,000 rows of 1024 in bf16: 579 us, against 190 us now).
 // Sums over rows are deterministic: a workgroup adds its rows in order in registers, its lanes in a fixed order in LDS, and a second launch adds the
 // workgroups' partials in order.  Statistics, sums and the residual are fp32; y and h are rounded once each, at their stores (h comes from the unrounded y).
 #include "row_types.h"
@@ -37,11 +37,9 @@ struct NormArgs {
 };
 enum { SUM_POST_W = 0, SUM_POST_B, SUM_PRE_W, SUM_PRE_B, SUM_GATE, SUMS };
 
-__device__ __forceinline__ float gate_act(float v, int act) {
-    if (act == MARIUS_ACT_RELU) return v > 0.f ? v : 0.f;
-    if (act == MARIUS_ACT_SIGMOID) return 1.f / (1.f + expf(-v));
-    return v;
-}
+// (sigmoid: the hardware's exponential and reciprocal, a step of fp32 or two together)
+__device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
+__device__ __forceinline__ float gate_act(float v, int act) { return act == MARIUS_ACT_RELU ? fmaxf(v, 0.f) : act == MARIUS_ACT_SIGMOID ? sigmoid(v) : v; }
 // act' from the gate g and a = act(g)
 __device__ __forceinline__ float gate_slope(float g, float a, int act) {
     if (act == MARIUS_ACT_RELU) return g > 0.f ? 1.f : 0.f;
@@ -49,9 +47,15 @@ __device__ __forceinline__ float gate_slope(float g, float a, int act) {
     return 1.f;
 }
 
+// What is done to every element of a lane's pieces; the conditions that hold for a whole launch stand outside of it (in front of every element they cost more than
+// the arithmetic: 250 vector operations an element, 50,000 rows of 1024 in bf16 back in 334 us).
+#define EACH(NCH, VEC)                  \
+    _Pragma("unroll") for (int j = 0; j < NCH; ++j) _Pragma("unroll") for (int e = 0; e < VEC; ++e)
+
 // A row's lanes: tpr lanes of a wave (a power of two), or, BLK, the workgroup.  Every lane holds NCH pieces of VEC elements.
 template <int VEC, int NCH, bool BLK>
 struct Row {
+    typedef float Values[NCH][VEC];
     int tpr, lane, rows, mine;  // lanes of a row, this one's number, rows a workgroup holds, this one's
     int at[NCH], first[NCH];
     bool tail;
@@ -77,25 +81,38 @@ struct Row {
         for (int j = 0; j < NCH; ++j) p[j].load((const T*)base + row * ld + at[j]);
     }
     template <typename T>
-    __device__ __forceinline__ void store(void* base, int64_t row, int64_t ld, const float (&v)[NCH][VEC]) const {
+    __device__ __forceinline__ void store(void* base, int64_t row, int64_t ld, const Values& v) const {
 #pragma unroll
         for (int j = 0; j < NCH; ++j) put<T, VEC>((T*)base + row * ld + at[j], v[j]);
     }
-    // sums over the row of what every element contributes; elements that are a neighbour's have to be zero
+    template <typename T>
+    __device__ __forceinline__ void get(const Piece<T, VEC> (&p)[NCH], Values& v) const {
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) p[j].get(v[j]);
+    }
+    // elements that are a neighbour's (or behind the row): zero, for a sum
+    __device__ __forceinline__ void leave_own(Values& v) const {
+        if (tail) EACH(NCH, VEC) v[j][e] = e >= first[j] ? v[j][e] : 0.f;
+    }
+    // sums over the row of N values a lane
     template <int N>
     __device__ __forceinline__ void sums(float (&v)[N]) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (BLK || tpr >= 2) v[i] = add_half<2>(v[i]);
-            if (BLK || tpr >= 4) v[i] = add_half<4>(v[i]);
-            if (BLK || tpr >= 8) v[i] = add_half<8>(v[i]);
-            if (BLK || tpr >= 16) v[i] = add_half<16>(v[i]);
-            if (BLK || tpr >= 32) v[i] = add_half<32>(v[i]);
-            if (BLK || tpr >= 64) v[i] = add_half<64>(v[i]);
+            if (BLK) {
+                v[i] = group_sum<64>(v[i]);
+            } else {
+                if (tpr >= 2) v[i] = add_half<2>(v[i]);
+                if (tpr >= 4) v[i] = add_half<4>(v[i]);
+                if (tpr >= 8) v[i] = add_half<8>(v[i]);
+                if (tpr >= 16) v[i] = add_half<16>(v[i]);
+                if (tpr >= 32) v[i] = add_half<32>(v[i]);
+                if (tpr >= 64) v[i] = add_half<64>(v[i]);
+            }
         }
         if (BLK) {
             // (one barrier: what the next reduction writes is the other half, and the one after that is behind the next barrier)
-            const int nw = (int)blockDim.x >> 6, w = (int)threadIdx.x >> 6;
+            const int nw = (int)blockDim.x >> 6, w = (int)threadIdx.x >> 6, q = (int)threadIdx.x & 15;
             float* r = red + turn * (NORM_MAX_T / 64) * 2;
             turn ^= 1;
             if ((threadIdx.x & 63) == 0)
@@ -103,76 +120,61 @@ struct Row {
                 for (int i = 0; i < N; ++i) r[w * 2 + i] = v[i];
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                v[i] = 0.f;
-                for (int k = 0; k < nw; ++k) v[i] += r[k * 2 + i];
-            }
+            for (int i = 0; i < N; ++i) v[i] = group_sum<16>(q < nw ? r[q * 2 + i] : 0.f);
         }
     }
-    __device__ __forceinline__ float own(float v, int j, int e) const { return tail && e < first[j] ? 0.f : v; }
     // v -> the normalised row (v - mean) r; r = 1 / sqrt(mean square deviation + eps)
-    __device__ __forceinline__ float normalise(float (&v)[NCH][VEC], const NormArgs& A) {
+    __device__ __forceinline__ float normalise(Values& v, const NormArgs& A) {
+        Values t;
         if (A.layer) {
             float s[1] = {0.f};
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) s[0] += own(v[j][e], j, e);
+            EACH(NCH, VEC) t[j][e] = v[j][e];
+            leave_own(t);
+            EACH(NCH, VEC) s[0] += t[j][e];
             sums<1>(s);
             const float mean = s[0] * inv_d;
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) v[j][e] -= mean;
+            EACH(NCH, VEC) v[j][e] -= mean;
         }
         float s[1] = {0.f};
-#pragma unroll
-        for (int j = 0; j < NCH; ++j)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) s[0] += own(v[j][e] * v[j][e], j, e);
+        EACH(NCH, VEC) t[j][e] = v[j][e];
+        leave_own(t);
+        EACH(NCH, VEC) s[0] += t[j][e] * t[j][e];
         sums<1>(s);
-        const float r = 1.f / sqrtf(s[0] * inv_d + A.eps);
-#pragma unroll
-        for (int j = 0; j < NCH; ++j)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[j][e] *= r;
+        const float r = __builtin_amdgcn_rsqf(s[0] * inv_d + A.eps);  // (one step of fp32)
+        EACH(NCH, VEC) v[j][e] *= r;
         return r;
     }
     // a: gradient of the normalised row vn -> of what was normalised: r (a - [mean a] - vn mean(a vn))
-    __device__ __forceinline__ void gradient(float (&a)[NCH][VEC], const float (&vn)[NCH][VEC], const NormArgs& A, float r) {
+    __device__ __forceinline__ void gradient(Values& a, const Values& vn, const NormArgs& A, float r) {
+        Values t;
         float s[2] = {0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < NCH; ++j)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                s[0] += own(a[j][e] * vn[j][e], j, e);
-                s[1] += own(a[j][e], j, e);
-            }
+        EACH(NCH, VEC) t[j][e] = a[j][e];
+        leave_own(t);
+        EACH(NCH, VEC) {
+            s[0] += t[j][e] * vn[j][e];
+            s[1] += t[j][e];
+        }
         sums<2>(s);
         const float ma = A.layer ? s[1] * inv_d : 0.f, mv = s[0] * inv_d;
-#pragma unroll
-        for (int j = 0; j < NCH; ++j)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) a[j][e] = r * (a[j][e] - ma - vn[j][e] * mv);
+        EACH(NCH, VEC) a[j][e] = r * (a[j][e] - ma - vn[j][e] * mv);
     }
-    __device__ __forceinline__ void param(const void* p, int type, float missing, float (&v)[NCH][VEC]) const {
+    __device__ __forceinline__ void param(const void* p, int type, float missing, Values& v) const {
+        if (p) {
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) {
-            if (p) piece_any<VEC>(p, type, at[j], v[j]);
-            else
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) v[j][e] = missing;
+            for (int j = 0; j < NCH; ++j) piece_any<VEC>(p, type, at[j], v[j]);
+        } else {
+            EACH(NCH, VEC) v[j][e] = missing;
         }
     }
-    template <typename T>
-    __device__ __forceinline__ void get(const Piece<T, VEC> (&p)[NCH], float (&v)[NCH][VEC]) const {
-#pragma unroll
-        for (int j = 0; j < NCH; ++j) p[j].get(v[j]);
+    // g -> act(g)
+    __device__ __forceinline__ void open(Values& g, int act) const {
+        if (act == MARIUS_ACT_SIGMOID) EACH(NCH, VEC) g[j][e] = sigmoid(g[j][e]);
+        else if (act == MARIUS_ACT_RELU) EACH(NCH, VEC) g[j][e] = fmaxf(g[j][e], 0.f);
     }
 };
 
-template <typename S, typename T, int VEC, int NCH, bool BLK>
-__global__ __launch_bounds__(BLK ? NORM_MAX_T : NORM_T) void residual_norm_kernel(NormArgs A) {
+template <typename S, typename T, int VEC, int NCH, bool BLK, int GATE>
+__global__ __launch_bounds__(!BLK ? NORM_T : NCH > 1 ? NORM_MAX_T / 2 : NORM_MAX_T) void residual_norm_kernel(NormArgs A) {
     __shared__ float red[BLK ? 4 * NORM_MAX_T / 64 : 1];
     Row<VEC, NCH, BLK> R(A, red);
     float w2[NCH][VEC], b2[NCH][VEC], w1[NCH][VEC], b1[NCH][VEC], gc[NCH][VEC];
@@ -180,49 +182,46 @@ __global__ __launch_bounds__(BLK ? NORM_MAX_T : NORM_T) void residual_norm_kerne
     R.param(A.post ? A.post_b : nullptr, A.param_type, 0.f, b1);
     R.param(A.pre ? A.pre_w : nullptr, A.param_type, 1.f, w2);
     R.param(A.pre ? A.pre_b : nullptr, A.param_type, 0.f, b2);
-    R.param(A.gate_mode == 1 ? A.gate : nullptr, A.param_type, 1.f, gc);
-    if (A.gate_mode == 1)
-#pragma unroll
-        for (int j = 0; j < NCH; ++j)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) gc[j][e] = gate_act(gc[j][e], A.act);
-    for (int64_t base = (int64_t)blockIdx.x * R.rows; base < A.n; base += (int64_t)gridDim.x * R.rows) {
-        const bool live = base + R.mine < A.n;
+    if (GATE == 1) {
+        R.param(A.gate, A.param_type, 1.f, gc);
+        R.open(gc, A.act);
+    }
+    const int64_t stride = (int64_t)gridDim.x * R.rows;
+    for (int64_t base = (int64_t)blockIdx.x * R.rows; base < A.n; base += stride) {
+        const bool live = BLK || base + R.mine < A.n;
         const int64_t row = live ? base + R.mine : A.n - 1;  // (lanes behind the last row take part in the sums with its values and store nothing)
         Piece<S, VEC> xp[NCH];
         Piece<T, VEC> zp[NCH], gp[NCH];
         float y[NCH][VEC];
         R.load(xp, A.x, row, A.x_ld);
         if (A.z) R.load(zp, A.z, row, A.z_ld);
-        if (A.gate_mode == 2) R.load(gp, A.gate, row, A.gate_ld);
+        if (GATE == 2) R.load(gp, A.gate, row, A.gate_ld);
         R.get(xp, y);
         if (A.z) {
-            float u[NCH][VEC], open[NCH][VEC];
+            float u[NCH][VEC];
             R.get(zp, u);
-            if (A.gate_mode == 2) R.get(gp, open);
-            if (A.post) R.normalise(u, A);
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    if (A.post) u[j][e] = u[j][e] * w1[j][e] + b1[j][e];
-                    y[j][e] = A.scale * y[j][e] + (A.gate_mode == 2 ? gate_act(open[j][e], A.act) : gc[j][e]) * u[j][e];
-                }
+            if (A.post) {
+                R.normalise(u, A);
+                EACH(NCH, VEC) u[j][e] = u[j][e] * w1[j][e] + b1[j][e];
+            }
+            if (GATE == 2) {
+                R.get(gp, gc);
+                R.open(gc, A.act);
+            }
+            if (GATE) EACH(NCH, VEC) u[j][e] *= gc[j][e];
+            EACH(NCH, VEC) y[j][e] = A.scale * y[j][e] + u[j][e];
             if (live) R.template store<S>(A.y, row, A.y_ld, y);
         }
         if (A.pre) {
             R.normalise(y, A);
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) y[j][e] = y[j][e] * w2[j][e] + b2[j][e];
+            EACH(NCH, VEC) y[j][e] = y[j][e] * w2[j][e] + b2[j][e];
             if (live) R.template store<T>(A.h, row, A.h_ld, y);
         }
     }
 }
 
-template <typename S, typename T, int VEC, int NCH, bool BLK>
-__global__ __launch_bounds__(BLK ? NORM_MAX_T : NORM_T) void residual_norm_backward_kernel(NormArgs A) {
+template <typename S, typename T, int VEC, int NCH, bool BLK, int GATE>
+__global__ __launch_bounds__(!BLK ? NORM_T : NCH > 1 ? NORM_MAX_T / 2 : NORM_MAX_T) void residual_norm_backward_kernel(NormArgs A) {
     __shared__ float red[BLK ? 4 * NORM_MAX_T / 64 : 1];
     __shared__ float fold[BLK ? 1 : NORM_T * VEC];
     Row<VEC, NCH, BLK> R(A, red);
@@ -230,21 +229,16 @@ __global__ __launch_bounds__(BLK ? NORM_MAX_T : NORM_T) void residual_norm_backw
     R.param(A.post ? A.post_w : nullptr, A.param_type, 1.f, w1);
     R.param(A.post ? A.post_b : nullptr, A.param_type, 0.f, b1);
     R.param(A.pre ? A.pre_w : nullptr, A.param_type, 1.f, w2);
-    R.param(A.gate_mode == 1 ? A.gate : nullptr, A.param_type, 1.f, gc);
-    if (A.gate_mode == 1)
+    if (GATE == 1) {
+        R.param(A.gate, A.param_type, 1.f, gc);
+        R.open(gc, A.act);
+    }
 #pragma unroll
-        for (int j = 0; j < NCH; ++j)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) gc[j][e] = gate_act(gc[j][e], A.act);
-#pragma unroll
-    for (int k = 0; k < SUMS; ++k)
-#pragma unroll
-        for (int j = 0; j < NCH; ++j)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[k][j][e] = 0.f;
-    const bool pre = A.pre && A.dh, reads_z = A.z && (A.post || A.gate_mode);
-    for (int64_t base = (int64_t)blockIdx.x * R.rows; base < A.n; base += (int64_t)gridDim.x * R.rows) {
-        const bool live = base + R.mine < A.n;
+    for (int k = 0; k < SUMS; ++k) EACH(NCH, VEC) acc[k][j][e] = 0.f;
+    const bool pre = A.pre && A.dh, reads_z = A.post || GATE;
+    const int64_t stride = (int64_t)gridDim.x * R.rows;
+    for (int64_t base = (int64_t)blockIdx.x * R.rows; base < A.n; base += stride) {
+        const bool live = BLK || base + R.mine < A.n;
         const int64_t row = live ? base + R.mine : A.n - 1;
         Piece<S, VEC> dyp[NCH], yp[NCH];
         Piece<T, VEC> dhp[NCH], zp[NCH], gp[NCH];
@@ -255,78 +249,57 @@ __global__ __launch_bounds__(BLK ? NORM_MAX_T : NORM_T) void residual_norm_backw
         }
         if (A.dy) R.load(dyp, A.dy, row, A.dy_ld);
         if (reads_z) R.load(zp, A.z, row, A.z_ld);
-        if (A.gate_mode == 2) R.load(gp, A.gate, row, A.gate_ld);
-#pragma unroll
-        for (int j = 0; j < NCH; ++j)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) dt[j][e] = 0.f;
+        if (GATE == 2) R.load(gp, A.gate, row, A.gate_ld);
         if (pre) {
             float y[NCH][VEC];
             R.get(yp, y);
             R.get(dhp, dt);
             const float r = R.normalise(y, A);
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    if (live) {
-                        acc[SUM_PRE_W][j][e] += dt[j][e] * y[j][e];
-                        acc[SUM_PRE_B][j][e] += dt[j][e];
-                    }
-                    dt[j][e] *= w2[j][e];
-                }
+            if (live) EACH(NCH, VEC) {
+                acc[SUM_PRE_W][j][e] += dt[j][e] * y[j][e];
+                acc[SUM_PRE_B][j][e] += dt[j][e];
+            }
+            EACH(NCH, VEC) dt[j][e] *= w2[j][e];
             R.gradient(dt, y, A, r);
-        }
-        if (A.dy) {
-            float dy[NCH][VEC];
-            R.get(dyp, dy);
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) dt[j][e] += dy[j][e];
+            if (A.dy) {
+                float dy[NCH][VEC];
+                R.get(dyp, dy);
+                EACH(NCH, VEC) dt[j][e] += dy[j][e];
+            }
+        } else {
+            R.get(dyp, dt);  // (one of the two gradients is there)
         }
         if (A.dx && live) {
             float dx[NCH][VEC];
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) dx[j][e] = A.scale * dt[j][e];
+            EACH(NCH, VEC) dx[j][e] = A.scale * dt[j][e];
             R.template store<S>(A.dx, row, A.dx_ld, dx);
         }
         if (!A.z) continue;
         float z[NCH][VEC], r = 1.f;
         if (reads_z) R.get(zp, z);
         if (A.post) r = R.normalise(z, A);
-        if (A.gate_mode) {
-            float g[NCH][VEC], dg[NCH][VEC];
-            if (A.gate_mode == 2) R.get(gp, g);
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float u = A.post ? z[j][e] * w1[j][e] + b1[j][e] : z[j][e], du = dt[j][e] * u;
-                    if (A.gate_mode == 2) {
-                        const float open = gate_act(g[j][e], A.act);
-                        dg[j][e] = du * gate_slope(g[j][e], open, A.act);
-                        dt[j][e] *= open;
-                    } else {
-                        if (live) acc[SUM_GATE][j][e] += du;
-                        dt[j][e] *= gc[j][e];
-                    }
-                }
-            if (A.gate_mode == 2 && live) R.template store<T>(A.dgate, row, A.dgate_ld, dg);
+        if (GATE) {
+            float u[NCH][VEC];
+            if (A.post) EACH(NCH, VEC) u[j][e] = z[j][e] * w1[j][e] + b1[j][e];
+            else EACH(NCH, VEC) u[j][e] = z[j][e];
+            EACH(NCH, VEC) u[j][e] *= dt[j][e];  // gradient of act(g)
+            if (GATE == 1) {
+                if (live) EACH(NCH, VEC) acc[SUM_GATE][j][e] += u[j][e];
+            } else {
+                R.get(gp, gc);
+                if (A.act == MARIUS_ACT_RELU) EACH(NCH, VEC) u[j][e] = gc[j][e] > 0.f ? u[j][e] : 0.f;
+                R.open(gc, A.act);
+                if (A.act == MARIUS_ACT_SIGMOID) EACH(NCH, VEC) u[j][e] *= gc[j][e] * (1.f - gc[j][e]);
+                if (live) R.template store<T>(A.dgate, row, A.dgate_ld, u);
+            }
+            EACH(NCH, VEC) dt[j][e] *= gc[j][e];
         }
         if (A.post) {
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    if (live) {
-                        acc[SUM_POST_W][j][e] += dt[j][e] * z[j][e];
-                        acc[SUM_POST_B][j][e] += dt[j][e];
-                    }
-                    dt[j][e] *= w1[j][e];
-                }
+            if (live) EACH(NCH, VEC) {
+                acc[SUM_POST_W][j][e] += dt[j][e] * z[j][e];
+                acc[SUM_POST_B][j][e] += dt[j][e];
+            }
+            EACH(NCH, VEC) dt[j][e] *= w1[j][e];
             R.gradient(dt, z, A, r);
         }
         if (live) R.template store<T>(A.dz, row, A.dz_ld, dt);
@@ -388,7 +361,7 @@ __global__ __launch_bounds__(1024) void residual_norm_sums_kernel(NormSumArgs A)
     }
 }
 
-// a row of up to 64 pieces of four elements stays in one wave, a longer one takes a workgroup of as many waves as hold it (two pieces a lane beyond 4096 elements)
+// a row of up to 64 pieces of four elements stays in one wave, a longer one takes a workgroup of as many waves as hold it (four pieces a lane beyond 4096 elements)
 struct NormShape {
     int vec, tpr, nch, threads;
     bool blk;
@@ -398,7 +371,7 @@ static NormShape norm_shape(int d) {
     const int units = (int)cdiv(d, s.vec);
     s.blk = units > 64;
     if (s.blk) {
-        s.nch = units > NORM_MAX_T ? 2 : 1;
+        s.nch = units > NORM_MAX_T ? 4 : 1;
         s.threads = s.tpr = (int)cdiv(cdiv(units, s.nch), 64) * 64;
     } else {
         while (s.tpr < units) s.tpr <<= 1;
@@ -410,20 +383,26 @@ static unsigned norm_groups(const NormShape& s, int64_t n, int most) {
     return (unsigned)(groups < most ? groups : most);
 }
 
-template <typename S, typename T>
-static void launch_norm(const NormArgs& A, const NormShape& s, bool backward, unsigned grid, hipStream_t st) {
+template <typename S, typename T, int GATE>
+static void launch_norm_gated(const NormArgs& A, const NormShape& s, bool backward, unsigned grid, hipStream_t st) {
     const dim3 g(grid), b(s.threads);
     if (backward) {
-        if (s.vec == 1) residual_norm_backward_kernel<S, T, 1, 1, false><<<g, b, 0, st>>>(A);
-        else if (!s.blk) residual_norm_backward_kernel<S, T, 4, 1, false><<<g, b, 0, st>>>(A);
-        else if (s.nch == 1) residual_norm_backward_kernel<S, T, 4, 1, true><<<g, b, 0, st>>>(A);
-        else residual_norm_backward_kernel<S, T, 4, 2, true><<<g, b, 0, st>>>(A);
+        if (s.vec == 1) residual_norm_backward_kernel<S, T, 1, 1, false, GATE><<<g, b, 0, st>>>(A);
+        else if (!s.blk) residual_norm_backward_kernel<S, T, 4, 1, false, GATE><<<g, b, 0, st>>>(A);
+        else if (s.nch == 1) residual_norm_backward_kernel<S, T, 4, 1, true, GATE><<<g, b, 0, st>>>(A);
+        else residual_norm_backward_kernel<S, T, 4, 4, true, GATE><<<g, b, 0, st>>>(A);
     } else {
-        if (s.vec == 1) residual_norm_kernel<S, T, 1, 1, false><<<g, b, 0, st>>>(A);
-        else if (!s.blk) residual_norm_kernel<S, T, 4, 1, false><<<g, b, 0, st>>>(A);
-        else if (s.nch == 1) residual_norm_kernel<S, T, 4, 1, true><<<g, b, 0, st>>>(A);
-        else residual_norm_kernel<S, T, 4, 2, true><<<g, b, 0, st>>>(A);
+        if (s.vec == 1) residual_norm_kernel<S, T, 1, 1, false, GATE><<<g, b, 0, st>>>(A);
+        else if (!s.blk) residual_norm_kernel<S, T, 4, 1, false, GATE><<<g, b, 0, st>>>(A);
+        else if (s.nch == 1) residual_norm_kernel<S, T, 4, 1, true, GATE><<<g, b, 0, st>>>(A);
+        else residual_norm_kernel<S, T, 4, 4, true, GATE><<<g, b, 0, st>>>(A);
     }
+}
+template <typename S, typename T>
+static void launch_norm(const NormArgs& A, const NormShape& s, bool backward, unsigned grid, hipStream_t st) {
+    if (A.gate_mode == 0) launch_norm_gated<S, T, 0>(A, s, backward, grid, st);
+    else if (A.gate_mode == 1) launch_norm_gated<S, T, 1>(A, s, backward, grid, st);
+    else launch_norm_gated<S, T, 2>(A, s, backward, grid, st);
 }
 static void launch_norm_typed(const NormArgs& A, const NormShape& s, int stream_type, int type, bool backward, unsigned grid, hipStream_t st) {
     if (type == MARIUS_F32) launch_norm<float, float>(A, s, backward, grid, st);
