@@ -711,95 +711,31 @@ def segment_adagrad_scatter_group(jobs):
 
 
 # ------------------------------------------------------------------------------------------------ the training block of an attention encoder
-FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # MARIUS_F32 / BF16 / F16
-NORM = {"RMS": 0, "LAYER": 1}
+# The calls below are made by the host module (csrc/host/encoder_ops.cpp: checks, outputs, workspaces), which is given the addresses of the entry points here.
+_host_ops = None
+
+
+def _ops():
+    global _host_ops
+    if _host_ops is None:
+        from . import host
+
+        _host_ops = host()
+    return _host_ops
+
+
+def _entry(name):
+    """the address of an entry point of the loaded library"""
+    known = lib().__dict__
+    address = known.get("&" + name)
+    if address is None:
+        address = known["&" + name] = C.cast(getattr(lib(), name), C.c_void_p).value
+    return address
 
 
 def _require(ok, message, *args):
     if not ok:
         raise MariusHipError(message % args)
-
-
-def _same_device(first, **tensors):
-    """every tensor on the device of `first`, which has to be a GPU"""
-    _dev(first)
-    for name, t in tensors.items():
-        _require(t is None or t.device == first.device, "%s is on %s, the call is on %s", name, None if t is None else t.device, first.device)
-
-
-def _type_of(name, t):
-    _require(t.dtype in FLOAT_TYPES, "%s: float32, bfloat16 or float16 required, got %s", name, t.dtype)
-    return FLOAT_TYPES[t.dtype]
-
-
-class _on:
-    """the device of `t` current for the launches inside (a launch goes to the current device)"""
-
-    def __init__(self, t):
-        self.guard = torch.cuda.device(t.device) if t.is_cuda and t.device.index != torch.cuda.current_device() else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
-def _matrix(t):
-    """`t` [n, d] as rows of contiguous elements that do not overlap (a copy where it is not laid out so)"""
-    return t if t.size(1) <= 1 and t.is_contiguous() or t.stride(1) == 1 and (t.stride(0) >= t.size(1) or t.size(0) <= 1) else t.contiguous()
-
-
-def _ld(t):
-    return 0 if t is None else max(t.stride(0), t.size(1))
-
-
-def _norm_desc(stream, block, gate, weights, post_norm, pre_norm, kind, eps, residual_scale, gate_activation):
-    """the checked descriptor of a residual norm over the stream rows; `weights`: (post_weight, post_bias, pre_weight, pre_bias)"""
-    _require(stream.dim() == 2, "residual_norm: rows [n, d] required, got %s", list(stream.shape))
-    n, d = stream.shape
-    _require(kind in NORM, "residual_norm: kind is one of %s", sorted(NORM))
-    _require(gate_activation in ACT, "Unsupported activation function")
-    _require(block is not None or pre_norm, "residual_norm: neither a block nor a norm: nothing to compute")
-    _require(block is not None or (not post_norm and gate is None), "residual_norm: a post norm and a gate need a block")
-    _require(block is not None or residual_scale == 1.0, "residual_norm: a residual scale needs a block")
-    _require(block is None or block.shape == stream.shape, "residual_norm: block and stream differ in shape")
-    names = ("post_weight", "post_bias", "pre_weight", "pre_bias")
-    _same_device(stream, block=block, gate=gate, **dict(zip(names, weights)))
-    m = ResidualNorm(n=n, d=d, stream_type=_type_of("stream", stream), kind=NORM[kind], post_norm=bool(post_norm), pre_norm=bool(pre_norm), has_block=block is not None,
-                     gate_activation=ACT[gate_activation], eps=eps, residual_scale=residual_scale)
-    m.type = m.stream_type if block is None else _type_of("block", block)
-    _require(m.stream_type in (m.type, 0), "residual_norm: the stream is float32 or of the block's type (%s)", None if block is None else block.dtype)
-    params = []
-    for name, t, there in zip(names, weights, (post_norm, post_norm, pre_norm, pre_norm)):
-        if t is not None:
-            _require(there, "residual_norm: %s of a norm that is not there", name)
-            _require(t.shape == (d,), "residual_norm: %s has shape %s, rows have %d elements", name, list(t.shape), d)
-            params.append(t)
-    keep = []
-    if gate is not None:
-        _require(gate.shape in ((d,), (n, d)), "residual_norm: gate is [d] or [n, d], got %s", list(gate.shape))
-        if gate.dim() == 1:
-            m.gate_mode = 1
-            params.append(gate)
-        else:
-            _require(gate.dtype == block.dtype, "residual_norm: an element gate is of the block's type, got %s", gate.dtype)
-            gate = _matrix(gate)
-            m.gate_mode, m.gate_ld = 2, _ld(gate)
-    m.param_type = _type_of("weights", params[0]) if params else 0
-    _require(all(t.dtype == params[0].dtype for t in params), "residual_norm: weights, biases and a channel gate are of one type")
-    for name, t in zip(names, weights):
-        if t is not None:
-            t = t.contiguous()
-            keep.append(t)
-            setattr(m, name, t.data_ptr())
-    if gate is not None:
-        gate = gate.contiguous() if m.gate_mode == 1 else gate
-        keep.append(gate)
-        m.gate = gate.data_ptr()
-    return m, keep
 
 
 def residual_norm(x, block=None, gate=None, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, *, post_norm=False, pre_norm=True, kind="RMS", eps=1e-6,
@@ -808,17 +744,8 @@ def residual_norm(x, block=None, gate=None, post_weight=None, post_bias=None, pr
     (None otherwise).  x [n, d]: the residual stream, float32 or of the block's type, which y takes; gate [d] (of the weights' type) or [n, d] (of the block's);
     h is of the block's type.  Without a block h = norm(x) and y is x itself."""
     _dev(x)
-    m, keep = _norm_desc(x, block, gate, (post_weight, post_bias, pre_weight, pre_bias), post_norm, pre_norm, kind, eps, residual_scale, gate_activation)
-    n, d = x.shape
-    _require(n == 0 or 1 <= d <= 8192, "residual_norm: rows of 1 to 8192 elements, got %d", d)
-    y = x if block is None else torch.empty((n, d), dtype=x.dtype, device=x.device)
-    h = torch.empty((n, d), dtype=x.dtype if block is None else block.dtype, device=x.device) if pre_norm else None
-    if x.numel() == 0:
-        return y, h
-    xs, bs = _matrix(x), None if block is None else _matrix(block)
-    with _on(x):
-        check(lib().marius_residual_norm_forward(C.byref(m), ptr(xs), _ld(xs), ptr(bs), _ld(bs), None if block is None else ptr(y), d, ptr(h), d, stream_ptr()), "residual_norm")
-    return y, h
+    return _ops().residual_norm(_entry("marius_residual_norm_forward"), x, block, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, kind, eps, residual_scale,
+                                gate_activation)
 
 
 def residual_norm_backward(grad_y, grad_h, y, block=None, gate=None, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, *, post_norm=False, pre_norm=True,
@@ -826,33 +753,8 @@ def residual_norm_backward(grad_y, grad_h, y, block=None, gate=None, post_weight
     """Gradients of residual_norm from those of y and h (either may be None: zero), the stored y and the block: a dict of dx, dblock, dgate, dpost_weight, dpost_bias,
     dpre_weight, dpre_bias, None where the argument is.  Sums over rows are added in a fixed order (the same bits on every run)."""
     _dev(y)
-    weights = (post_weight, post_bias, pre_weight, pre_bias)
-    m, keep = _norm_desc(y, block, gate, weights, post_norm, pre_norm, kind, eps, residual_scale, gate_activation)
-    n, d = y.shape
-    out_type = y.dtype if block is None else block.dtype
-    _require(n == 0 or 1 <= d <= 8192, "residual_norm_backward: rows of 1 to 8192 elements, got %d", d)
-    _same_device(y, grad_y=grad_y, grad_h=grad_h)
-    _require(grad_y is None or (grad_y.shape == y.shape and grad_y.dtype == y.dtype), "residual_norm_backward: grad_y is not like y")
-    _require(grad_h is None or (pre_norm and grad_h.shape == y.shape and grad_h.dtype == out_type), "residual_norm_backward: grad_h is not like h")
-    _require(grad_y is not None or grad_h is not None, "residual_norm_backward: no gradient to go back from")
-    like = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-    got = {"dx": torch.empty((n, d), dtype=y.dtype, device=y.device) if need_dx else None,
-           "dblock": None if block is None else torch.empty((n, d), dtype=out_type, device=y.device), "dgate": like(gate)}
-    for name, t in zip(("dpost_weight", "dpost_bias", "dpre_weight", "dpre_bias"), weights):
-        got[name] = like(t)
-    if d == 0:
-        return got
-    gy, gh, ys, bs = (None if t is None else _matrix(t) for t in (grad_y, grad_h, y, block))
-    g = ResidualNormGrads(grad_y_ld=_ld(gy), grad_h_ld=_ld(gh), dx_ld=d, dblock_ld=d, dgate_ld=d)
-    g.grad_y, g.grad_h = ptr(gy), ptr(gh)
-    for name, t in got.items():
-        setattr(g, name, ptr(t))
-    sums = m.gate_mode == 1 or any(t is not None for t in weights)
-    wsb = lib().marius_residual_norm_workspace_bytes(n, d) if sums else 0
-    ws = torch.empty(wsb, dtype=torch.uint8, device=y.device) if wsb else None
-    with _on(y):
-        check(lib().marius_residual_norm_backward(C.byref(m), C.byref(g), ptr(ys), _ld(ys), ptr(bs), _ld(bs), ptr(ws), wsb, stream_ptr()), "residual_norm_backward")
-    return got
+    return _ops().residual_norm_backward(_entry("marius_residual_norm_backward"), _entry("marius_residual_norm_workspace_bytes"), grad_y, grad_h, y, block, gate, post_weight, post_bias,
+                                         pre_weight, pre_bias, post_norm, pre_norm, kind, eps, residual_scale, gate_activation, need_dx)
 
 
 def plan_chunk(entries):
@@ -870,7 +772,7 @@ class NeighborPlan:
 
     def __init__(self, index, offsets, num_rows, index_b=None, offsets_b=None, self_offset=None):
         _dev(index)
-        _same_device(index, offsets=offsets, index_b=index_b, offsets_b=offsets_b)
+        _require(all(t is None or t.device == index.device for t in (offsets, index_b, offsets_b)), "NeighborPlan: index and offsets are on one device")
         _require((index_b is None) == (offsets_b is None), "NeighborPlan: a second list has both index and offsets")
         lists = [index, offsets] + ([] if index_b is None else [index_b, offsets_b])
         _require(all(t.dtype == torch.int64 and t.dim() == 1 for t in lists), "NeighborPlan: index and offsets are int64 vectors")
@@ -885,7 +787,7 @@ class NeighborPlan:
         offs, self._index, owner = torch.zeros(n + 1, **i32), torch.empty(total + spare, **i32), torch.empty(total, **i32)
         keys, status = torch.empty(total, dtype=torch.int64, device=dev), torch.zeros(4, **i32)
         L = lib()
-        with _on(index):
+        with torch.cuda.device(dev if dev.type == "cuda" else -1):  # (launches go to the current device)
             wsb = max(L.marius_nbr_plan_workspace_bytes(n), L.marius_nbr_plan_workspace_bytes(num_rows))
             ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
             check(L.marius_nbr_plan_lists(ptr(lists[0]), ptr(lists[1]), ta, ptr(lists[2]), ptr(lists[3]), tb, n, num_rows, own, ptr(offs), ptr(self._index), ptr(owner),
@@ -913,6 +815,7 @@ class NeighborPlan:
         self.n, self.num_rows, self.num_entries, self.device, self.owner, self.offsets = n, num_rows, total, dev, owner, offs
         self.index = self._index[:total]
         self.desc = NeighborPlanDesc(n=n, rows=num_rows, T=total)
+        self.address = C.addressof(self.desc)
         d = self.desc
         d.index, d.items, d.splits, d.r_owner, d.r_entry, d.r_items, d.r_splits = (t.data_ptr() for t in (self._index, self._items, self._splits, self._r_owner, self._r_entry,
                                                                                                         self._r_items, self._r_splits))
@@ -935,29 +838,9 @@ class NeighborPlan:
         return first[owner] + torch.arange(total, device=self.device) - starts[owner]
 
 
-def _heads(t):
-    return t if t.stride(2) == 1 else t.contiguous()
-
-
-def _attention_desc(q, k, v, plan, scale, bias, stats):
+def _plan(plan):
     _require(isinstance(plan, NeighborPlan), "neighbor_attention: a NeighborPlan is needed")
-    _same_device(q, k=k, v=v, bias=bias, stats=stats)
-    _require(plan.device == q.device, "neighbor_attention: the plan is on %s, the rows are on %s", plan.device, q.device)
-    _require(q.dim() == 3 and k.dim() == 3 and v.shape == k.shape, "neighbor_attention: q [n, heads, dim] and k, v [rows, kv_heads, dim] required")
-    n, H, D = q.shape
-    _require(n == plan.n and k.size(0) == plan.num_rows, "neighbor_attention: the plan has %d targets over %d rows, got %d and %d", plan.n, plan.num_rows, n, k.size(0))
-    _require(k.size(2) == D and 1 <= D <= 256, "neighbor_attention: heads of 1 to 256 elements, the same in q, k and v")
-    _require(k.size(1) > 0 and H > 0 and H % k.size(1) == 0 and H <= 1024, "neighbor_attention: query heads (up to 1024) are a multiple of the key heads")
-    _require(k.dtype == q.dtype and v.dtype == q.dtype, "neighbor_attention: q, k and v are of one type")
-    m = NeighborAttention(heads=H, kv_heads=k.size(1), dim=D, type=_type_of("q", q), scale=D ** -0.5 if scale is None else scale)
-    q, k, v = _heads(q), _heads(k), _heads(v)
-    m.q, m.k, m.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    m.q_row, m.q_head, m.k_row, m.k_head, m.v_row, m.v_head = q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1)
-    if bias is not None:
-        _require(bias.shape == (plan.num_entries, H) and bias.dtype == torch.float32, "neighbor_attention: bias is float32 [%d, %d]", plan.num_entries, H)
-        bias = bias.contiguous()
-        m.bias = bias.data_ptr()
-    return m, (q, k, v, bias)
+    return plan
 
 
 def neighbor_attention(q, k, v, plan, scale=None, bias=None):
@@ -966,104 +849,36 @@ def neighbor_attention(q, k, v, plan, scale=None, bias=None):
     given.  bias [entries, heads] float32 is added to the scores, -inf masks an entry.  A list without a live entry gives zeros.  stats (a list's largest score, the
     log of its sum) is what the backward pass needs; their sum is the log-sum-exp."""
     _dev(q)
-    m, keep = _attention_desc(q, k, v, plan, scale, bias, None)
-    n, H, D = q.shape
-    out, stats = torch.empty((n, H, D), dtype=q.dtype, device=q.device), torch.empty((n, H, 2), dtype=torch.float32, device=q.device)
-    m.stats = stats.data_ptr()
-    with _on(q):
-        wsb = lib().marius_neighbor_attention_workspace_bytes(C.byref(plan.desc), H, m.kv_heads, D, 0)
-        ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
-        check(lib().marius_neighbor_attention_forward(C.byref(plan.desc), C.byref(m), ptr(out), ptr(ws), wsb, stream_ptr()), "neighbor_attention")
-    return out, stats
+    return _ops().neighbor_attention(_entry("marius_neighbor_attention_forward"), _entry("marius_neighbor_attention_workspace_bytes"), _plan(plan).address, plan.index, q, k, v, scale, bias)
 
 
 def neighbor_attention_backward(grad_out, q, k, v, stats, plan, scale=None, bias=None, need_dbias=True):
     """(dq, dk, dv, dbias) of neighbor_attention, the probabilities recomputed from `stats`; dbias is None without a bias (or where not needed).  Rows that no list names
     get zero gradients.  No atomics: the same bits on every run."""
     _dev(q)
-    m, keep = _attention_desc(q, k, v, plan, scale, bias, stats)
-    n, H, D = q.shape
-    _same_device(q, grad_out=grad_out)
-    _require(grad_out.shape == q.shape and grad_out.dtype == q.dtype, "neighbor_attention_backward: grad_out is not like the output")
-    _require(stats.shape == (n, H, 2) and stats.dtype == torch.float32, "neighbor_attention_backward: stats is float32 [%d, %d, 2]", n, H)
-    grad_out, stats = _heads(grad_out), stats.contiguous()
-    m.stats = stats.data_ptr()
-    dq = torch.empty((n, H, D), dtype=q.dtype, device=q.device)
-    dk, dv = (torch.empty((plan.num_rows, m.kv_heads, D), dtype=q.dtype, device=q.device) for _ in range(2))
-    dbias = torch.empty(bias.shape, dtype=torch.float32, device=q.device) if bias is not None and need_dbias else None
-    with _on(q):
-        wsb = lib().marius_neighbor_attention_workspace_bytes(C.byref(plan.desc), H, m.kv_heads, D, 1)
-        ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
-        check(lib().marius_neighbor_attention_backward(C.byref(plan.desc), C.byref(m), ptr(grad_out), grad_out.stride(0), grad_out.stride(1), ptr(dq), ptr(dk), ptr(dv), ptr(dbias),
-                                                       ptr(ws), wsb, stream_ptr()), "neighbor_attention_backward")
-    return dq, dk, dv, dbias
+    return _ops().neighbor_attention_backward(_entry("marius_neighbor_attention_backward"), _entry("marius_neighbor_attention_workspace_bytes"), _plan(plan).address, plan.index, grad_out,
+                                              q, k, v, stats, scale, bias, need_dbias)
 
 
 ADAMW_BLOCK = 256  # elements of an 8-bit state that share a scale
 
 
-class AdamWTensors:
+def AdamWTensors(params, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_avg_sq_scales=None):
     """The parameter tensors of an optimizer with their states, for adamw_step: parameters of one type (float32, bfloat16, float16), contiguous, on one device.
     States: float32 like the parameter, or (8 bits) float8_e4m3fn codes with float32 scales [ceil(n / 256)], exp_avg_sq then holding the ROOT of the second moment."""
-
-    def __init__(self, params, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_avg_sq_scales=None):
-        self.params = list(params)
-        _require(len(self.params) > 0, "AdamWTensors: no parameters")
-        _require((exp_avg_scales is None) == (exp_avg_sq_scales is None), "AdamWTensors: lists of different lengths")
-        self.states = [list(exp_avgs), list(exp_avg_sqs)] + ([] if exp_avg_scales is None else [list(exp_avg_scales), list(exp_avg_sq_scales)])
-        _require(all(len(s) == len(self.params) for s in self.states), "AdamWTensors: lists of different lengths")
-        self.bits = 32 if exp_avg_scales is None else 8
-        first = self.params[0]
-        _dev(first)
-        self.device, self.type, self.dtype = first.device, _type_of("parameters", first), first.dtype
-        import numpy as np
-
-        self.table = np.zeros((len(self.params), 7), dtype=np.int64)  # marius_adamw_tensor, row by row
-        for i, p in enumerate(self.params):
-            mine = [s[i] for s in self.states]
-            _require(p.dtype == self.dtype and p.is_contiguous(), "AdamWTensors: parameter %d is not a contiguous %s tensor", i, self.dtype)
-            _require(all(t.device == self.device and t.is_contiguous() for t in [p] + mine), "AdamWTensors: tensors of parameter %d are contiguous and on %s", i, self.device)
-            kind = torch.float32 if self.bits == 32 else torch.float8_e4m3fn
-            _require(all(t.dtype == kind and t.numel() == p.numel() for t in mine[:2]), "AdamWTensors: states of parameter %d are %s of its size", i, kind)
-            _require(all(t.dtype == torch.float32 and t.numel() == -(-p.numel() // ADAMW_BLOCK) for t in mine[2:]), "AdamWTensors: scales of parameter %d are float32, one for %d",
-                     i, ADAMW_BLOCK)
-            self.table[i, 2:2 + len(mine)] = [t.data_ptr() for t in mine]
-        self.sizes = [p.numel() for p in self.params]
+    params = list(params)
+    if params:
+        _dev(params[0])
+    return _ops().AdamWTensors(params, list(exp_avgs), list(exp_avg_sqs), exp_avg_scales, exp_avg_sq_scales)
 
 
 def adamw_step(tensors, grads, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2, grad_scale=None):
     """One AdamW step over all tensors of an AdamWTensors (marius_adamw_step), in place.  grads: one per parameter, of one type; None leaves its parameter and states as
     they are.  step counts from 1: a number, or an int64 device tensor of one element (a captured call has to take that: a replay reads it anew).  grad_scale: float32
     device tensor of one element every gradient is multiplied by (a clipping factor, the inverse of a loss scale)."""
-    _require(isinstance(tensors, AdamWTensors), "adamw_step: AdamWTensors are needed")
-    grads = list(grads)
-    _require(len(grads) == len(tensors.params), "adamw_step: %d gradients for %d parameters", len(grads), len(tensors.params))
-    kind, dev, table, keep = None, tensors.device, tensors.table, []
-    for i, (g, p) in enumerate(zip(grads, tensors.params)):
-        if g is None:
-            table[i, 6] = 0
-            continue
-        if kind is None:
-            kind = g.dtype
-        if g.dtype != kind or g.device != dev or g.numel() != tensors.sizes[i]:
-            raise MariusHipError("adamw_step: gradient %d is not a %s tensor of %d elements on %s" % (i, kind, tensors.sizes[i], dev))
-        if p.device != dev or p.dtype != tensors.dtype or p.numel() != tensors.sizes[i] or not p.is_contiguous():
-            raise MariusHipError("adamw_step: parameter %d is no longer what the states were made for" % i)
-        if not g.is_contiguous():
-            g = g.contiguous()
-            keep.append(g)
-        table[i, 0], table[i, 1], table[i, 6] = p.data_ptr(), g.data_ptr(), tensors.sizes[i]
-    if kind is None:
-        return
-    _require(kind in FLOAT_TYPES, "adamw_step: float32, bfloat16 or float16 gradients required, got %s", kind)
-    on_device = isinstance(step, torch.Tensor)
-    _require(not on_device or (step.dtype == torch.int64 and step.numel() == 1 and step.device == dev), "adamw_step: a step on the device is one int64 on %s", dev)
-    _require(grad_scale is None or (grad_scale.dtype == torch.float32 and grad_scale.numel() == 1 and grad_scale.device == dev), "adamw_step: grad_scale is one float32 on %s", dev)
-    with _on(tensors.params[0]):
-        _require(on_device or not (dev.type == "cuda" and torch.cuda.is_current_stream_capturing()),
-                 "adamw_step: a captured step needs its number on the device (a replay would repeat this one's)")
-        check(lib().marius_adamw_step(C.c_void_p(table.ctypes.data), len(grads), tensors.type, FLOAT_TYPES[kind], tensors.bits, 0 if on_device else int(step),
-                                      ptr(step) if on_device else None, lr, beta1, beta2, eps, weight_decay, ptr(grad_scale), stream_ptr()), "adamw_step")
+    _require(isinstance(tensors, _ops().AdamWTensors), "adamw_step: AdamWTensors are needed")
+    _ops().adamw_step(_entry("marius_adamw_step"), tensors, grads, step, lr, beta1, beta2, eps, weight_decay, grad_scale,
+                      torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing())
 
 
 def profile_enable(on=True, only=None):
