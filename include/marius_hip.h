@@ -622,7 +622,8 @@ typedef struct marius_neighbor_plan {
 } marius_neighbor_plan;
 
 /* Attention of the targets over their lists (nbr_attention.hip): s_e = scale * q_i . k_j + bias_e per query head, o_i = sum softmax(s)_e v_j; heads is a multiple
- * of kv_heads (query heads h and key head h / (heads / kv_heads)), heads of 1 to 256 elements, contiguous; row and head strides in elements are the caller's.
+ * of kv_heads (query heads h and key head h / (heads / kv_heads)), heads of 1 to 256 elements, contiguous; row and head strides in elements are the caller's (rows
+ * at most 4 GiB apart).
  * bias [T, heads] fp32 or NULL, in the plan's entry order; -inf masks an entry: its key and value are not used.  A list without a live entry gives o = 0.
  * stats [n, heads, 2] fp32, written by the forward and read by the backward pass: largest score (-inf: none) and the log of the sum of exp(score - largest).
  * Forward: out [n, heads, dim].  Backward: dq [n, heads, dim], dk / dv [rows, kv_heads, dim] (contiguous; rows that no list names get zero), dbias [T, heads] or NULL.

@@ -16,6 +16,8 @@
 // them is how many dependent loads (item -> row number -> row) are in flight.  UN entries are loaded at a time, the next ones' numbers while these are
 // computed.  Parts of a long list are written as partial results and joined by a second launch in order.
 // Bound by the gather of rows: 2 rows per entry in each of the three sweeps.
+#include <type_traits>
+
 #include "row_types.h"
 
 namespace marius {
@@ -24,8 +26,9 @@ constexpr float NA_INF = __builtin_inff();
 constexpr int NA_WAVES = 4;
 
 struct NaArgs {
-    const void *q, *k, *v, *go;
-    int64_t q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, go_ld, go_hd;   // row and head strides, elements
+    const char *q, *k, *v, *go;
+    int64_t q_hd, k_hd, v_hd, go_hd;                            // head strides, bytes
+    uint32_t q_ld, k_ld, v_ld, go_ld;                           // row strides, bytes (an address is one multiply-add of 32 bits by 32 on 64)
     const float* bias;                                          // [T, H] or NULL
     float *out_bias, *stats, *part;
     float2* part2;                                              // a part's (m, sum), or its delta
@@ -38,12 +41,78 @@ struct NaArgs {
     float scale;
 };
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// A lane's part of a head's row, and what of it is the lane's own.  Elements that are a neighbour's are cleared where the row does not fill its lanes (`tail`, the
+// same for a whole launch), in every row that is loaded: they add nothing to sums over the row and nothing is stored for them.
+template <typename T, int VEC, int LPH>
+struct Part {
+    int at, first;
+    bool tail;
+    uint32_t mask[(sizeof(T) * VEC + 3) / 4];
+    __device__ __forceinline__ Part(int l, int D) : tail(D != LPH * VEC) {
+        const Place<VEC> p(l, D);
+        at = p.at;
+        first = p.first;
+        constexpr int PER = sizeof(T) >= 4 ? 1 : 4 / (int)sizeof(T);  // elements of a word
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(mask) / 4); ++i) {
+            mask[i] = 0;
+#pragma unroll
+            for (int e = 0; e < PER && i * PER + e < VEC; ++e) mask[i] |= i * PER + e >= first ? (PER == 1 ? ~0u : 0xffffu << (16 * e)) : 0u;
+        }
+    }
+    __device__ __forceinline__ void leave_own(Piece<T, VEC>& p) const {
+        if (!tail) return;
+        uint32_t w[sizeof(mask) / 4] = {};
+        __builtin_memcpy(w, p.t, sizeof(p.t));
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(mask) / 4); ++i) w[i] &= mask[i];
+        __builtin_memcpy(p.t, w, sizeof(p.t));
+    }
+    template <typename O>
+    __device__ __forceinline__ void store(O* p, const float (&v)[VEC]) const {
+        if (!tail || first == 0) {
+            put<O, VEC>(p + at, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (e >= first) p[at + e] = (O)v[e];
+        }
+    }
+};
+// a row that stays in registers for products with many others: bf16 as it is (a product of pairs is one instruction; products are exact, sums fp32), the others as fp32
+template <typename T, int VEC>
+struct Fixed {
+    static constexpr bool PAIRS = std::is_same<T, __bf16>::value && VEC % 2 == 0;
+    Piece<T, VEC> raw;
+    float f[PAIRS ? 1 : VEC];
+    __device__ __forceinline__ void set(const Piece<T, VEC>& p) {
+        raw = p;
+        if constexpr (!PAIRS) p.get(f);
+    }
+    __device__ __forceinline__ float dot(const Piece<T, VEC>& o) const {
+        float s = 0.f;
+        if constexpr (PAIRS) {
+            bf16x2 a[VEC / 2], b[VEC / 2];
+            __builtin_memcpy(a, raw.t, sizeof(a));
+            __builtin_memcpy(b, o.t, sizeof(b));
+#pragma unroll
+            for (int e = 0; e < VEC / 2; ++e) s = __builtin_amdgcn_fdot2_f32_bf16(a[e], b[e], s, false);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s += f[e] * (float)o.t[e];
+        }
+        return s;
+    }
+};
 // weight of a running sum that goes from maximum m to `ref`; a maximum of -inf has weight zero
 __device__ __forceinline__ float weight_to(float m, float ref) { return m == -NA_INF ? 0.f : __expf(m - ref); }
 __device__ __forceinline__ float finite_ref(float m) { return m == -NA_INF ? 0.f : m; }
+__device__ __forceinline__ const char* row_at(const char* base, int row, uint32_t ld) { return base + (uint64_t)(uint32_t)row * ld; }
 
 // which item, head and piece a lane works on
-template <int VEC, int LPH>
+template <int LPH>
 struct Lane {
     int l, h, slot;
     bool head;
@@ -57,33 +126,35 @@ struct Lane {
     }
 };
 template <int UN>
-__device__ __forceinline__ void load_numbers(const int32_t* p, int (&v)[UN]) { __builtin_memcpy(v, p, sizeof(v)); }  // (lists end with UN spare entries)
+__device__ __forceinline__ void load_numbers(const int32_t* p, int (&v)[UN]) { __builtin_memcpy(v, p, sizeof(v)); }  // (lists end with four spare entries)
+// biases of UN entries from t on, for one head; behind the list -inf
+template <int UN>
+__device__ __forceinline__ void load_biases(const NaArgs& A, int t, int end, int h, float (&b)[UN]) {
+#pragma unroll
+    for (int u = 0; u < UN; ++u) b[u] = t + u < end ? A.bias[(uint64_t)(uint32_t)(t + u) * (uint32_t)A.H + h] : -NA_INF;
+}
 
 // ---------------------------------------------------------------------------------------------------------------- forward
 template <typename T, int VEC, int LPH, bool BIAS>
 __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_kernel(NaArgs A) {
     constexpr int UN = 4;
-    const Lane<VEC, LPH> w(A, A.H);
+    const Lane<LPH> w(A, A.H);
     if (w.slot >= A.n_items || !w.head) return;
     const int4 it = A.items[w.slot];
-    const Place<VEC> at(w.l, A.D, A.D != LPH * VEC);
+    const Part<T, VEC, LPH> part(w.l, A.D);
     const int kv = w.h / (A.H / A.Hkv);
-    float q[VEC], acc[VEC], m = -NA_INF, sum = 0.f, bias[UN];
+    float acc[VEC], m = -NA_INF, sum = 0.f, bias[UN];
     Piece<T, VEC> raw;
-    raw.load((const T*)A.q + (int64_t)it.x * A.q_ld + w.h * A.q_hd + at.at);
-    raw.get(q);
-    at.leave_own(q);
+    Fixed<T, VEC> q;
+    raw.load((const T*)(row_at(A.q, it.x, A.q_ld) + w.h * A.q_hd) + part.at);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        q[e] *= A.scale;
-        acc[e] = 0.f;
-    }
-    const T *kp = (const T*)A.k + kv * A.k_hd + at.at, *vp = (const T*)A.v + kv * A.v_hd + at.at;
+    for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+    const char *kp = A.k + kv * A.k_hd + part.at * sizeof(T), *vp = A.v + kv * A.v_hd + part.at * sizeof(T);
     int next[UN];
     load_numbers<UN>(A.index + it.y, next);
-    if (BIAS)
-#pragma unroll
-        for (int u = 0; u < UN; ++u) bias[u] = it.y + u < it.z ? A.bias[(int64_t)(it.y + u) * A.H + w.h] : -NA_INF;
+    if (BIAS) load_biases<UN>(A, it.y, it.z, w.h, bias);
+    part.leave_own(raw);
+    q.set(raw);
     for (int t = it.y; t < it.z; t += UN) {
         Piece<T, VEC> kk[UN], vv[UN];
         float s[UN];
@@ -91,9 +162,9 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_kernel(NaArgs A) 
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
             ok[u] = t + u < it.z;
-            const int64_t j = ok[u] ? next[u] : next[0];  // (behind the list: its last rows once more, computed on by nobody)
-            kk[u].load(kp + j * A.k_ld);
-            vv[u].load(vp + j * A.v_ld);
+            const int j = ok[u] ? next[u] : next[0];  // (behind the list: its last rows once more, computed on by nobody)
+            kk[u].load((const T*)row_at(kp, j, A.k_ld));
+            vv[u].load((const T*)row_at(vp, j, A.v_ld));
             s[u] = 0.f;
             if (BIAS) {
                 s[u] = bias[u];
@@ -102,19 +173,13 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_kernel(NaArgs A) 
         }
         if (t + UN < it.z) {
             load_numbers<UN>(A.index + t + UN, next);
-            if (BIAS)
-#pragma unroll
-                for (int u = 0; u < UN; ++u) bias[u] = t + UN + u < it.z ? A.bias[(int64_t)(t + UN + u) * A.H + w.h] : -NA_INF;
+            if (BIAS) load_biases<UN>(A, t + UN, it.z, w.h, bias);
         }
         float top = m;
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
-            float k[VEC], d = 0.f;
-            kk[u].get(k);
-            at.leave_own(k);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) d += q[e] * k[e];
-            d = group_sum<LPH>(d);
+            part.leave_own(kk[u]);
+            const float d = group_sum<LPH>(q.dot(kk[u])) * A.scale;
             s[u] = ok[u] ? d + s[u] : -NA_INF;
             top = fmaxf(top, s[u]);
         }
@@ -128,22 +193,21 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_kernel(NaArgs A) 
             if (!ok[u]) continue;
             const float p = __expf(s[u] - ref);
             sum += p;
-            float v[VEC];
-            vv[u].get(v);
+            part.leave_own(vv[u]);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] += p * v[e];
+            for (int e = 0; e < VEC; ++e) acc[e] += p * (float)vv[u].t[e];
         }
     }
     if (it.w >= 0) {
         const int64_t o = (int64_t)it.w * A.H + w.h;
-        put<float, VEC>(A.part + o * A.D + at.at, acc);
+        part.store(A.part + o * A.D, acc);
         if (w.l == 0) A.part2[o] = make_float2(m, sum);
     } else {
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // (NaN stays)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] *= inv;
         const int64_t o = (int64_t)it.x * A.H + w.h;
-        put<T, VEC>((T*)A.out + o * A.D + at.at, acc);
+        part.store((T*)A.out + o * A.D, acc);
         if (w.l == 0) {
             A.stats[o * 2] = m;
             A.stats[o * 2 + 1] = sum == 0.f ? 0.f : logf(sum);
@@ -158,7 +222,7 @@ __global__ __launch_bounds__(64 * NA_JOIN) void nbr_attention_join_kernel(NaArgs
     __shared__ float red[NA_JOIN][VEC + 2][64];
     const int4 sp = A.splits[blockIdx.x];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = blockIdx.y * (64 / LPH) + lane / LPH, hc = h < A.H ? h : A.H - 1;
-    const Place<VEC> at(lane & (LPH - 1), A.D, A.D != LPH * VEC);
+    const Part<T, VEC, LPH> part(lane & (LPH - 1), A.D);
     float acc[VEC], m = -NA_INF, sum = 0.f;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
@@ -173,7 +237,7 @@ __global__ __launch_bounds__(64 * NA_JOIN) void nbr_attention_join_kernel(NaArgs
     for (int s = wave; s < sp.z; s += NA_JOIN) {
         const int64_t o = (int64_t)(sp.y + s) * A.H + hc;
         float v[VEC];
-        __builtin_memcpy(v, A.part + o * A.D + at.at, sizeof(v));
+        __builtin_memcpy(v, A.part + o * A.D + part.at, sizeof(v));
         const float2 ms = A.part2[o];
         join(ms.x, ms.y, v);
     }
@@ -193,15 +257,15 @@ __global__ __launch_bounds__(64 * NA_JOIN) void nbr_attention_join_kernel(NaArgs
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] *= inv;
     const int64_t o = (int64_t)sp.x * A.H + h;
-    put<T, VEC>((T*)A.out + o * A.D + at.at, acc);
+    part.store((T*)A.out + o * A.D, acc);
     if ((lane & (LPH - 1)) == 0) {
         A.stats[o * 2] = m;
         A.stats[o * 2 + 1] = sum == 0.f ? 0.f : logf(sum);
     }
 }
 // the same for sums: two rows of D, and (`more`) a number of their own; true for the lanes that hold the result
-template <int VEC, int LPH>
-__device__ __forceinline__ bool join_sums(const NaArgs& A, int heads, bool more, const Place<VEC>& at, int h, float (&a)[VEC], float (&b)[VEC], float& first) {
+template <int VEC>
+__device__ __forceinline__ bool join_sums(const NaArgs& A, int heads, bool more, int at, int h, float (&a)[VEC], float (&b)[VEC], float& first) {
     __shared__ float red[NA_JOIN][2 * VEC + 1][64];
     const int4 sp = A.splits[blockIdx.x];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hc = h < heads ? h : heads - 1;
@@ -212,8 +276,8 @@ __device__ __forceinline__ bool join_sums(const NaArgs& A, int heads, bool more,
     for (int s = wave; s < sp.z; s += NA_JOIN) {
         const int64_t o = (int64_t)(sp.y + s) * heads + hc;
         float x[VEC], y[VEC];
-        __builtin_memcpy(x, A.part + o * 2 * A.D + at.at, sizeof(x));
-        __builtin_memcpy(y, A.part + o * 2 * A.D + A.D + at.at, sizeof(y));
+        __builtin_memcpy(x, A.part + o * 2 * A.D + at, sizeof(x));
+        __builtin_memcpy(y, A.part + o * 2 * A.D + A.D + at, sizeof(y));
         if (more) first += A.part2[o].x;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
@@ -255,32 +319,28 @@ __device__ __forceinline__ void dq_of(float (&pdk)[VEC], const float (&pk)[VEC],
 template <typename T, int VEC, int LPH, bool BIAS>
 __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dq_kernel(NaArgs A) {
     constexpr int UN = 4;
-    const Lane<VEC, LPH> w(A, A.H);
+    const Lane<LPH> w(A, A.H);
     if (w.slot >= A.n_items || !w.head) return;
     const int4 it = A.items[w.slot];
-    const Place<VEC> at(w.l, A.D, A.D != LPH * VEC);
+    const Part<T, VEC, LPH> part(w.l, A.D);
     const int kv = w.h / (A.H / A.Hkv);
     const int64_t o = (int64_t)it.x * A.H + w.h;
-    float q[VEC], go[VEC], pdk[VEC], pk[VEC], delta = 0.f, bias[UN];
+    float pdk[VEC], pk[VEC], delta = 0.f, bias[UN];
     Piece<T, VEC> raw, raw2;
-    raw.load((const T*)A.q + (int64_t)it.x * A.q_ld + w.h * A.q_hd + at.at);
-    raw2.load((const T*)A.go + (int64_t)it.x * A.go_ld + w.h * A.go_hd + at.at);
+    Fixed<T, VEC> q, go;
+    raw.load((const T*)(row_at(A.q, it.x, A.q_ld) + w.h * A.q_hd) + part.at);
+    raw2.load((const T*)(row_at(A.go, it.x, A.go_ld) + w.h * A.go_hd) + part.at);
     const float m = A.stats[o * 2], logl = A.stats[o * 2 + 1];
-    raw.get(q);
-    raw2.get(go);
-    at.leave_own(q);
-    at.leave_own(go);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        q[e] *= A.scale;
-        pdk[e] = pk[e] = 0.f;
-    }
-    const T *kp = (const T*)A.k + kv * A.k_hd + at.at, *vp = (const T*)A.v + kv * A.v_hd + at.at;
+    for (int e = 0; e < VEC; ++e) pdk[e] = pk[e] = 0.f;
+    const char *kp = A.k + kv * A.k_hd + part.at * sizeof(T), *vp = A.v + kv * A.v_hd + part.at * sizeof(T);
     int next[UN];
     load_numbers<UN>(A.index + it.y, next);
-    if (BIAS)
-#pragma unroll
-        for (int u = 0; u < UN; ++u) bias[u] = it.y + u < it.z ? A.bias[(int64_t)(it.y + u) * A.H + w.h] : -NA_INF;
+    if (BIAS) load_biases<UN>(A, it.y, it.z, w.h, bias);
+    part.leave_own(raw);
+    part.leave_own(raw2);
+    q.set(raw);
+    go.set(raw2);
     for (int t = it.y; t < it.z; t += UN) {
         Piece<T, VEC> kk[UN], vv[UN];
         float b[UN];
@@ -288,9 +348,9 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dq_kernel(NaArgs 
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
             ok[u] = t + u < it.z;
-            const int64_t j = ok[u] ? next[u] : next[0];
-            kk[u].load(kp + j * A.k_ld);
-            vv[u].load(vp + j * A.v_ld);
+            const int j = ok[u] ? next[u] : next[0];
+            kk[u].load((const T*)row_at(kp, j, A.k_ld));
+            vv[u].load((const T*)row_at(vp, j, A.v_ld));
             b[u] = 0.f;
             if (BIAS) {
                 b[u] = bias[u];
@@ -299,85 +359,72 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dq_kernel(NaArgs 
         }
         if (t + UN < it.z) {
             load_numbers<UN>(A.index + t + UN, next);
-            if (BIAS)
-#pragma unroll
-                for (int u = 0; u < UN; ++u) bias[u] = t + UN + u < it.z ? A.bias[(int64_t)(t + UN + u) * A.H + w.h] : -NA_INF;
+            if (BIAS) load_biases<UN>(A, t + UN, it.z, w.h, bias);
         }
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
             if (!ok[u]) continue;
-            float k[VEC], own[VEC], v[VEC], s = 0.f, d = 0.f;
-            kk[u].get(k);
-            vv[u].get(v);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) own[e] = k[e];
-            at.leave_own(own);
-            at.leave_own(v);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                s += q[e] * own[e];
-                d += go[e] * v[e];
-            }
-            s = group_sum<LPH>(s) + b[u];
-            d = group_sum<LPH>(d);
+            part.leave_own(kk[u]);
+            part.leave_own(vv[u]);
+            const float s = group_sum<LPH>(q.dot(kk[u])) * A.scale + b[u], d = group_sum<LPH>(go.dot(vv[u]));
             const float p = probability(s, m, logl), pd = p * d;
             delta += pd;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                pdk[e] += pd * k[e];
-                pk[e] += p * k[e];
+                const float k = (float)kk[u].t[e];
+                pdk[e] += pd * k;
+                pk[e] += p * k;
             }
         }
     }
     if (it.w >= 0) {
         const int64_t p = (int64_t)it.w * A.H + w.h;
-        put<float, VEC>(A.part + p * 2 * A.D + at.at, pdk);
-        put<float, VEC>(A.part + p * 2 * A.D + A.D + at.at, pk);
+        part.store(A.part + p * 2 * A.D, pdk);
+        part.store(A.part + p * 2 * A.D + A.D, pk);
         if (w.l == 0) A.part2[p] = make_float2(delta, 0.f);
     } else {
         dq_of<VEC>(pdk, pk, delta, A.scale);
-        put<T, VEC>((T*)A.out + o * A.D + at.at, pdk);
+        part.store((T*)A.out + o * A.D, pdk);
         if (w.l == 0) A.rowstats[o] = make_float4(m, logl, delta, 0.f);
     }
 }
 template <typename T, int VEC, int LPH>
 __global__ __launch_bounds__(64 * NA_JOIN) void nbr_attention_dq_join_kernel(NaArgs A) {
     const int lane = threadIdx.x & 63, h = blockIdx.y * (64 / LPH) + lane / LPH;
-    const Place<VEC> at(lane & (LPH - 1), A.D, A.D != LPH * VEC);
+    const Part<T, VEC, LPH> part(lane & (LPH - 1), A.D);
     float pdk[VEC], pk[VEC], delta;
-    if (!join_sums<VEC, LPH>(A, A.H, true, at, h, pdk, pk, delta)) return;
+    if (!join_sums<VEC>(A, A.H, true, part.at, h, pdk, pk, delta)) return;
     dq_of<VEC>(pdk, pk, delta, A.scale);
     const int64_t o = (int64_t)A.splits[blockIdx.x].x * A.H + h;
-    put<T, VEC>((T*)A.out + o * A.D + at.at, pdk);
+    part.store((T*)A.out + o * A.D, pdk);
     if ((lane & (LPH - 1)) == 0) A.rowstats[o] = make_float4(A.stats[o * 2], A.stats[o * 2 + 1], delta, 0.f);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- backward over the rows' lists: dk, dv, db
+// UN entries at a time: four where items are long enough to fill them, two where most rows are in a list or two
 template <typename T, int VEC, int LPH, bool BIAS, int UN>
 __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dkv_kernel(NaArgs A) {
-    const Lane<VEC, LPH> w(A, A.Hkv);
+    const Lane<LPH> w(A, A.Hkv);
     if (w.slot >= A.n_items || !w.head) return;
     const int4 it = A.items[w.slot];
-    const Place<VEC> at(w.l, A.D, A.D != LPH * VEC);
+    const Part<T, VEC, LPH> part(w.l, A.D);
     const int R = A.H / A.Hkv;
-    float k[VEC], v[VEC], dk[VEC], dv[VEC];
+    float dk[VEC], dv[VEC];
     Piece<T, VEC> raw, raw2;
-    raw.load((const T*)A.k + (int64_t)it.x * A.k_ld + w.h * A.k_hd + at.at);
-    raw2.load((const T*)A.v + (int64_t)it.x * A.v_ld + w.h * A.v_hd + at.at);
+    Fixed<T, VEC> k, v;
+    raw.load((const T*)(row_at(A.k, it.x, A.k_ld) + w.h * A.k_hd) + part.at);
+    raw2.load((const T*)(row_at(A.v, it.x, A.v_ld) + w.h * A.v_hd) + part.at);
     int next[UN], next_e[UN];
     load_numbers<UN>(A.owner + it.y, next);
     if (BIAS) load_numbers<UN>(A.entry + it.y, next_e);
-    raw.get(k);
-    raw2.get(v);
-    at.leave_own(k);
-    at.leave_own(v);
+    part.leave_own(raw);
+    part.leave_own(raw2);
+    k.set(raw);
+    v.set(raw2);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        k[e] *= A.scale;
-        dk[e] = dv[e] = 0.f;
-    }
+    for (int e = 0; e < VEC; ++e) dk[e] = dv[e] = 0.f;
     for (int t = it.y; t < it.z; t += UN) {
-        int64_t i[UN], e_at[UN];
+        int i[UN], e_at[UN];
         bool in[UN];
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
@@ -391,71 +438,58 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dkv_kernel(NaArgs
         }
         for (int r = 0; r < R; ++r) {
             const int h = w.h * R + r;
+            const char *qp = A.q + h * A.q_hd + part.at * sizeof(T), *gp = A.go + h * A.go_hd + part.at * sizeof(T);
             Piece<T, VEC> qq[UN], gg[UN];
             float4 st[UN];
             float bias[UN];
 #pragma unroll
             for (int u = 0; u < UN; ++u) {
-                st[u] = A.rowstats[i[u] * A.H + h];
-                bias[u] = BIAS ? A.bias[e_at[u] * A.H + h] : 0.f;
-                qq[u].load((const T*)A.q + i[u] * A.q_ld + h * A.q_hd + at.at);
-                gg[u].load((const T*)A.go + i[u] * A.go_ld + h * A.go_hd + at.at);
+                st[u] = *(const float4*)row_at((const char*)(A.rowstats + h), i[u], (uint32_t)A.H * sizeof(float4));
+                bias[u] = BIAS ? *(const float*)row_at((const char*)(A.bias + h), e_at[u], (uint32_t)A.H * sizeof(float)) : 0.f;
+                qq[u].load((const T*)row_at(qp, i[u], A.q_ld));
+                gg[u].load((const T*)row_at(gp, i[u], A.go_ld));
             }
 #pragma unroll
             for (int u = 0; u < UN; ++u) {
                 if (!in[u]) continue;
-                float q[VEC], g[VEC], oq[VEC], og[VEC], s = 0.f, d = 0.f;
-                qq[u].get(q);
-                gg[u].get(g);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    oq[e] = q[e];
-                    og[e] = g[e];
-                }
-                at.leave_own(oq);
-                at.leave_own(og);
+                part.leave_own(qq[u]);
+                part.leave_own(gg[u]);
                 const bool live = !BIAS || bias[u] != -NA_INF;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    s += oq[e] * k[e];
-                    d += og[e] * v[e];
-                }
-                s = group_sum<LPH>(s) + bias[u];
-                d = group_sum<LPH>(d);
+                const float s = group_sum<LPH>(k.dot(qq[u])) * A.scale + bias[u], d = group_sum<LPH>(v.dot(gg[u]));
                 const float p = live ? probability(s, st[u].x, st[u].y) : 0.f, ds = live ? p * (d - st[u].z) : 0.f;
-                if (BIAS && A.out_bias && w.l == 0) A.out_bias[e_at[u] * A.H + h] = ds;
+                if (BIAS && A.out_bias && w.l == 0) *(float*)row_at((const char*)(A.out_bias + h), e_at[u], (uint32_t)A.H * sizeof(float)) = ds;
                 if (!live) continue;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    dk[e] += ds * q[e];
-                    dv[e] += p * g[e];
+                    dk[e] += ds * (float)qq[u].t[e];
+                    dv[e] += p * (float)gg[u].t[e];
                 }
             }
         }
     }
     if (it.w >= 0) {
-        float* part = A.part + ((int64_t)it.w * A.Hkv + w.h) * 2 * A.D;
-        put<float, VEC>(part + at.at, dk);
-        put<float, VEC>(part + A.D + at.at, dv);
+        const int64_t p = (int64_t)it.w * A.Hkv + w.h;
+        part.store(A.part + p * 2 * A.D, dk);
+        part.store(A.part + p * 2 * A.D + A.D, dv);
     } else {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) dk[e] *= A.scale;
-        const int64_t o = ((int64_t)it.x * A.Hkv + w.h) * A.D + at.at;
-        put<T, VEC>((T*)A.dk + o, dk);
-        put<T, VEC>((T*)A.dv + o, dv);
+        const int64_t o = ((int64_t)it.x * A.Hkv + w.h) * A.D;
+        part.store((T*)A.dk + o, dk);
+        part.store((T*)A.dv + o, dv);
     }
 }
 template <typename T, int VEC, int LPH>
 __global__ __launch_bounds__(64 * NA_JOIN) void nbr_attention_dkv_join_kernel(NaArgs A) {
     const int lane = threadIdx.x & 63, h = blockIdx.y * (64 / LPH) + lane / LPH;
-    const Place<VEC> at(lane & (LPH - 1), A.D, A.D != LPH * VEC);
+    const Part<T, VEC, LPH> part(lane & (LPH - 1), A.D);
     float dk[VEC], dv[VEC], none;
-    if (!join_sums<VEC, LPH>(A, A.Hkv, false, at, h, dk, dv, none)) return;
+    if (!join_sums<VEC>(A, A.Hkv, false, part.at, h, dk, dv, none)) return;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) dk[e] *= A.scale;
-    const int64_t o = ((int64_t)A.splits[blockIdx.x].x * A.Hkv + h) * A.D + at.at;
-    put<T, VEC>((T*)A.dk + o, dk);
-    put<T, VEC>((T*)A.dv + o, dv);
+    const int64_t o = ((int64_t)A.splits[blockIdx.x].x * A.Hkv + h) * A.D;
+    part.store((T*)A.dk + o, dk);
+    part.store((T*)A.dv + o, dv);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- launches
@@ -516,16 +550,19 @@ static int na_args(const marius_neighbor_plan* P, const marius_neighbor_attentio
     MARIUS_REQUIRE(m->dim > 0 && m->dim <= 256, "%s: heads of 1 to 256 elements", what);
     MARIUS_REQUIRE(P->n == 0 || (m->q && P->items), "%s: null pointer", what);
     MARIUS_REQUIRE(P->T == 0 || (m->k && m->v && P->index), "%s: null pointer", what);
+    const int64_t size = m->type == MARIUS_F32 ? 4 : 2;
+    for (int64_t row : {m->q_row, m->k_row, m->v_row})
+        MARIUS_REQUIRE(row >= 0 && row * size < (1ll << 32), "%s: rows are at most 4 GiB apart", what);
     A = NaArgs{};
-    A.q = m->q;
-    A.k = m->k;
-    A.v = m->v;
-    A.q_ld = m->q_row;
-    A.q_hd = m->q_head;
-    A.k_ld = m->k_row;
-    A.k_hd = m->k_head;
-    A.v_ld = m->v_row;
-    A.v_hd = m->v_head;
+    A.q = (const char*)m->q;
+    A.k = (const char*)m->k;
+    A.v = (const char*)m->v;
+    A.q_ld = (uint32_t)(m->q_row * size);
+    A.q_hd = m->q_head * size;
+    A.k_ld = (uint32_t)(m->k_row * size);
+    A.k_hd = m->k_head * size;
+    A.v_ld = (uint32_t)(m->v_row * size);
+    A.v_hd = m->v_head * size;
     A.bias = m->bias;
     A.stats = m->stats;
     A.H = m->heads;
@@ -580,9 +617,11 @@ extern "C" int marius_neighbor_attention_backward(const marius_neighbor_plan* P,
     const size_t need = marius_neighbor_attention_workspace_bytes(P, m->heads, m->kv_heads, m->dim, 1);
     MARIUS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "neighbor_attention_backward: workspace too small");
     hipStream_t st = as_stream(stream);
-    A.go = grad_out;
-    A.go_ld = grad_row;
-    A.go_hd = grad_head;
+    const int64_t size = m->type == MARIUS_F32 ? 4 : 2;
+    MARIUS_REQUIRE(grad_row >= 0 && grad_row * size < (1ll << 32), "neighbor_attention_backward: rows are at most 4 GiB apart");
+    A.go = (const char*)grad_out;
+    A.go_ld = (uint32_t)(grad_row * size);
+    A.go_hd = grad_head * size;
     A.rowstats = (float4*)workspace;
     A.part2 = (float2*)(A.rowstats + (size_t)P->n * A.H);
     A.part = (float*)((char*)A.part2 + na_small_bytes(P, A.H));

@@ -58,7 +58,7 @@ struct Row {
     typedef float Values[NCH][VEC];
     int tpr, lane, rows, mine;  // lanes of a row, this one's number, rows a workgroup holds, this one's
     int at[NCH], first[NCH];
-    bool tail;
+    bool tail;                  // (uniform: the row does not fill its lanes' pieces)
     float inv_d, *red;          // red: LDS of two reductions, used in turn
     int turn;
     __device__ __forceinline__ Row(const NormArgs& A, float* red_) : red(red_), turn(0) {
@@ -70,7 +70,7 @@ struct Row {
         inv_d = 1.f / (float)A.d;
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            const Place<VEC> p(j * tpr + lane, A.d, tail);
+            const Place<VEC> p(j * tpr + lane, A.d);
             at[j] = p.at;
             first[j] = p.first;
         }

@@ -22,21 +22,14 @@ __device__ __forceinline__ void put(T* p, const float (&v)[VEC]) {
     for (int e = 0; e < VEC; ++e) t[e] = (T)v[e];
     __builtin_memcpy(p, t, sizeof(t));
 }
-// Where piece number `unit` of a row of `d` elements lies.  A row that is no multiple of VEC ends with a piece that ends with the row and overlaps its
-// neighbour's (both compute and store the same there); lanes behind the row repeat the last piece.  `first` is the first element that is the piece's own (VEC:
-// none); leave_own keeps the others out of sums over the row (both factors of a product, so that no infinity of a neighbour's element turns into NaN).  d >= VEC.
+// Where piece number `unit` of a row of `d` elements lies (d >= VEC).  A row that is no multiple of VEC ends with a piece that ends with the row and overlaps
+// its neighbour's; lanes behind the row repeat the last piece.  `first` is the first element that is the piece's own (VEC: none).
 template <int VEC>
 struct Place {
     int at, first;
-    bool tail;  // (uniform: the row does not fill its lanes' pieces)
-    __device__ __forceinline__ Place(int unit, int d, bool tail_) : at(unit * VEC < d - VEC ? unit * VEC : d - VEC), tail(tail_) {
+    __device__ __forceinline__ Place(int unit, int d) : at(unit * VEC < d - VEC ? unit * VEC : d - VEC) {
         first = unit * VEC - at;
         first = first > VEC ? VEC : first;
-    }
-    __device__ __forceinline__ void leave_own(float (&v)[VEC]) const {
-        if (!tail) return;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = e >= first ? v[e] : 0.f;
     }
 };
 

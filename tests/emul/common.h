@@ -382,6 +382,7 @@ inline emul::vec<unsigned, 2> emul_lane_pair(unsigned v, int bit) {
 }
 inline emul::vec<unsigned, 2> __builtin_amdgcn_permlane16_swap(unsigned a, unsigned, bool, bool) { return emul_lane_pair(a, 16); }
 inline emul::vec<unsigned, 2> __builtin_amdgcn_permlane32_swap(unsigned a, unsigned, bool, bool) { return emul_lane_pair(a, 32); }
+inline float __builtin_amdgcn_fdot2_f32_bf16(emul::vec<__bf16, 2> a, emul::vec<__bf16, 2> b, float c, bool) { return c + (float)a[0] * (float)b[0] + (float)a[1] * (float)b[1]; }
 inline float __builtin_amdgcn_rcpf(float v) { return 1.f / v; }
 inline float __builtin_amdgcn_rsqf(float v) { return 1.f / sqrtf(v); }
 // e4m3 (OCP): v_cvt_pk_f32_fp8 / v_cvt_pk_fp8_f32 on two of a word's four codes; to nearest even, values the type does not reach become NaN
