@@ -23,7 +23,7 @@
 namespace marius {
 
 constexpr float NA_INF = __builtin_inff();
-constexpr int NA_WAVES = 4;
+constexpr int NA_WAVES = 1;  // (waves of a workgroup: items differ in length, and a workgroup holds its registers until its longest wave ends: 4 waves 951 us, 2 852, 1 840 for the hubs of a power-law graph back)
 
 struct NaArgs {
     const char *q, *k, *v, *go;
@@ -38,6 +38,7 @@ struct NaArgs {
     const int4 *items, *splits;
     int n_items, n_splits, H, Hkv, D, hp;                       // hp: heads per slot
     bool dense;                                                 // items of more than two entries on average
+    bool spread;                                                // sweep over the rows' lists: a lane group for each query head, not for each key head
     float scale;
 };
 
@@ -404,16 +405,16 @@ __global__ __launch_bounds__(64 * NA_JOIN) void nbr_attention_dq_join_kernel(NaA
 // UN entries at a time: four where items are long enough to fill them, two where most rows are in a list or two
 template <typename T, int VEC, int LPH, bool BIAS, int UN>
 __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dkv_kernel(NaArgs A) {
-    const Lane<LPH> w(A, A.Hkv);
+    const Lane<LPH> w(A, A.spread ? A.H : A.Hkv);
     if (w.slot >= A.n_items || !w.head) return;
     const int4 it = A.items[w.slot];
     const Part<T, VEC, LPH> part(w.l, A.D);
-    const int R = A.H / A.Hkv;
+    const int share = A.H / A.Hkv, R = A.spread ? 1 : share, kv = A.spread ? w.h / share : w.h;
     float dk[VEC], dv[VEC];
     Piece<T, VEC> raw, raw2;
     Fixed<T, VEC> k, v;
-    raw.load((const T*)(row_at(A.k, it.x, A.k_ld) + w.h * A.k_hd) + part.at);
-    raw2.load((const T*)(row_at(A.v, it.x, A.v_ld) + w.h * A.v_hd) + part.at);
+    raw.load((const T*)(row_at(A.k, it.x, A.k_ld) + kv * A.k_hd) + part.at);
+    raw2.load((const T*)(row_at(A.v, it.x, A.v_ld) + kv * A.v_hd) + part.at);
     int next[UN], next_e[UN];
     load_numbers<UN>(A.owner + it.y, next);
     if (BIAS) load_numbers<UN>(A.entry + it.y, next_e);
@@ -467,14 +468,23 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dkv_kernel(NaArgs
             }
         }
     }
+    if (A.spread) {  // the lanes of the query heads that share this key head
+        for (int o = LPH; o < LPH * share; o <<= 1)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                dk[e] += __shfl_xor(dk[e], o, 64);
+                dv[e] += __shfl_xor(dv[e], o, 64);
+            }
+        if (w.h & (share - 1)) return;
+    }
     if (it.w >= 0) {
-        const int64_t p = (int64_t)it.w * A.Hkv + w.h;
+        const int64_t p = (int64_t)it.w * A.Hkv + kv;
         part.store(A.part + p * 2 * A.D, dk);
         part.store(A.part + p * 2 * A.D + A.D, dv);
     } else {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) dk[e] *= A.scale;
-        const int64_t o = ((int64_t)it.x * A.Hkv + w.h) * A.D;
+        const int64_t o = ((int64_t)it.x * A.Hkv + kv) * A.D;
         part.store((T*)A.dk + o, dk);
         part.store((T*)A.dv + o, dv);
     }
@@ -497,10 +507,13 @@ enum NaPass { NA_FWD = 0, NA_DQ, NA_DKV };
 
 template <typename T, int VEC, int LPH>
 static void na_launch(NaArgs A, NaPass pass, hipStream_t st) {
-    const int heads = pass == NA_DKV ? A.Hkv : A.H, groups = 64 / LPH;
+    const int groups = 64 / LPH, share = A.H / A.Hkv;
+    // key heads that a power of two of query heads share: their lane groups work side by side where a slot holds them all, and are added at the end
+    A.spread = pass == NA_DKV && share > 1 && (share & (share - 1)) == 0 && share <= groups;
+    const int heads = pass == NA_DKV && !A.spread ? A.Hkv : A.H;
     A.hp = 1;
     while (A.hp < groups && A.hp < heads) A.hp <<= 1;
-    const dim3 grid((unsigned)cdiv(A.n_items, NA_WAVES * (groups / A.hp)), (unsigned)cdiv(heads, A.hp)), jgrid((unsigned)A.n_splits, (unsigned)cdiv(heads, groups));
+    const dim3 grid((unsigned)cdiv(A.n_items, NA_WAVES * (groups / A.hp)), (unsigned)cdiv(heads, A.hp)), jgrid((unsigned)A.n_splits, (unsigned)cdiv(pass == NA_DKV ? A.Hkv : A.H, groups));
     const dim3 block(64 * NA_WAVES);
     if (pass == NA_FWD) {
         if (A.bias) nbr_attention_kernel<T, VEC, LPH, true><<<grid, block, 0, st>>>(A);

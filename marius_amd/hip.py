@@ -758,9 +758,10 @@ def residual_norm_backward(grad_y, grad_h, y, block=None, gate=None, post_weight
 
 
 def plan_chunk(entries):
-    """entries of a work item: as few as still pay for their partial results, because an item's loads follow one another (measured, us, at 16 / 32 / 64 / 128 entries:
-    a training pass over 1.5 M entries 1647 / 1327 / 1236 / 1249, over 200,000 entries 111 / 113 / 133 / 181, one served list of 8192 29 / 26 / 27 / 29)"""
-    return 64 if entries >= 1 << 20 else 32
+    """entries of a work item: as few as still pay for their partial results, because an item's loads follow one another (measured, us, at 16 / 32 / 64 / 128 / 256
+    entries: a pass there and back over 1.5 M entries 1529 / 1184 / 1078 / 1027 / 1035, over 200,000 entries 103 / 103 / 121 / 174 / 254, one served list of 8192
+    16 / 14 / 16 / 22 / 35)"""
+    return 128 if entries >= 1 << 20 else 32
 
 
 class NeighborPlan:
