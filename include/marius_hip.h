@@ -645,7 +645,7 @@ int marius_neighbor_attention_backward(const marius_neighbor_plan* plan, const m
 
 /* AdamW over many tensors (adamw.hip): p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps), moments m and v updated first; t = step (from 1),
  * or *step_dev (a captured call replays with the step it finds there).  Every gradient is multiplied by *grad_scale (NULL: 1).  All tensors of a call have
- * parameters of param_type and gradients of grad_type; a launch takes 64 tensors.  state_bits 32: exp_avg / exp_avg_sq fp32 [n].  state_bits 8: e4m3 codes [n] and one
+ * parameters of param_type and gradients of grad_type; more than 64 of them go through a table in `workspace` (marius_adamw_workspace_bytes(count) bytes, 0 up to 64).  state_bits 32: exp_avg / exp_avg_sq fp32 [n].  state_bits 8: e4m3 codes [n] and one
  * fp32 scale for every 256 elements [ceil(n / 256)]; exp_avg_sq then holds the ROOT of the second moment (value = code * scale in both), and a root above zero stays
  * above zero. */
 typedef struct marius_adamw_tensor {
@@ -655,8 +655,10 @@ typedef struct marius_adamw_tensor {
     float *exp_avg_scale, *exp_avg_sq_scale;
     int64_t n;
 } marius_adamw_tensor;
+size_t marius_adamw_workspace_bytes(int32_t count);
 int marius_adamw_step(const marius_adamw_tensor* tensors, int32_t count, int32_t param_type, int32_t grad_type, int32_t state_bits, int64_t step, const int64_t* step_dev,
-                      double lr, double beta1, double beta2, double eps, double weight_decay, const float* grad_scale, marius_stream_t stream);
+                      double lr, double beta1, double beta2, double eps, double weight_decay, const float* grad_scale, void* workspace, size_t workspace_bytes,
+                      marius_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -50,7 +50,7 @@ void* data(const MaybeTensor& t) { return t ? t->data_ptr() : nullptr; }
 marius_stream_t stream_of(const at::Device& device) {
     return device.is_cuda() ? (marius_stream_t)c10::hip::getCurrentHIPStream(device.index()).stream() : nullptr;
 }
-Tensor bytes(size_t n, const Tensor& like) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
+Tensor bytes(size_t n, const Tensor& like) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte).requires_grad(false)); }
 
 // rows [n, d] of contiguous elements that do not overlap (a copy where `t` is not laid out so) and their stride
 struct Rows {
@@ -331,7 +331,7 @@ struct AdamWTensors {
     }
 };
 // `entry`: marius_adamw_step; `step`: an int or an int64 device tensor
-void adamw_step(uintptr_t entry, AdamWTensors& a, const std::vector<MaybeTensor>& grads, const py::object& step, double lr, double beta1, double beta2, double eps,
+void adamw_step(uintptr_t entry, uintptr_t workspace_entry, AdamWTensors& a, const std::vector<MaybeTensor>& grads, const py::object& step, double lr, double beta1, double beta2, double eps,
                 double weight_decay, const MaybeTensor& grad_scale, bool capturing) {
     const size_t count = a.params.size();
     require(grads.size() == count, "adamw_step: ", grads.size(), " gradients for ", count, " parameters");
@@ -369,8 +369,10 @@ void adamw_step(uintptr_t entry, AdamWTensors& a, const std::vector<MaybeTensor>
     require(*kind == at::kFloat || *kind == at::kBFloat16 || *kind == at::kHalf, "adamw_step: float32, bfloat16 or float16 gradients required, got ", *kind);
     const int grad_type = *kind == at::kFloat ? MARIUS_F32 : *kind == at::kBFloat16 ? MARIUS_BF16 : MARIUS_F16;
     const c10::OptionalDeviceGuard guard(device);
+    const size_t need = ((decltype(&marius_adamw_workspace_bytes))workspace_entry)((int32_t)count);
+    const Tensor ws = need ? bytes(need, a.states[0][0]) : Tensor();
     check(((decltype(&marius_adamw_step))entry)(table.data(), (int32_t)count, a.type, grad_type, a.bits, on_device ? 0 : step.cast<int64_t>(), (const int64_t*)data(counter), lr, beta1,
-                                                beta2, eps, weight_decay, (const float*)data(grad_scale), stream_of(device)),
+                                                beta2, eps, weight_decay, (const float*)data(grad_scale), need ? ws.data_ptr() : nullptr, need, stream_of(device)),
           "adamw_step");
 }
 

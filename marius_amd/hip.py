@@ -146,7 +146,8 @@ SIGNATURES = {
     "marius_neighbor_attention_workspace_bytes": (_sz, [C.POINTER(NeighborPlanDesc), _i32, _i32, _i32, _i32]),
     "marius_neighbor_attention_forward": (C.c_int, [C.POINTER(NeighborPlanDesc), C.POINTER(NeighborAttention), _vp, _vp, _sz, _vp]),
     "marius_neighbor_attention_backward": (C.c_int, [C.POINTER(NeighborPlanDesc), C.POINTER(NeighborAttention), _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
-    "marius_adamw_step": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i64, _vp, _f64, _f64, _f64, _f64, _f64, _vp, _vp]),
+    "marius_adamw_step": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i64, _vp, _f64, _f64, _f64, _f64, _f64, _vp, _vp, _sz, _vp]),
+    "marius_adamw_workspace_bytes": (_sz, [_i32]),
     "marius_owner_offsets_counts": (C.c_int, [_vp, _vp, _i64, _i32, _vp, _vp, _vp]),
     "marius_a2a_record_words": (_i32, [_i32]),
     "marius_a2a_record_checksum": (C.c_uint64, [_vp, _i32]),
@@ -878,7 +879,7 @@ def adamw_step(tensors, grads, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, 
     they are.  step counts from 1: a number, or an int64 device tensor of one element (a captured call has to take that: a replay reads it anew).  grad_scale: float32
     device tensor of one element every gradient is multiplied by (a clipping factor, the inverse of a loss scale)."""
     _require(isinstance(tensors, _ops().AdamWTensors), "adamw_step: AdamWTensors are needed")
-    _ops().adamw_step(_entry("marius_adamw_step"), tensors, grads, step, lr, beta1, beta2, eps, weight_decay, grad_scale,
+    _ops().adamw_step(_entry("marius_adamw_step"), _entry("marius_adamw_workspace_bytes"), tensors, grads, step, lr, beta1, beta2, eps, weight_decay, grad_scale,
                       torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing())
 
 
