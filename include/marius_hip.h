@@ -602,14 +602,16 @@ int marius_residual_norm_backward(const marius_residual_norm* desc, const marius
  *   their list, bit 1: a row outside [0, rows).  A caller reads status before it goes on: the calls below and the attention take the lists as they are.
  * marius_nbr_plan_reverse: the entries grouped by row, in list order: r_offsets [rows + 1], r_owner [T]; perm of marius_sort_unique = r_entry.
  *   (The attention reads index, r_owner and r_entry four entries at a time: allocate four more than T; what they hold does not matter.)
- * marius_nbr_plan_items: lists cut into work items of at most `chunk` entries: items {list, first, end, slot or -1} (at most n + T / chunk), splits {list, first
- *   slot, parts, 0} of the lists that were cut (at most T / chunk), totals [3] = items, slots, splits. */
+ * marius_nbr_plan_items: lists cut into work items of at most `chunk` entries: items {list, first, end, slot or -1} (at most n + T / chunk; the longest first),
+ *   splits {list, first slot, parts, 0} of the lists that were cut (at most T / chunk), totals [3] = items, slots, splits.  Workspace:
+ *   marius_nbr_plan_items_workspace_bytes, at a multiple of 16 bytes. */
 size_t marius_nbr_plan_workspace_bytes(int64_t n);
 int marius_nbr_plan_lists(const int64_t* index_a, const int64_t* offsets_a, int64_t T_a, const int64_t* index_b, const int64_t* offsets_b, int64_t T_b, int64_t n, int64_t rows,
                           int64_t self_offset, int32_t* offsets, int32_t* index, int32_t* owner, int64_t* keys, int32_t* status, void* workspace, size_t workspace_bytes,
                           marius_stream_t stream);
 int marius_nbr_plan_reverse(const int64_t* uniq, const int32_t* seg_offsets, const int64_t* num_unique_dev, const int32_t* perm, const int32_t* owner, int64_t T, int64_t rows,
                             int32_t* r_offsets, int32_t* r_owner, marius_stream_t stream);
+size_t marius_nbr_plan_items_workspace_bytes(int64_t n, int32_t max_items);
 int marius_nbr_plan_items(const int32_t* offsets, int64_t n, int32_t chunk, int32_t* items, int32_t max_items, int32_t* splits, int32_t max_splits, int32_t* totals,
                           void* workspace, size_t workspace_bytes, marius_stream_t stream);
 typedef struct marius_neighbor_plan {

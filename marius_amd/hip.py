@@ -142,6 +142,7 @@ SIGNATURES = {
     "marius_nbr_plan_workspace_bytes": (_sz, [_i64]),
     "marius_nbr_plan_lists": (C.c_int, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "marius_nbr_plan_reverse": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp]),
+    "marius_nbr_plan_items_workspace_bytes": (_sz, [_i64, _i32]),
     "marius_nbr_plan_items": (C.c_int, [_vp, _i64, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _sz, _vp]),
     "marius_neighbor_attention_workspace_bytes": (_sz, [C.POINTER(NeighborPlanDesc), _i32, _i32, _i32, _i32]),
     "marius_neighbor_attention_forward": (C.c_int, [C.POINTER(NeighborPlanDesc), C.POINTER(NeighborAttention), _vp, _vp, _sz, _vp]),
@@ -790,7 +791,9 @@ class NeighborPlan:
         keys, status = torch.empty(total, dtype=torch.int64, device=dev), torch.zeros(4, **i32)
         L = lib()
         with torch.cuda.device(dev if dev.type == "cuda" else -1):  # (launches go to the current device)
-            wsb = max(L.marius_nbr_plan_workspace_bytes(n), L.marius_nbr_plan_workspace_bytes(num_rows))
+            chunk = plan_chunk(total)
+            more = total // chunk
+            wsb = max(L.marius_nbr_plan_items_workspace_bytes(m, m + more) for m in (n, num_rows))
             ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
             check(L.marius_nbr_plan_lists(ptr(lists[0]), ptr(lists[1]), ta, ptr(lists[2]), ptr(lists[3]), tb, n, num_rows, own, ptr(offs), ptr(self._index), ptr(owner),
                                           ptr(keys), ptr(status), ptr(ws), wsb, stream_ptr()), "nbr_plan_lists")
@@ -804,8 +807,6 @@ class NeighborPlan:
             self._r_entry = um.perm
             check(L.marius_nbr_plan_reverse(ptr(um.uniq), ptr(um.seg), ptr(um.count), ptr(um.perm), ptr(owner), total, num_rows, ptr(r_offs), ptr(self._r_owner), stream_ptr()),
                   "nbr_plan_reverse")
-            chunk = plan_chunk(total)
-            more = total // chunk
             totals = torch.zeros(2, 4, **i32)
             made = []
             for k, (o, m) in enumerate(((offs, n), (r_offs, num_rows))):
