@@ -8,7 +8,10 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <cmath>
 #include <optional>
+#include <sstream>
 
 #include "marius_hip.h"
 
@@ -328,6 +331,16 @@ struct AdamWTensors {
             t.exp_avg_sq_scale = bits == 8 ? (float*)states[3][i].data_ptr() : nullptr;
             t.n = w.numel();
         }
+        // no tensor twice, none inside another: every launch updates all of them at once
+        std::vector<std::pair<const char*, const char*>> spans;
+        auto span = [&](const Tensor& t) {
+            if (t.numel() > 0) spans.emplace_back((const char*)t.data_ptr(), (const char*)t.data_ptr() + t.nbytes());
+        };
+        for (const Tensor& w : params) span(w);
+        for (const auto& s : states)
+            for (const Tensor& t : s) span(t);
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i) require(spans[i - 1].second <= spans[i].first, "AdamWTensors: a tensor appears twice, or overlaps another");
     }
 };
 // `entry`: marius_adamw_step; `step`: an int or an int64 device tensor
@@ -346,6 +359,7 @@ void adamw_step(uintptr_t entry, uintptr_t workspace_entry, AdamWTensors& a, con
             continue;
         }
         const Tensor &g = *grads[i], &w = a.params[i];
+        require(g.layout() == at::kStrided, "adamw_step: gradient ", i, " is not a dense tensor");
         if (!kind) kind = g.scalar_type();
         require(g.scalar_type() == *kind && g.device() == device && g.numel() == t.n, "adamw_step: gradient ", i, " is not a ", *kind, " tensor of ", t.n, " elements on ", device);
         require(w.device() == device && w.scalar_type() == a.params[0].scalar_type() && w.numel() == t.n && w.is_contiguous(), "adamw_step: parameter ", i,

@@ -86,7 +86,25 @@ class DENSEGraph:
         self.in_neighbors_mapping_ = self.out_neighbors_mapping_ = None
         self.src_sorted_edges_ = self.dst_sorted_edges_ = None
         self.in_num_neighbors_ = self.out_num_neighbors_ = None
-        self.plan_ = None
+        self.plan_ = self.plan_relations_ = None
+
+    def entryRelations(self, num_relations):
+        """the relation of every entry of the layer's plan, in its order; num_relations for a target's own row.  Made, and checked, once for a plan"""
+        plan = self.neighborPlan()
+        if self.plan_relations_ is None or self.plan_relations_[0] != num_relations:
+            relation = torch.full((plan.num_entries,), -1, **_i64(plan.device))
+            edges = [e for m, e in ((self.out_neighbors_mapping_, self.src_sorted_edges_), (self.in_neighbors_mapping_, self.dst_sorted_edges_)) if m is not None]
+            for part, e in enumerate(edges):
+                if e.size(1) != 3:
+                    raise H.MariusHipError("relation biases need edges of three columns")
+                relation[plan.places(part)] = e.select(1, 1)
+            own = plan.places("own")
+            relation[own] = 0
+            if relation.numel() > 0 and (int(relation.min()) < 0 or int(relation.max()) >= num_relations):
+                raise H.MariusHipError("an edge's relation lies outside the %d relations" % num_relations)
+            relation[own] = num_relations
+            self.plan_relations_ = (num_relations, relation)
+        return self.plan_relations_[1]
 
     def neighborPlan(self):
         """the attention's plan of this layer's lists (outgoing, incoming neighbours, the target's own row), made once between two prepareForNextLayer calls"""
@@ -137,7 +155,7 @@ class DENSEGraph:
 
     def prepareForNextLayer(self):
         """graph.cpp:290-325 (views only)"""
-        self.plan_ = None
+        self.plan_ = self.plan_relations_ = None
         rm = int(self.hop_offsets_[1] - self.hop_offsets_[0])
         fin_nodes = int(self.hop_offsets_[2] - self.hop_offsets_[1])
         if self.src_sorted_edges_.size(0) > 0:
@@ -356,6 +374,7 @@ class _NeighborAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
         q, k, v, bias, stats = ctx.saved_tensors
         dq, dk, dv, dbias = H.neighbor_attention_backward(grad_out, q, k, v, stats, ctx.plan, ctx.scale, bias, need_dbias=ctx.needs_input_grad[3])
@@ -373,6 +392,7 @@ class _ResidualNorm(torch.autograd.Function):
         return tuple(t for t, there in ((y, ctx.with_y), (h, ctx.with_h)) if there)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
         grads = list(grads)
         grad_y = grads.pop(0) if ctx.with_y else None
@@ -424,22 +444,12 @@ class GraphAttentionLayer(torch.nn.Module):
         self.wkv = glorot(2 * self.kv_heads * self.dim, input_dim)
         self.relation_bias = torch.nn.Parameter(torch.zeros(num_relations + 1, heads, device=device)) if num_relations > 0 else None
 
-    def entryBias(self, dense_graph, plan):
-        """the scores' bias, entry by entry in the plan's order: the relation's row of the table, its last row for a target's own entry"""
-        relation = torch.full((plan.num_entries,), self.relation_bias.size(0) - 1, **_i64(plan.device))
-        edges = [e for m, e in ((dense_graph.out_neighbors_mapping_, dense_graph.src_sorted_edges_), (dense_graph.in_neighbors_mapping_, dense_graph.dst_sorted_edges_)) if m is not None]
-        for part, e in enumerate(edges):
-            if e.size(1) != 3:
-                raise H.MariusHipError("GraphAttentionLayer: relation biases need edges of three columns")
-            relation[plan.places(part)] = e.select(1, 1)
-        return self.relation_bias.index_select(0, relation)
-
     def forward(self, inputs, dense_graph, train=True):
         plan = dense_graph.neighborPlan()
         n = plan.n
         q = torch.matmul(inputs.narrow(0, inputs.size(0) - n, n), self.wq.t()).view(n, self.heads, self.dim)
         kv = torch.matmul(inputs, self.wkv.t()).view(inputs.size(0), 2, self.kv_heads, self.dim)
-        bias = None if self.relation_bias is None else self.entryBias(dense_graph, plan)
+        bias = None if self.relation_bias is None else self.relation_bias.index_select(0, dense_graph.entryRelations(self.relation_bias.size(0) - 1))
         out = neighbor_attention(q, kv[:, 0], kv[:, 1], plan, None, bias)
         return torch.matmul(out.view(n, self.heads * self.dim), self.wo.t())
 

@@ -771,11 +771,13 @@ class NeighborPlan:
 
     index [T] int64 (rows), offsets [n] int64 (first entry of every target's list, the last one ends at T) as DENSEGraph holds them; a second list (index_b,
     offsets_b) is appended target by target (outgoing + incoming neighbours), then the target's own row self_offset + i where self_offset is given.  A bias of the attention
-    has one row for each entry in that order.  Making a plan reads two small results back (the checks, the counts of work items)."""
+    has one row for each entry in that order.  Making a plan reads two small results back (the checks, the counts of work items): it cannot be captured, the attention
+    over it can.  As for a tensor, a plan used on another stream than the one it was made on and dropped while that runs needs record_stream."""
 
     def __init__(self, index, offsets, num_rows, index_b=None, offsets_b=None, self_offset=None):
         _dev(index)
         _require(all(t is None or t.device == index.device for t in (offsets, index_b, offsets_b)), "NeighborPlan: index and offsets are on one device")
+        _require(not (torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()), "NeighborPlan: a plan is made before a capture, its checks read results back")
         _require((index_b is None) == (offsets_b is None), "NeighborPlan: a second list has both index and offsets")
         lists = [index, offsets] + ([] if index_b is None else [index_b, offsets_b])
         _require(all(t.dtype == torch.int64 and t.dim() == 1 for t in lists), "NeighborPlan: index and offsets are int64 vectors")
@@ -824,6 +826,11 @@ class NeighborPlan:
                                                                                                         self._r_items, self._r_splits))
         (d.n_items, d.n_slots, d.n_splits, _), (d.r_n_items, d.r_n_slots, d.r_n_splits, _) = counts
         self._starts, self._ends, self._own = (lists[1], lists[3]), (ta, tb), own >= 0
+
+    def record_stream(self, stream):
+        """the plan is in use on `stream` (torch.Tensor.record_stream of everything it holds)"""
+        for t in (self._index, self._items, self._splits, self._r_owner, self._r_entry, self._r_items, self._r_splits):
+            t.record_stream(stream)
 
     def places(self, part):
         """where a part's entries lie in the plan's order: part 0, 1 (the lists, entry by entry) or "own" (the targets' own rows) -> int64 positions.  A bias is laid out by them."""

@@ -171,6 +171,11 @@ def test_adamw_refuses(HE):
     refused(HE, "betas in", HE.adamw_step, t, s, 1, beta1=1.0)
     refused(HE, "one int64", HE.adamw_step, t, s, torch.tensor([1.0]))
     refused(HE, "one float32", HE.adamw_step, t, s, 1, grad_scale=torch.zeros(2))
+    refused(HE, "not a dense tensor", HE.adamw_step, t, [torch.zeros(300).to_sparse()], 1)
+    refused(HE, "twice", HE.AdamWTensors, p + p, s + [torch.zeros(300)], [torch.zeros(300), torch.zeros(300)])
+    flat = torch.zeros(500)
+    refused(HE, "overlaps", HE.AdamWTensors, [flat[:300], flat[200:]], s + [torch.zeros(300)], [torch.zeros(300), torch.zeros(300)])
+    refused(HE, "twice", HE.AdamWTensors, p, s, s)
     p[0].data = torch.zeros(301)
     refused(HE, "no longer", HE.adamw_step, t, s, 1)
 
@@ -220,9 +225,26 @@ def test_emulated_encoder_and_optimizer(HE):
     T.test_optimizer_state_is_saved_and_loaded(HE, CPU)
 
 
+def test_emulated_small_forms(HE):
+    from marius_amd import gnn
+
+    T.test_residual_norm_of_tiny_rows_without_eps(HE, CPU)
+    T.test_second_derivatives_are_refused(HE, gnn, CPU)
+    T.test_gradient_of_a_sum_reaches_every_operand(HE, gnn, CPU)
+
+
 def test_encoder_modules_refuse(HE):
     from marius_amd import gnn
     from marius_amd.optim import AdamW
+
+    graph = T.sampled(gnn, CPU, 50, 300, [4], True, True, 5, 1)
+    graph.performMap()
+    assert int(graph.entryRelations(5).max()) == 5
+    refused(HE, "outside the 3 relations", graph.entryRelations, 3)
+    pairs = T.sampled(gnn, CPU, 50, 300, [4], True, False, 5, 1)
+    pairs.performMap()
+    pairs.dst_sorted_edges_ = pairs.dst_sorted_edges_[:, [0, 2]].contiguous()
+    refused(HE, "three columns", pairs.entryRelations, 5)
 
     refused(HE, "multiple of the number of heads", gnn.GraphAttentionLayer, 8, 10, 4, device=CPU)
     refused(HE, "comes with the call", gnn.ResidualNorm(4, gate="ELEMENT", device=CPU), torch.zeros(2, 4), torch.zeros(2, 4))

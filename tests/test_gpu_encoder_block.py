@@ -461,6 +461,8 @@ def test_block_captured_and_replayed(H, dev, kind):
     with torch.cuda.graph(graph):
         with pytest.raises(H.MariusHipError, match="captured step"):
             H.adamw_step(tensors, [m], 1)
+        with pytest.raises(H.MariusHipError, match="before a capture"):
+            H.NeighborPlan(plan.index.long(), plan.offsets[:-1].long(), rows)
         captured = block()
     torch.cuda.synchronize()
     for r in range(3):
@@ -519,3 +521,38 @@ def test_optimizer_state_is_saved_and_loaded(H, dev):
         two.step()                                                              # nothing to do: no gradients
         with pytest.raises(H.MariusHipError):
             AdamW(a, state_bits=40 - bits).load_state_dict(one.state_dict())
+
+
+def test_residual_norm_of_tiny_rows_without_eps(H, dev):
+    """rows whose squares are subnormal numbers, eps = 0: the mean square is off by 2^-149 an element, 2e-6 of it here, and its root by half of that"""
+    x = torch.randn(5, 64, generator=torch.Generator().manual_seed(3)) * 3e-20
+    h = H.residual_norm(x.to(dev), eps=0.0)[1].cpu().double()
+    want = x.double() / x.double().pow(2).mean(1, keepdim=True).sqrt()
+    assert float((h - want).abs().max()) <= 1e-5 * float(want.abs().max())
+
+
+def test_second_derivatives_are_refused(H, G, dev):
+    x = torch.randn(3, 8, device=dev, requires_grad=True)
+    norm = G.ResidualNorm(8, device=dev)
+    (g,) = torch.autograd.grad(norm(x)[1].pow(2).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    plan = H.NeighborPlan(torch.tensor([0, 1, 2], device=dev), torch.tensor([0, 1], device=dev), 3)
+    q, k = torch.randn(2, 2, 4, device=dev, requires_grad=True), torch.randn(3, 2, 4, device=dev)
+    (g,) = torch.autograd.grad(G.neighbor_attention(q, k, k, plan).pow(2).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_gradient_of_a_sum_reaches_every_operand(H, G, dev):
+    """a gradient whose strides are all zero (a sum's), single-element rows, heads and lists"""
+    q, k = torch.randn(2, 2, 4, device=dev, requires_grad=True), torch.randn(3, 1, 4, device=dev, requires_grad=True)
+    plan = H.NeighborPlan(torch.tensor([0, 1, 2], device=dev), torch.tensor([0, 1], device=dev), 3)
+    G.neighbor_attention(q, k, k, plan).sum().backward()
+    want = R.attention(q.detach(), k.detach(), k.detach(), torch.tensor([0, 1, 2]), torch.tensor([0, 1, 1]), 0.5, None, torch.ones(2, 2, 4))
+    R.close(q.grad, *want["dq"], 1, "dq")
+    R.close(k.grad, want["dk"][0] + want["dv"][0], want["dk"][1] + want["dv"][1], 2, "dk + dv")
+    x = torch.randn(5, 1, device=dev, requires_grad=True)
+    y, h = G.ResidualNorm(1, post_norm=True, bias=True, device=dev)(x, torch.randn(5, 1, device=dev))
+    (y.sum() + h.sum()).backward()
+    assert torch.isfinite(x.grad).all()
