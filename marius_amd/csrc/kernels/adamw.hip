@@ -246,7 +246,7 @@ extern "C" int marius_adamw_step(const marius_adamw_tensor* tensors, int32_t cou
         if (s.n == 0) continue;
         MARIUS_REQUIRE(s.param && s.grad && s.exp_avg && s.exp_avg_sq && (state_bits == 32 || (s.exp_avg_scale && s.exp_avg_sq_scale)), "adamw_step: null pointer in tensor %d", k);
         const int64_t more = cdiv(s.n, AW_TILE);
-        MARIUS_REQUIRE(more < (1ll << 30) && tiles + more < (1ll << 30), "adamw_step: over 2^41 elements in one call");
+        MARIUS_REQUIRE(tiles + more < (1ll << 24), "adamw_step: over 2^35 elements in one call");  // (a launch holds less than 2^32 lanes)
         tiles += more;
         ++live;
     }
