@@ -7,7 +7,7 @@
 namespace marius {
 
 constexpr float NA_INF = __builtin_inff();
-constexpr int NA_JOIN = 8;   // waves that join the parts of a long list
+constexpr int NA_JOIN = 2;   // waves that join the parts of a long list, for one head (hubs back: all heads of a list in one workgroup of 8 waves 778 us, one head in 2 waves 759, 4 761, 8 787)
 constexpr int NA_WAVES = 1;  // (waves of a workgroup: items differ in length, and a workgroup holds its registers until its longest wave ends: 4 waves 951 us, 2 852, 1 840 for the hubs of a power-law graph back)
 
 struct NaArgs {
@@ -130,19 +130,25 @@ __device__ __forceinline__ void load_biases(const NaArgs& A, int t, int end, int
 // p from a score and its list's (m, log l); a list without a live entry has m = -inf
 __device__ __forceinline__ float probability(float s, float m, float logl) { return __expf((s - finite_ref(m)) - logl); }
 
-// The parts of a long list: wave w takes parts w, w + NA_JOIN, ... in order, then the waves' results are joined in order.  This for sums: two rows of D, and (`more`) a number of their own; true for the lanes that hold the result
-template <int VEC>
-__device__ __forceinline__ bool join_sums(const NaArgs& A, int heads, bool more, int at, int h, float (&a)[VEC], float (&b)[VEC], float& first) {
-    __shared__ float red[NA_JOIN][2 * VEC + 1][64];
+// The parts of a long list, one head a workgroup: lane group g of G takes parts g, g + G, ... in order, then the groups' results are added in a fixed order.
+template <int LPH>
+struct JoinLane {
+    static constexpr int G = 64 * NA_JOIN / LPH;
+    int l, g, wave, h;
+    __device__ __forceinline__ JoinLane() : l(threadIdx.x & (LPH - 1)), g(threadIdx.x / LPH), wave(threadIdx.x >> 6), h(blockIdx.y) {}
+};
+// This for sums: two rows of D, and (`more`) a number of their own; true for the lanes that hold the result.
+template <int VEC, int LPH>
+__device__ __forceinline__ bool join_sums(const NaArgs& A, const JoinLane<LPH>& w, int heads, bool more, int at, float (&a)[VEC], float (&b)[VEC], float& first) {
+    __shared__ float red[NA_JOIN][2 * VEC + 1][LPH];
     if (na_block() >= (uint32_t)A.n_splits) return false;
     const int4 sp = A.splits[na_block()];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hc = h < heads ? h : heads - 1;
     first = 0.f;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) a[e] = b[e] = 0.f;
 #pragma unroll 4
-    for (int s = wave; s < sp.z; s += NA_JOIN) {
-        const int64_t o = (int64_t)(sp.y + s) * heads + hc;
+    for (int s = w.g; s < sp.z; s += w.G) {
+        const int64_t o = (int64_t)(sp.y + s) * heads + w.h;
         float x[VEC], y[VEC];
         __builtin_memcpy(x, A.part + o * 2 * A.D + at, sizeof(x));
         __builtin_memcpy(y, A.part + o * 2 * A.D + A.D + at, sizeof(y));
@@ -154,19 +160,30 @@ __device__ __forceinline__ bool join_sums(const NaArgs& A, int heads, bool more,
         }
     }
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        red[wave][e][lane] = a[e];
-        red[wave][VEC + e][lane] = b[e];
-    }
-    red[wave][2 * VEC][lane] = first;
-    __syncthreads();
-    if (wave != 0 || h >= heads) return false;
-    for (int s = 1; s < NA_JOIN; ++s) {
-        first += red[s][2 * VEC][lane];
+    for (int o = LPH; o < 64; o <<= 1) {
+        first += __shfl_xor(first, o, 64);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            a[e] += red[s][e][lane];
-            b[e] += red[s][VEC + e][lane];
+            a[e] += __shfl_xor(a[e], o, 64);
+            b[e] += __shfl_xor(b[e], o, 64);
+        }
+    }
+    if ((threadIdx.x & 63) < LPH) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            red[w.wave][e][w.l] = a[e];
+            red[w.wave][VEC + e][w.l] = b[e];
+        }
+        red[w.wave][2 * VEC][w.l] = first;
+    }
+    __syncthreads();
+    if (w.g != 0) return false;
+    for (int s = 1; s < NA_JOIN; ++s) {
+        first += red[s][2 * VEC][w.l];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            a[e] += red[s][e][w.l];
+            b[e] += red[s][VEC + e][w.l];
         }
     }
     return true;
@@ -185,7 +202,7 @@ static void na_launch(NaArgs A, int heads, hipStream_t st) {
     A.hp = 1;
     while (A.hp < groups && A.hp < lanes_heads) A.hp <<= 1;
     Pass::template launch<T, VEC, LPH>(A, na_grid(cdiv(A.n_items, NA_WAVES * (groups / A.hp)), cdiv(lanes_heads, A.hp)), dim3(64 * NA_WAVES), st);
-    if (A.n_splits > 0) Pass::template join<T, VEC, LPH>(A, na_grid(A.n_splits, cdiv(heads, groups)), dim3(64 * NA_JOIN), st);
+    if (A.n_splits > 0) Pass::template join<T, VEC, LPH>(A, na_grid(A.n_splits, heads), dim3(64 * NA_JOIN), st);
 }
 template <typename Pass, typename T>
 static void na_launch_width(const NaArgs& A, int heads, hipStream_t st) {

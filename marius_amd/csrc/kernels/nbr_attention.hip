@@ -101,50 +101,60 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_kernel(NaArgs A) 
     }
 }
 
-// The parts of a long list: wave w takes parts w, w + NA_JOIN, ... in order, then the waves' results are joined in order.
+// the parts of a long list
 template <typename T, int VEC, int LPH>
 __global__ __launch_bounds__(64 * NA_JOIN) void nbr_attention_join_kernel(NaArgs A) {
-    __shared__ float red[NA_JOIN][VEC + 2][64];
+    __shared__ float red[NA_JOIN][VEC + 2][LPH];
     if (na_block() >= (uint32_t)A.n_splits) return;
     const int4 sp = A.splits[na_block()];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = blockIdx.y * (64 / LPH) + lane / LPH, hc = h < A.H ? h : A.H - 1;
-    const Part<T, VEC, LPH> part(lane & (LPH - 1), A.D);
+    const JoinLane<LPH> w;
+    const Part<T, VEC, LPH> part(w.l, A.D);
     float acc[VEC], m = -NA_INF, sum = 0.f;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
     auto join = [&](float om, float os, const float(&v)[VEC]) {
-        const float top = fmaxf(m, om), ref = finite_ref(top), w = weight_to(m, ref), ow = weight_to(om, ref);
-        sum = sum * w + os * ow;
+        const float top = fmaxf(m, om), ref = finite_ref(top), mine = weight_to(m, ref), other = weight_to(om, ref);
+        sum = sum * mine + os * other;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] = acc[e] * w + v[e] * ow;
+        for (int e = 0; e < VEC; ++e) acc[e] = acc[e] * mine + v[e] * other;
         m = top;
     };
 #pragma unroll 4
-    for (int s = wave; s < sp.z; s += NA_JOIN) {
-        const int64_t o = (int64_t)(sp.y + s) * A.H + hc;
+    for (int s = w.g; s < sp.z; s += w.G) {
+        const int64_t o = (int64_t)(sp.y + s) * A.H + w.h;
         float v[VEC];
         __builtin_memcpy(v, A.part + o * A.D + part.at, sizeof(v));
         const float2 ms = A.part2[o];
         join(ms.x, ms.y, v);
     }
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) red[wave][e][lane] = acc[e];
-    red[wave][VEC][lane] = m;
-    red[wave][VEC + 1][lane] = sum;
+    for (int o = LPH; o < 64; o <<= 1) {
+        float v[VEC];
+        const float om = __shfl_xor(m, o, 64), os = __shfl_xor(sum, o, 64);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = __shfl_xor(acc[e], o, 64);
+        join(om, os, v);
+    }
+    if ((threadIdx.x & 63) < LPH) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) red[w.wave][e][w.l] = acc[e];
+        red[w.wave][VEC][w.l] = m;
+        red[w.wave][VEC + 1][w.l] = sum;
+    }
     __syncthreads();
-    if (wave != 0 || h >= A.H) return;
+    if (w.g != 0) return;
     for (int s = 1; s < NA_JOIN; ++s) {
         float v[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = red[s][e][lane];
-        join(red[s][VEC][lane], red[s][VEC + 1][lane], v);
+        for (int e = 0; e < VEC; ++e) v[e] = red[s][e][w.l];
+        join(red[s][VEC][w.l], red[s][VEC + 1][w.l], v);
     }
     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] *= inv;
-    const int64_t o = (int64_t)sp.x * A.H + h;
+    const int64_t o = (int64_t)sp.x * A.H + w.h;
     part.store((T*)A.out + o * A.D, acc);
-    if ((lane & (LPH - 1)) == 0) {
+    if (w.l == 0) {
         A.stats[o * 2] = m;
         A.stats[o * 2 + 1] = sum == 0.f ? 0.f : logf(sum);
     }

@@ -92,13 +92,13 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dkv_kernel(NaArgs
 }
 template <typename T, int VEC, int LPH>
 __global__ __launch_bounds__(64 * NA_JOIN) void nbr_attention_dkv_join_kernel(NaArgs A) {
-    const int lane = threadIdx.x & 63, h = blockIdx.y * (64 / LPH) + lane / LPH;
-    const Part<T, VEC, LPH> part(lane & (LPH - 1), A.D);
+    const JoinLane<LPH> w;
+    const Part<T, VEC, LPH> part(w.l, A.D);
     float dk[VEC], dv[VEC], none;
-    if (!join_sums<VEC>(A, A.Hkv, false, part.at, h, dk, dv, none)) return;
+    if (!join_sums<VEC, LPH>(A, w, A.Hkv, false, part.at, dk, dv, none)) return;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) dk[e] *= A.scale;
-    const int64_t o = ((int64_t)A.splits[na_block()].x * A.Hkv + h) * A.D;
+    const int64_t o = ((int64_t)A.splits[na_block()].x * A.Hkv + w.h) * A.D;
     part.store((T*)A.dk + o, dk);
     part.store((T*)A.dv + o, dv);
 }

@@ -85,14 +85,14 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_dq_kernel(NaArgs 
 }
 template <typename T, int VEC, int LPH>
 __global__ __launch_bounds__(64 * NA_JOIN) void nbr_attention_dq_join_kernel(NaArgs A) {
-    const int lane = threadIdx.x & 63, h = blockIdx.y * (64 / LPH) + lane / LPH;
-    const Part<T, VEC, LPH> part(lane & (LPH - 1), A.D);
+    const JoinLane<LPH> w;
+    const Part<T, VEC, LPH> part(w.l, A.D);
     float pdk[VEC], pk[VEC], delta;
-    if (!join_sums<VEC>(A, A.H, true, part.at, h, pdk, pk, delta)) return;
+    if (!join_sums<VEC, LPH>(A, w, A.H, true, part.at, pdk, pk, delta)) return;
     dq_of<VEC>(pdk, pk, delta, A.scale);
-    const int64_t o = (int64_t)A.splits[na_block()].x * A.H + h;
+    const int64_t o = (int64_t)A.splits[na_block()].x * A.H + w.h;
     part.store((T*)A.out + o * A.D, pdk);
-    if ((lane & (LPH - 1)) == 0) A.rowstats[o] = make_float4(A.stats[o * 2], A.stats[o * 2 + 1], delta, 0.f);
+    if (w.l == 0) A.rowstats[o] = make_float4(A.stats[o * 2], A.stats[o * 2 + 1], delta, 0.f);
 }
 
 struct DqPass {

@@ -760,9 +760,9 @@ def residual_norm_backward(grad_y, grad_h, y, block=None, gate=None, post_weight
 
 
 def plan_chunk(entries):
-    """entries of a work item: as few as still pay for their partial results, because an item's loads follow one another (measured, us, at 16 / 32 / 64 / 128 / 256
-    entries: a pass there and back over 1.5 M entries 1529 / 1184 / 1078 / 1027 / 1035, over 200,000 entries 103 / 103 / 121 / 174 / 254, one served list of 8192
-    16 / 14 / 16 / 22 / 35)"""
+    """entries of a work item: as few as still pay for their partial results, because an item's loads follow one another (measured, us, at 32 / 64 / 128 / 192
+    entries: a pass there and back over 1.5 M entries 1207 / 1073 / 1008 / 996, over 200,000 entries 88 / 112 / 173 / 233; one served list of 8192 entries at
+    16 / 32 / 64: 14.5 / 13.4 / 16.0)"""
     return 128 if entries >= 1 << 20 else 32
 
 
