@@ -204,8 +204,8 @@ struct Heads {
     int64_t row, head;
     explicit Heads(const Tensor& given) : t(given) {
         if (t.stride(2) != 1 && t.size(2) > 1) t = t.contiguous();
-        row = t.stride(0);
-        head = t.stride(1);
+        row = t.size(0) > 1 ? t.stride(0) : 0;  // (of a single row or head: whatever a view left there)
+        head = t.size(1) > 1 ? t.stride(1) : 0;
     }
 };
 struct AttentionCall {
@@ -388,6 +388,8 @@ void adamw_step(uintptr_t entry, uintptr_t workspace_entry, AdamWTensors& a, con
     check(((decltype(&marius_adamw_step))entry)(table.data(), (int32_t)count, a.type, grad_type, a.bits, on_device ? 0 : step.cast<int64_t>(), (const int64_t*)data(counter), lr, beta1,
                                                 beta2, eps, weight_decay, (const float*)data(grad_scale), need ? ws.data_ptr() : nullptr, need, stream_of(device)),
           "adamw_step");
+    for (size_t i = 0; i < count; ++i)  // a graph that saved the old values may not go back through the new ones
+        if (grads[i] && !a.params[i].is_inference()) a.params[i].unsafeGetTensorImpl()->bump_version();
 }
 
 }  // namespace

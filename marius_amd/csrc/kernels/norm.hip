@@ -39,10 +39,10 @@ enum { SUM_POST_W = 0, SUM_POST_B, SUM_PRE_W, SUM_PRE_B, SUM_GATE, SUMS };
 
 // (sigmoid: the hardware's exponential and reciprocal, a step of fp32 or two together)
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
-__device__ __forceinline__ float gate_act(float v, int act) { return act == MARIUS_ACT_RELU ? fmaxf(v, 0.f) : act == MARIUS_ACT_SIGMOID ? sigmoid(v) : v; }
+__device__ __forceinline__ float gate_act(float v, int act) { return act == MARIUS_ACT_RELU ? (v < 0.f ? 0.f : v) : act == MARIUS_ACT_SIGMOID ? sigmoid(v) : v; }
 // act' from the gate g and a = act(g)
 __device__ __forceinline__ float gate_slope(float g, float a, int act) {
-    if (act == MARIUS_ACT_RELU) return g > 0.f ? 1.f : 0.f;
+    if (act == MARIUS_ACT_RELU) return g <= 0.f ? 0.f : 1.f;
     if (act == MARIUS_ACT_SIGMOID) return a * (1.f - a);
     return 1.f;
 }
@@ -175,7 +175,7 @@ struct Row {
     // g -> act(g)
     __device__ __forceinline__ void open(Values& g, int act) const {
         if (act == MARIUS_ACT_SIGMOID) EACH(NCH, VEC) g[j][e] = sigmoid(g[j][e]);
-        else if (act == MARIUS_ACT_RELU) EACH(NCH, VEC) g[j][e] = fmaxf(g[j][e], 0.f);
+        else if (act == MARIUS_ACT_RELU) EACH(NCH, VEC) g[j][e] = g[j][e] < 0.f ? 0.f : g[j][e];  // (NaN stays)
     }
 };
 
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(!BLK ? NORM_T : NCH > 1 ? NORM_MAX_T / 2 : NORM_MAX
                 if (live) EACH(NCH, VEC) acc[SUM_GATE][j][e] += u[j][e];
             } else {
                 R.get(gp, gc);
-                if (A.act == MARIUS_ACT_RELU) EACH(NCH, VEC) u[j][e] = gc[j][e] > 0.f ? u[j][e] : 0.f;
+                if (A.act == MARIUS_ACT_RELU) EACH(NCH, VEC) u[j][e] = gc[j][e] <= 0.f ? 0.f : u[j][e];
                 R.open(gc, A.act);
                 if (A.act == MARIUS_ACT_SIGMOID) EACH(NCH, VEC) u[j][e] *= gc[j][e] * (1.f - gc[j][e]);
                 if (live) R.template store<T>(A.dgate, row, A.dgate_ld, u);

@@ -388,6 +388,7 @@ class _ResidualNorm(torch.autograd.Function):
     def forward(ctx, x, block, gate, post_weight, post_bias, pre_weight, pre_bias, how):
         y, h = H.residual_norm(x, block, gate, post_weight, post_bias, pre_weight, pre_bias, **how)
         ctx.how, ctx.with_y, ctx.with_h = how, block is not None, h is not None
+        ctx.set_materialize_grads(False)  # (the last layer's y has no gradient: none is read)
         ctx.save_for_backward(y, block, gate, post_weight, post_bias, pre_weight, pre_bias)
         return tuple(t for t, there in ((y, ctx.with_y), (h, ctx.with_h)) if there)
 
@@ -397,6 +398,8 @@ class _ResidualNorm(torch.autograd.Function):
         grads = list(grads)
         grad_y = grads.pop(0) if ctx.with_y else None
         grad_h = grads.pop(0) if ctx.with_h else None
+        if grad_y is None and grad_h is None:
+            return (None,) * 8
         got = H.residual_norm_backward(grad_y, grad_h, *ctx.saved_tensors, need_dx=ctx.needs_input_grad[0], **ctx.how)
         return tuple(got[k] for k in ("dx", "dblock", "dgate", "dpost_weight", "dpost_bias", "dpre_weight", "dpre_bias")) + (None,)
 

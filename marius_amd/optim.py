@@ -1,4 +1,4 @@
-"""AdamW over all parameters of a model in one launch per 64 tensors (marius_adamw_step), beside the dense Adagrad / Adam steps of marius_amd.hip."""
+"""AdamW over all parameters of a model in one launch (marius_adamw_step), beside the dense Adagrad / Adam steps of marius_amd.hip."""
 import torch
 
 from . import hip as H

@@ -251,3 +251,13 @@ def test_encoder_modules_refuse(HE):
     refused(HE, "comes with the call", gnn.ResidualNorm(4, device=CPU), torch.zeros(2, 4), torch.zeros(2, 4), torch.zeros(2, 4))
     refused(HE, "no parameters", AdamW, [])
     refused(HE, "32 or in 8", AdamW, [torch.zeros(3)], state_bits=16)
+
+
+def test_emulated_single_rows_nan_gates_and_absent_gradients(HE):
+    from marius_amd import gnn
+
+    T.test_views_of_one_row_may_have_any_stride(HE, CPU)
+    for gate in ("channel", "element"):
+        T.test_nan_goes_through_a_relu_gate(HE, CPU, gate)
+    T.test_norm_without_a_gradient_of_its_stream(HE, gnn, CPU)
+    T.test_adamw_step_is_seen_by_graphs_that_saved_the_parameter(HE, CPU)

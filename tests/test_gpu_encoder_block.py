@@ -556,3 +556,51 @@ def test_gradient_of_a_sum_reaches_every_operand(H, G, dev):
     y, h = G.ResidualNorm(1, post_norm=True, bias=True, device=dev)(x, torch.randn(5, 1, device=dev))
     (y.sum() + h.sum()).backward()
     assert torch.isfinite(x.grad).all()
+
+
+def test_views_of_one_row_may_have_any_stride(H, dev):
+    """a dimension of size one says nothing with its stride"""
+    plan = H.NeighborPlan(torch.tensor([0, 0], device=dev), torch.tensor([0], device=dev), 1)
+    q, k, grad = (torch.randn(1, 2, 8, device=dev) for _ in range(3))
+    far = lambda t: t.as_strided((1, 2, 8), (1 << 40, 8, 1))  # noqa: E731
+    out, stats = H.neighbor_attention(far(q), far(k), far(k), plan)
+    assert torch.equal(out, H.neighbor_attention(q, k, k, plan)[0])
+    for a, b in zip(H.neighbor_attention_backward(far(grad), far(q), far(k), far(k), stats, plan), H.neighbor_attention_backward(grad, q, k, k, stats, plan)):
+        assert a is b is None or torch.equal(a, b)
+
+
+@pytest.mark.parametrize("gate", ["channel", "element"])
+def test_nan_goes_through_a_relu_gate(H, dev, gate):
+    x, z, g = torch.randn(3, 8, device=dev), torch.randn(3, 8, device=dev), torch.randn(8, device=dev)
+    g[2], g[3] = float("nan"), -1.0
+    g = g if gate == "channel" else g.expand(3, 8).contiguous()
+    how = dict(pre_norm=False, gate_activation="RELU")
+    y = H.residual_norm(x, z, g, **how)[0]
+    assert y[:, 2].isnan().all() and torch.equal(y[:, 3], x[:, 3])
+    got = H.residual_norm_backward(torch.ones_like(x), None, y, z, g, **how)
+    assert got["dblock"][:, 2].isnan().all() and (got["dblock"][:, 3] == 0).all()
+
+
+def test_norm_without_a_gradient_of_its_stream(H, G, dev):
+    """the last block's y is not used: its gradient is absent, not zeros"""
+    norm = G.ResidualNorm(16, device=dev)
+    grads = []
+    for use in (0.0, None):
+        x, z = (torch.linspace(-1, 2, 48, device=dev).view(3, 16).sin().requires_grad_(True) for _ in range(2))
+        y, h = norm(x, z)
+        ((h * h).sum() if use is None else (h * h).sum() + use * y.sum()).backward()
+        grads.append((x.grad, z.grad))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_adamw_step_is_seen_by_graphs_that_saved_the_parameter(H, dev):
+    from marius_amd.optim import AdamW
+
+    p, q = (torch.nn.Parameter(torch.randn(4, device=dev)) for _ in range(2))
+    opt = AdamW([p, q])
+    loss = (p * p).sum()
+    p.grad, before = torch.ones_like(p), (p._version, q._version)
+    opt.step()
+    assert (p._version, q._version) == (before[0] + 1, before[1])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
