@@ -3,6 +3,7 @@ the sizes a fiber per work-item can walk; refusals of every entry point; the ref
 import ctypes as C
 import math
 import os
+import subprocess
 import sys
 
 import pytest
@@ -261,3 +262,18 @@ def test_emulated_single_rows_nan_gates_and_absent_gradients(HE):
         T.test_nan_goes_through_a_relu_gate(HE, CPU, gate)
     T.test_norm_without_a_gradient_of_its_stream(HE, gnn, CPU)
     T.test_adamw_step_is_seen_by_graphs_that_saved_the_parameter(HE, CPU)
+
+
+def test_encoder_block_under_address_and_undefined_behaviour_sanitizers():
+    """the forms above that reach every kernel at odd sizes, and every refusal, once more in a python started under libasan with the kernel files built with
+    -fsanitize=address,undefined (libstdc++ is loaded with it: the host module's refusals are C++ exceptions)"""
+    if os.environ.get("MARIUS_EMUL_SANITIZE") == "1":
+        pytest.skip("already inside the sanitizer run")
+    libraries = [subprocess.run(["gcc", "-print-file-name=" + name], stdout=subprocess.PIPE, text=True).stdout.strip() for name in ("libasan.so", "libstdc++.so")]
+    if not all(os.path.isabs(p) and os.path.exists(p) for p in libraries):
+        pytest.skip("no libasan.so next to gcc")
+    env = dict(os.environ, MARIUS_EMUL_SANITIZE="1", LD_PRELOAD=" ".join(libraries), ASAN_OPTIONS="detect_leaks=0:abort_on_error=1", UBSAN_OPTIONS="halt_on_error=1:print_stacktrace=1")
+    select = "not sanitizers" if os.environ.get("MARIUS_EMUL_SANITIZE_ALL") == "1" else "small_forms or single_rows or refuse or adamw or masks or (residual_norm and 2047) or (single and 256)"
+    r = subprocess.run([sys.executable, "-m", "pytest", os.path.abspath(__file__), "-x", "-q", "-p", "no:cacheprovider", "-k", select], env=env, stdout=subprocess.PIPE,
+                       stderr=subprocess.STDOUT, text=True, timeout=2400, cwd=os.path.dirname(HERE))
+    assert r.returncode == 0 and " passed" in r.stdout, r.stdout[-4000:]
