@@ -39,13 +39,13 @@ class AdamW:
         if self.capturable:
             for t in self._step_dev.values():
                 t.add_(1)
-        else:
-            self.num_steps += 1
         for at, tensors in self._groups:
             grads = [self.params[i].grad for i in at]
             for kind in {g.dtype for g in grads if g is not None}:   # (one kind of gradient in every program we know of)
-                H.adamw_step(tensors, [g if g is not None and g.dtype == kind else None for g in grads], self._step_dev[tensors.device] if self.capturable else self.num_steps,
+                H.adamw_step(tensors, [g if g is not None and g.dtype == kind else None for g in grads], self._step_dev[tensors.device] if self.capturable else self.num_steps + 1,
                              self.lr, *self.betas, self.eps, self.weight_decay, grad_scale)
+        if not self.capturable:
+            self.num_steps += 1  # (a refused step does not count)
 
     def state_dict(self):
         steps = int(next(iter(self._step_dev.values()))) if self.capturable else self.num_steps

@@ -262,6 +262,7 @@ def test_emulated_single_rows_nan_gates_and_absent_gradients(HE):
         T.test_nan_goes_through_a_relu_gate(HE, CPU, gate)
     T.test_norm_without_a_gradient_of_its_stream(HE, gnn, CPU)
     T.test_adamw_step_is_seen_by_graphs_that_saved_the_parameter(HE, CPU)
+    T.test_a_refused_optimizer_step_does_not_count(HE, CPU)
 
 
 def test_encoder_block_under_address_and_undefined_behaviour_sanitizers():

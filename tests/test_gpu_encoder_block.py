@@ -604,3 +604,67 @@ def test_adamw_step_is_seen_by_graphs_that_saved_the_parameter(H, dev):
     assert (p._version, q._version) == (before[0] + 1, before[1])
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("rows,kind", [(20000, BF16), (900000, F32)])
+def test_neighbor_attention_over_a_million_entries(H, dev, rows, kind):
+    """a plan whose work items are the longer ones: a hub, many ordinary lists, empty ones; rows in many lists, or in one or none"""
+    g = torch.Generator().manual_seed(rows)
+    lengths = torch.randint(0, 70, (31000,), generator=g)
+    lengths[17] = 40000
+    index, offsets = lists(lengths.numel(), rows, lengths.tolist(), 4)
+    assert index.numel() > 1 << 20
+    both_ways(H, dev, index, offsets, rows, 2, 1, 16, kind, relation_bias(2, 3), seed=5)
+
+
+def test_neighbor_attention_rows_behind_four_gib(H, dev):
+    """k and v of 4.6 GB each: the rows that lie behind 2^32 bytes give what the same rows give alone"""
+    rows, n, dim = 9_000_000, 40, 128
+    near = torch.randint(0, 64, (n * 9,), generator=torch.Generator().manual_seed(1)).to(dev)
+    offsets = (torch.arange(n) * 9).to(dev)
+    q, g, k = rows_of(n, 2, dim, F32, dev, 1), rows_of(n, 2, dim, F32, dev, 2), rows_of(64, 1, dim, F32, dev, 3)
+    small = H.NeighborPlan(near, offsets, 64)
+    out, stats = H.neighbor_attention(q, k, k, small)
+    want = H.neighbor_attention_backward(g, q, k, k, stats, small)
+    wide = torch.zeros(rows, 1, dim, device=dev)
+    wide[rows - 64:] = k
+    plan = H.NeighborPlan(near + (rows - 64), offsets, rows)
+    far, far_stats = H.neighbor_attention(q, wide, wide, plan)
+    dq, dk, dv, _ = H.neighbor_attention_backward(g, q, wide, wide, far_stats, plan)
+    assert torch.equal(far, out) and torch.equal(far_stats, stats) and torch.equal(dq, want[0])
+    assert torch.equal(dk[rows - 64:], want[1]) and torch.equal(dv[rows - 64:], want[2])
+    assert not bool(dk[:rows - 64].any()) and not bool(dv[:rows - 64].any())
+
+
+def test_adamw_of_many_tensors_in_two_graphs_of_one_pool(H, dev):
+    """a list that goes through a table in workspace, captured twice into one pool and replayed in turn: every replay is the eager step"""
+    sizes = [300] * 70
+    runs = [adamw_case(H, dev, sizes, F32, F32, 32, seed) for seed in (1, 2)]
+    eager = [adamw_case(H, dev, sizes, F32, F32, 32, seed) for seed in (1, 2)]
+    tensors, plain = ([H.AdamWTensors(ps, ms, vs) for ps, _, ms, vs, _, _ in rs] for rs in (runs, eager))
+    step, pool, graphs = torch.zeros(1, dtype=torch.int64, device=dev), torch.cuda.graph_pool_handle(), []
+    torch.cuda.synchronize()
+    for t, (_, gs, *_) in zip(tensors, runs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=pool):
+            H.adamw_step(t, gs, step)
+    for r in range(3):
+        step.add_(1)
+        for graph, p, (_, gs, *_) in zip(graphs, plain, eager):
+            graph.replay()
+            H.adamw_step(p, gs, step)
+        torch.cuda.synchronize()
+        for a, b in zip(runs, eager):
+            assert all(torch.equal(x, y) for k in (0, 2, 3) for x, y in zip(a[k], b[k])), r
+
+
+def test_a_refused_optimizer_step_does_not_count(H, dev):
+    from marius_amd.optim import AdamW
+
+    p = torch.nn.Parameter(torch.ones(8, device=dev))
+    opt = AdamW([p])
+    p.grad = torch.ones_like(p)
+    with pytest.raises(H.MariusHipError):
+        opt.step(grad_scale=torch.ones(2, device=dev))
+    opt.step()
+    assert opt.num_steps == 1 and bool((p < 1).all())
