@@ -49,7 +49,7 @@ enum {
  * marius_table_absmax_counted; marius_lp_layout lost the operand planes of the removed bf16x6 kernels and the stream-K partials; 8:
  * marius_lp_desc.upd_*, marius_segment_update.fused_below, marius_lp_fuses_endpoint_update, marius_segment_plan_occ_single; 9: the
  * fixed-capacity exchange entry points marius_a2a_capacity / marius_a2a_rows_post / marius_a2a_rows_wait, negative ids = padding slots in
- * marius_merge_unique_runs / marius_segment_plan; 10: marius_a2a_publish / marius_a2a_record_* / marius_owner_offsets_counts, marius_layer_post_hook*, marius_prepare_maps; 11: marius_lp_layout.flash_cfg, marius_prepare_maps_preferred, the neighbour-sampling / GraphSage entry points marius_nbr_* and marius_segment_gather_sum; 12: marius_residual_norm_*, marius_nbr_plan_* / marius_neighbor_attention_*, marius_adamw_step).  Every binder
+ * marius_merge_unique_runs / marius_segment_plan; 10: marius_a2a_publish / marius_a2a_record_* / marius_owner_offsets_counts, marius_layer_post_hook*, marius_prepare_maps; 11: marius_lp_layout.flash_cfg, marius_prepare_maps_preferred, the neighbour-sampling / GraphSage entry points marius_nbr_* and marius_segment_gather_sum; 12: marius_residual_norm_*, marius_nbr_plan_* / marius_neighbor_attention_*, marius_bin_sum, marius_adamw_step).  Every binder
  * compares the value it was built against with what the loaded library returns and refuses to run on a mismatch: marius_amd/hip.py lib(),
  * the host module's init (bindings.cpp), and the plug-in recipe of INTEGRATION.md. */
 #define MARIUS_HIP_ABI_VERSION 12
@@ -644,6 +644,11 @@ int marius_neighbor_attention_forward(const marius_neighbor_plan* plan, const ma
                                       marius_stream_t stream);
 int marius_neighbor_attention_backward(const marius_neighbor_plan* plan, const marius_neighbor_attention* desc, const void* grad_out, int64_t grad_row, int64_t grad_head,
                                        void* dq, void* dk, void* dv, float* dbias, void* workspace, size_t workspace_bytes, marius_stream_t stream);
+
+/* Rows summed by bins (bin_sum.hip), the gradient of a table of biases that the entries share: out[b, h] = sum of values[e, h] over the entries with bin[e] = b, for up to
+ * 256 bins; out [bins, heads] is written whole, an entry whose bin is not one of them is left out.  No atomics: the same bits on every run. */
+size_t marius_bin_sum_workspace_bytes(int64_t T, int32_t heads, int32_t bins);
+int marius_bin_sum(const float* values, const int64_t* bin, int64_t T, int32_t heads, int32_t bins, float* out, void* workspace, size_t workspace_bytes, marius_stream_t stream);
 
 /* AdamW over many tensors (adamw.hip): p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps), moments m and v updated first; t = step (from 1),
  * or *step_dev (a captured call replays with the step it finds there).  Every gradient is multiplied by *grad_scale (NULL: 1).  All tensors of a call have

@@ -404,6 +404,21 @@ class _ResidualNorm(torch.autograd.Function):
         return tuple(got[k] for k in ("dx", "dblock", "dgate", "dpost_weight", "dpost_bias", "dpre_weight", "dpre_bias")) + (None,)
 
 
+class _TableRows(torch.autograd.Function):
+    """rows of a small table, one for every entry: the gradient is a sum by bins (bin_sum.hip), not atomics on a handful of rows"""
+
+    @staticmethod
+    def forward(ctx, table, rows):
+        ctx.save_for_backward(rows)
+        ctx.bins = table.size(0)
+        return table.index_select(0, rows)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return H.bin_sum(grad, ctx.saved_tensors[0], ctx.bins), None
+
+
 def neighbor_attention(q, k, v, plan, scale=None, bias=None):
     """differentiable H.neighbor_attention: out [n, heads, dim]"""
     return _NeighborAttention.apply(q, k, v, bias, plan, scale)
@@ -452,7 +467,11 @@ class GraphAttentionLayer(torch.nn.Module):
         n = plan.n
         q = torch.matmul(inputs.narrow(0, inputs.size(0) - n, n), self.wq.t()).view(n, self.heads, self.dim)
         kv = torch.matmul(inputs, self.wkv.t()).view(inputs.size(0), 2, self.kv_heads, self.dim)
-        bias = None if self.relation_bias is None else self.relation_bias.index_select(0, dense_graph.entryRelations(self.relation_bias.size(0) - 1))
+        bias = None
+        if self.relation_bias is not None:
+            relations = dense_graph.entryRelations(self.relation_bias.size(0) - 1)
+            few = self.relation_bias.size(0) <= H.MAX_BINS and self.heads <= 1024  # (more rows: an embedding's gradient, summed over sorted entries)
+            bias = _TableRows.apply(self.relation_bias, relations) if few else torch.nn.functional.embedding(relations, self.relation_bias)
         out = neighbor_attention(q, kv[:, 0], kv[:, 1], plan, None, bias)
         return torch.matmul(out.view(n, self.heads * self.dim), self.wo.t())
 

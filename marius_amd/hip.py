@@ -147,6 +147,8 @@ SIGNATURES = {
     "marius_neighbor_attention_workspace_bytes": (_sz, [C.POINTER(NeighborPlanDesc), _i32, _i32, _i32, _i32]),
     "marius_neighbor_attention_forward": (C.c_int, [C.POINTER(NeighborPlanDesc), C.POINTER(NeighborAttention), _vp, _vp, _sz, _vp]),
     "marius_neighbor_attention_backward": (C.c_int, [C.POINTER(NeighborPlanDesc), C.POINTER(NeighborAttention), _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "marius_bin_sum_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "marius_bin_sum": (C.c_int, [_vp, _vp, _i64, _i32, _i32, _vp, _vp, _sz, _vp]),
     "marius_adamw_step": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i64, _vp, _f64, _f64, _f64, _f64, _f64, _vp, _vp, _sz, _vp]),
     "marius_adamw_workspace_bytes": (_sz, [_i32]),
     "marius_owner_offsets_counts": (C.c_int, [_vp, _vp, _i64, _i32, _vp, _vp, _vp]),
@@ -868,6 +870,27 @@ def neighbor_attention_backward(grad_out, q, k, v, stats, plan, scale=None, bias
     _dev(q)
     return _ops().neighbor_attention_backward(_entry("marius_neighbor_attention_backward"), _entry("marius_neighbor_attention_workspace_bytes"), _plan(plan).address, plan.index, grad_out,
                                               q, k, v, stats, scale, bias, need_dbias)
+
+
+MAX_BINS = 256  # of bin_sum
+
+
+def bin_sum(values, bins_of, bins):
+    """[bins, heads]: the rows of values [entries, heads] (float32) summed by the bin (int64) of their entry, 1 to 256 bins; an entry of no bin is left out.  No atomics:
+    the same bits on every run (the gradient of a small table of which every entry takes a row)."""
+    _dev(values)
+    _require(values.dim() == 2 and values.dtype == torch.float32 and 1 <= values.size(1) <= 1024, "bin_sum: values are float32 [entries, heads], up to 1024 heads")
+    _require(bins_of.dim() == 1 and bins_of.dtype == torch.int64 and bins_of.numel() == values.size(0), "bin_sum: an int64 bin for every entry")
+    _require(bins_of.device == values.device, "bin_sum: values and bins are on one device")
+    _require(1 <= bins <= MAX_BINS, "bin_sum: 1 to %d bins", MAX_BINS)
+    values, bins_of, dev = values.contiguous(), bins_of.contiguous(), values.device
+    T, heads, L = values.size(0), values.size(1), lib()
+    with torch.cuda.device(dev if dev.type == "cuda" else -1):  # (launches go to the current device)
+        out = torch.empty(bins, heads, dtype=torch.float32, device=dev)
+        wsb = L.marius_bin_sum_workspace_bytes(T, heads, bins)
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+        check(L.marius_bin_sum(ptr(values), ptr(bins_of), T, heads, bins, ptr(out), ptr(ws), wsb, stream_ptr()), "bin_sum")
+    return out
 
 
 ADAMW_BLOCK = 256  # elements of an 8-bit state that share a scale

@@ -12,7 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 KDIR = os.path.join(ROOT, "marius_amd", "csrc", "kernels")
 FILES = ["neighbor.hip", "rows.hip", "rng.hip", "encoder.hip", "segreduce.hip", "sort_unique.hip", "exchange.hip", "lp_decoder.hip", "eval_filter.hip",
-         "norm.hip", "adamw.hip", "nbr_plan.hip", "nbr_attention.hip", "nbr_attention_dq.hip", "nbr_attention_dkv.hip"]
+         "norm.hip", "adamw.hip", "nbr_plan.hip", "nbr_attention.hip", "nbr_attention_dq.hip", "nbr_attention_dkv.hip", "bin_sum.hip"]
 HEADERS = ["seg_plan.h", "lp_common.h", "row_types.h", "nbr_attention.h"]  # kernel-side headers the files include by name: copied next to them (their own `#include "common.h"` then finds the shim)
 
 

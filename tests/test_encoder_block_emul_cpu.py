@@ -265,6 +265,28 @@ def test_emulated_single_rows_nan_gates_and_absent_gradients(HE):
     T.test_a_refused_optimizer_step_does_not_count(HE, CPU)
 
 
+@pytest.mark.parametrize("entries,heads,bins", [(0, 3, 5), (9, 4, 6), (777, 5, 256), (300, 100, 3), (2049, 33, 41)])
+def test_emulated_bin_sum(HE, entries, heads, bins):
+    T.test_bin_sum(HE, CPU, entries, heads, bins)
+
+
+def test_emulated_layer_with_many_relations(HE):
+    from marius_amd import gnn
+
+    T.test_attention_layer_with_more_relations_than_bins(HE, gnn, CPU)
+
+
+def test_bin_sum_refuses(HE):
+    v, b = torch.zeros(4, 3), torch.zeros(4, dtype=torch.int64)
+    refused(HE, "float32 \\[entries, heads\\]", HE.bin_sum, v.double(), b, 2)
+    refused(HE, "float32 \\[entries, heads\\]", HE.bin_sum, v[0], b, 2)
+    refused(HE, "float32 \\[entries, heads\\]", HE.bin_sum, torch.zeros(4, 0), b, 2)
+    refused(HE, "int64 bin for every", HE.bin_sum, v, b.int(), 2)
+    refused(HE, "int64 bin for every", HE.bin_sum, v, b[:3], 2)
+    refused(HE, "1 to 256 bins", HE.bin_sum, v, b, 0)
+    refused(HE, "1 to 256 bins", HE.bin_sum, v, b, 257)
+
+
 def test_encoder_block_under_address_and_undefined_behaviour_sanitizers():
     """the forms above that reach every kernel at odd sizes, and every refusal, once more in a python started under libasan with the kernel files built with
     -fsanitize=address,undefined (libstdc++ is loaded with it: the host module's refusals are C++ exceptions)"""
@@ -274,7 +296,7 @@ def test_encoder_block_under_address_and_undefined_behaviour_sanitizers():
     if not all(os.path.isabs(p) and os.path.exists(p) for p in libraries):
         pytest.skip("no libasan.so next to gcc")
     env = dict(os.environ, MARIUS_EMUL_SANITIZE="1", LD_PRELOAD=" ".join(libraries), ASAN_OPTIONS="detect_leaks=0:abort_on_error=1", UBSAN_OPTIONS="halt_on_error=1:print_stacktrace=1")
-    select = "not sanitizers" if os.environ.get("MARIUS_EMUL_SANITIZE_ALL") == "1" else "small_forms or single_rows or refuse or adamw or masks or (residual_norm and 2047) or (single and 256)"
+    select = "not sanitizers" if os.environ.get("MARIUS_EMUL_SANITIZE_ALL") == "1" else "small_forms or single_rows or refuse or adamw or bin_sum or masks or (residual_norm and 2047) or (single and 256)"
     r = subprocess.run([sys.executable, "-m", "pytest", os.path.abspath(__file__), "-x", "-q", "-p", "no:cacheprovider", "-k", select], env=env, stdout=subprocess.PIPE,
                        stderr=subprocess.STDOUT, text=True, timeout=2400, cwd=os.path.dirname(HERE))
     assert r.returncode == 0 and " passed" in r.stdout, r.stdout[-4000:]

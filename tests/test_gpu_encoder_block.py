@@ -668,3 +668,52 @@ def test_a_refused_optimizer_step_does_not_count(H, dev):
         opt.step(grad_scale=torch.ones(2, device=dev))
     opt.step()
     assert opt.num_steps == 1 and bool((p < 1).all())
+
+
+def test_encoder_gradients_are_the_same_on_every_run(H, G, dev):
+    """every gradient of a whole encoder, the relation biases' among them (many entries share a row), bit for bit"""
+    torch.manual_seed(3)
+    enc = G.GraphAttentionEncoder(16, 32, 4, 2, 4, kv_heads=2, num_relations=5, device=dev)
+    runs = []
+    for _ in range(4):
+        enc.zero_grad()
+        graph = sampled(G, dev, 3000, 60000, [12, 9], True, True, 400, 3)
+        features = torch.randn(graph.node_ids_.numel(), 16, generator=torch.Generator().manual_seed(1)).to(dev)
+        enc(features, graph).square().sum().backward()
+        runs.append([p.grad.clone() for p in enc.parameters()])
+    for again in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], again))
+
+
+@pytest.mark.parametrize("T,heads,bins", [(0, 3, 5), (1, 1, 1), (9, 4, 6), (1000, 8, 6), (777, 5, 256), (3000, 64, 7), (300, 100, 3), (2049, 33, 41), (50000, 8, 6)])
+def test_bin_sum(H, dev, T, heads, bins):
+    """sums by bins against 64 bits, entries of no bin left out, strided values, the same bits again.  Bound: a sum of N products of one has N roundings of the running sum, each
+    at most half a step of the sum of magnitudes: N lanes, workgroups and entries together stay below T / 64 + 200 of them in a row."""
+    g = torch.Generator().manual_seed(T + heads)
+    v, b = torch.randn(T, heads, generator=g), torch.randint(-1, bins + 1, (T,), generator=g)
+    b = torch.where(torch.rand(T, generator=g) < 0.5, torch.zeros_like(b), b)
+    inside = (b >= 0) & (b < bins)
+    want, size = (torch.zeros(bins, heads, dtype=torch.float64).index_add(0, b[inside], x[inside].double()) for x in (v, v.abs()))
+    got = H.bin_sum(v.to(dev), b.to(dev), bins)
+    assert got.shape == (bins, heads) and bool(((got.cpu().double() - want).abs() <= (T / 64 + 200) * R.U * size).all())
+    wide = torch.zeros(T, heads + 3, device=dev)
+    wide[:, 1:1 + heads] = v.to(dev)
+    assert torch.equal(got, H.bin_sum(wide[:, 1:1 + heads], b.to(dev), bins))
+
+
+def test_attention_layer_with_more_relations_than_bins(H, G, dev):
+    """300 relations: the gradient of the relation biases is that of the same entries' biases, summed"""
+    layer = G.GraphAttentionLayer(8, 8, 2, num_relations=300, device=dev)
+    few = G.GraphAttentionLayer(8, 8, 2, num_relations=5, device=dev)
+    graph = sampled(G, dev, 100, 900, [5], True, True, 20, 2)
+    graph.performMap()
+    x = torch.randn(graph.node_ids_.numel(), 8, generator=torch.Generator().manual_seed(0)).to(dev)
+    with torch.no_grad():
+        for a, b in ((few.wq, layer.wq), (few.wo, layer.wo), (few.wkv, layer.wkv)):
+            a.copy_(b)
+    outs = [m(x, graph) for m in (layer, few)]
+    assert torch.equal(*outs)
+    for o in outs:
+        o.square().sum().backward()
+    a, b = layer.relation_bias.grad, few.relation_bias.grad
+    assert float((a[[0, 1, 2, 3, 4, 300]] - b).abs().max()) <= 400 * R.U * float(b.abs().max()) + 1e-7 and not bool(a[5:300].any())
