@@ -411,7 +411,8 @@ class _TableRows(torch.autograd.Function):
     def forward(ctx, table, rows):
         ctx.save_for_backward(rows)
         ctx.bins = table.size(0)
-        return table.index_select(0, rows)
+        with torch.cuda.device(table.device if table.is_cuda else -1):
+            return H.gather_rows(table.contiguous(), rows)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -470,7 +471,7 @@ class GraphAttentionLayer(torch.nn.Module):
         bias = None
         if self.relation_bias is not None:
             relations = dense_graph.entryRelations(self.relation_bias.size(0) - 1)
-            few = self.relation_bias.size(0) <= H.MAX_BINS and self.heads <= 1024  # (more rows: an embedding's gradient, summed over sorted entries)
+            few = self.relation_bias.size(0) <= H.MAX_BINS and self.relation_bias.dtype == torch.float32  # (more rows: an embedding's gradient, over sorted entries)
             bias = _TableRows.apply(self.relation_bias, relations) if few else torch.nn.functional.embedding(relations, self.relation_bias)
         out = neighbor_attention(q, kv[:, 0], kv[:, 1], plan, None, bias)
         return torch.matmul(out.view(n, self.heads * self.dim), self.wo.t())

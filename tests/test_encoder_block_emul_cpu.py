@@ -274,6 +274,7 @@ def test_emulated_layer_with_many_relations(HE):
     from marius_amd import gnn
 
     T.test_attention_layer_with_more_relations_than_bins(HE, gnn, CPU)
+    T.test_attention_layer_in_bfloat16(HE, gnn, CPU)
 
 
 def test_bin_sum_refuses(HE):

@@ -717,3 +717,19 @@ def test_attention_layer_with_more_relations_than_bins(H, G, dev):
         o.square().sum().backward()
     a, b = layer.relation_bias.grad, few.relation_bias.grad
     assert float((a[[0, 1, 2, 3, 4, 300]] - b).abs().max()) <= 400 * R.U * float(b.abs().max()) + 1e-7 and not bool(a[5:300].any())
+
+
+def test_attention_layer_in_bfloat16(H, G, dev):
+    """a layer whose weights are bfloat16 takes bfloat16 rows, but its relation biases have to stay float32: refused, not read as if they were"""
+    graph = sampled(G, dev, 100, 900, [5], True, True, 20, 2)
+    graph.performMap()
+    x = torch.randn(graph.node_ids_.numel(), 8, device=dev).bfloat16()
+    plain = G.GraphAttentionLayer(8, 8, 2, device=dev).bfloat16()
+    assert plain(x, graph).dtype == BF16
+    layer = G.GraphAttentionLayer(8, 8, 2, num_relations=5, device=dev).bfloat16()
+    with pytest.raises(H.MariusHipError, match="bias is float32"):
+        layer(x, graph)
+    layer.relation_bias.data = layer.relation_bias.data.float()
+    out = layer(x, graph)
+    out.float().square().sum().backward()
+    assert out.dtype == BF16 and layer.relation_bias.grad.dtype == F32 and bool(layer.wq.grad.isfinite().all())
