@@ -467,13 +467,13 @@ class GraphAttentionLayer(torch.nn.Module):
         plan = dense_graph.neighborPlan()
         n = plan.n
         q = torch.matmul(inputs.narrow(0, inputs.size(0) - n, n), self.wq.t()).view(n, self.heads, self.dim)
-        kv = torch.matmul(inputs, self.wkv.t()).view(inputs.size(0), 2, self.kv_heads, self.dim)
+        k, v = torch.matmul(inputs, self.wkv.t()).view(inputs.size(0), 2, self.kv_heads, self.dim).unbind(1)
         bias = None
         if self.relation_bias is not None:
             relations = dense_graph.entryRelations(self.relation_bias.size(0) - 1)
             few = self.relation_bias.size(0) <= H.MAX_BINS and self.relation_bias.dtype == torch.float32  # (more rows: an embedding's gradient, over sorted entries)
             bias = _TableRows.apply(self.relation_bias, relations) if few else torch.nn.functional.embedding(relations, self.relation_bias)
-        out = neighbor_attention(q, kv[:, 0], kv[:, 1], plan, None, bias)
+        out = neighbor_attention(q, k, v, plan, None, bias)
         return torch.matmul(out.view(n, self.heads * self.dim), self.wo.t())
 
 
