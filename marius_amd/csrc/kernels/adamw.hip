@@ -7,8 +7,8 @@
 // by), e4m3 times its scale: e4m3 reaches 2^18 down from a block's largest value, which for the root is 2^36 of v.  A root above zero never becomes zero (it
 // stays at the type's smallest value): a weight whose gradients are tiny beside its block's would otherwise be divided by eps alone.  scale = largest / 448,
 // the type's largest value; a block whose largest magnitude is below 2^-100 is zero (its reciprocal would leave fp32).  The step itself uses the new
-// moments before they are rounded.  All of it is single fp32 operations in the order written (no contraction): the same bits from any other
-// program that does them in this order.
+// moments before they are rounded.  All of it is single fp32 operations in the order written (no contraction): moments, codes and scales have the
+// bits of any other program that does them in this order; the parameter's quotient is a product with a reciprocal within a step of fp32.
 //
 // Bound by HBM: 28 bytes an element with fp32 states, 16.1 with 8-bit ones (fp32 parameters and gradients).  A workgroup takes tiles of 2048 elements, eight
 // per lane (16-byte loads of every stream; the 32 lanes of a block share its scale by shuffles), and finds its tensor by binary search: up to 64 tensors in
