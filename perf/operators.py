@@ -125,11 +125,11 @@ def _prepare_attention(c, g, dev):
 def _run_attention_own(s):
     from marius_amd import hip
 
-    out, stats = hip.neighbor_attention(s["q"], s["k"], s["v"], s["plan"], bias=s["bias"])
+    out, lse = hip.neighbor_attention(s["q"], s["k"], s["v"], s["plan"], bias=s["bias"])
     if s["c"]["way"] == "forward":
-        return {"out": out, "stats": stats}
-    dq, dk, dv, dbias = hip.neighbor_attention_backward(s["grad"], s["q"], s["k"], s["v"], stats, s["plan"], bias=s["bias"])
-    return {"out": out, "stats": stats, "dq": dq, "dk": dk, "dv": dv, "dbias": dbias}
+        return {"out": out, "lse": lse}
+    dq, dk, dv, dbias = hip.neighbor_attention_backward(s["grad"], s["q"], s["k"], s["v"], lse, s["plan"], bias=s["bias"])
+    return {"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv, "dbias": dbias}
 
 
 def _run_attention_plain(s):
@@ -147,9 +147,9 @@ def _run_attention_plain(s):
     total = torch.zeros(n, K, R, device=dev).index_add_(0, owner, p)
     safe = torch.where(total > 0, total, 1.0)
     out = torch.zeros(n, K, R, D, device=dev).index_add_(0, owner, p.unsqueeze(-1) * v[index]) / safe.unsqueeze(-1)
-    stats = torch.stack([top.view(n, H), torch.log(safe).view(n, H)], -1)    # a row's largest score and the log of its sum
+    lse = (top + torch.log(safe)).view(n, H)
     if c["way"] == "forward":
-        return {"out": out.view(n, H, D).to(t), "stats": stats}
+        return {"out": out.view(n, H, D).to(t), "lse": lse}
     g = s["grad"].float().view(n, K, R, D)
     p = p / safe[owner]
     dp = (g[owner] * v[index]).sum(-1)
@@ -157,7 +157,7 @@ def _run_attention_plain(s):
     dq = torch.zeros(n, K, R, D, device=dev).index_add_(0, owner, ds.unsqueeze(-1) * k[index]) * scale
     dk = torch.zeros(c["rows"], K, D, device=dev).index_add_(0, index, (ds.unsqueeze(-1) * q[owner]).sum(2)) * scale
     dv = torch.zeros(c["rows"], K, D, device=dev).index_add_(0, index, (p.unsqueeze(-1) * g[owner]).sum(2))
-    return {"out": out.view(n, H, D).to(t), "stats": stats, "dq": dq.view(n, H, D).to(t), "dk": dk.to(t), "dv": dv.to(t), "dbias": ds.view(E, H) if c["bias"] else None}
+    return {"out": out.view(n, H, D).to(t), "lse": lse, "dq": dq.view(n, H, D).to(t), "dk": dk.to(t), "dv": dv.to(t), "dbias": ds.view(E, H) if c["bias"] else None}
 
 
 def _exact_attention(s):
@@ -167,7 +167,7 @@ def _exact_attention(s):
     q, k, v = (s[x].double().requires_grad_(True) for x in ("q", "k", "v"))
     bias = None if s["bias"] is None else s["bias"].double().requires_grad_(True)
     owner = torch.searchsorted(s["offsets"], torch.arange(E, device=q.device), right=True) - 1
-    outs, stats = [], []
+    outs, lses = [], []
     for h in range(H):
         score = torch.einsum("ed,ed->e", q[:, h].index_select(0, owner), k[:, h // R].index_select(0, s["index"])) / math.sqrt(D)
         if bias is not None:
@@ -180,23 +180,23 @@ def _exact_attention(s):
         total = torch.zeros(n, dtype=torch.float64, device=q.device).index_add(0, owner, w)
         num = torch.zeros(n, D, dtype=torch.float64, device=q.device).index_add(0, owner, w.unsqueeze(1) * v[:, h // R].index_select(0, s["index"]))
         outs.append(num / torch.where(dead, 1.0, total).unsqueeze(1))
-        stats.append(torch.stack([torch.where(dead, -math.inf, top), torch.log(torch.where(dead, 1.0, total.detach()))], -1))
-    out, stats = torch.stack(outs, 1), torch.stack(stats, 1)
+        lses.append(torch.where(dead, -math.inf, top + torch.log(torch.where(dead, 1.0, total.detach()))))
+    out, lse = torch.stack(outs, 1), torch.stack(lses, 1)
     if c["way"] == "forward":
-        return {"out": out.detach(), "stats": stats}
+        return {"out": out.detach(), "lse": lse}
     out.backward(s["grad"].double())
-    return {"out": out.detach(), "stats": stats, "dq": q.grad, "dk": k.grad, "dv": v.grad, "dbias": None if bias is None else bias.grad}
+    return {"out": out.detach(), "lse": lse, "dq": q.grad, "dk": k.grad, "dv": v.grad, "dbias": None if bias is None else bias.grad}
 
 
 def _work_attention(c):
     n, E, H, K, D, b = c["n"], c["edges"], c["heads"], c["kv_heads"], c["dim"], BYTES[c["type"]]
     read = c["rows"] * (1.0 - math.exp(-E / c["rows"]))          # rows that any list names
     lists = 4 * E + 4 * n + (4 * E * H if c["bias"] else 0)
-    forward = {"bytes": b * (2 * n * H * D + 2 * read * K * D) + 8 * n * H + lists, "flops": 4.0 * E * H * D}
+    forward = {"bytes": b * (2 * n * H * D + 2 * read * K * D) + 4 * n * H + lists, "flops": 4.0 * E * H * D}
     if c["way"] == "forward":
         return forward
     # the backward pass reads q, k, v, the gradient and the statistics, recomputes the scores and writes dq, dk, dv (and the bias' gradient)
-    backward = {"bytes": b * (3 * n * H * D + 2 * read * K * D + 2 * c["rows"] * K * D) + 8 * n * H + lists + (4 * E * H if c["bias"] else 0), "flops": 10.0 * E * H * D}
+    backward = {"bytes": b * (3 * n * H * D + 2 * read * K * D + 2 * c["rows"] * K * D) + 4 * n * H + lists + (4 * E * H if c["bias"] else 0), "flops": 10.0 * E * H * D}
     return {x: forward[x] + backward[x] for x in forward}
 
 
