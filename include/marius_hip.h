@@ -49,10 +49,10 @@ enum {
  * marius_table_absmax_counted; marius_lp_layout lost the operand planes of the removed bf16x6 kernels and the stream-K partials; 8:
  * marius_lp_desc.upd_*, marius_segment_update.fused_below, marius_lp_fuses_endpoint_update, marius_segment_plan_occ_single; 9: the
  * fixed-capacity exchange entry points marius_a2a_capacity / marius_a2a_rows_post / marius_a2a_rows_wait, negative ids = padding slots in
- * marius_merge_unique_runs / marius_segment_plan; 10: marius_a2a_publish / marius_a2a_record_* / marius_owner_offsets_counts, marius_layer_post_hook*, marius_prepare_maps; 11: marius_lp_layout.flash_cfg, marius_prepare_maps_preferred, the neighbour-sampling / GraphSage entry points marius_nbr_* and marius_segment_gather_sum; 12: marius_residual_norm_*, marius_nbr_plan_* / marius_neighbor_attention_*, marius_bin_sum, marius_adamw_step).  Every binder
+ * marius_merge_unique_runs / marius_segment_plan; 10: marius_a2a_publish / marius_a2a_record_* / marius_owner_offsets_counts, marius_layer_post_hook*, marius_prepare_maps; 11: marius_lp_layout.flash_cfg, marius_prepare_maps_preferred, the neighbour-sampling / GraphSage entry points marius_nbr_* and marius_segment_gather_sum; 12: marius_residual_norm_*, marius_nbr_plan_* / marius_neighbor_attention_*, marius_bin_sum, marius_adamw_step; 13: marius_neighbor_attention.lse).  Every binder
  * compares the value it was built against with what the loaded library returns and refuses to run on a mismatch: marius_amd/hip.py lib(),
  * the host module's init (bindings.cpp), and the plug-in recipe of INTEGRATION.md. */
-#define MARIUS_HIP_ABI_VERSION 12
+#define MARIUS_HIP_ABI_VERSION 13
 int marius_hip_abi_version(void);
 /* The MARIUS_* environment switches of the kernel library (test / A-B selectors; a production run sets none) are read ONCE, when the
  * library is loaded.  A process that changes one afterwards (the parity tests do, to reach a non-default kernel) calls this to re-read them. */
@@ -628,6 +628,8 @@ typedef struct marius_neighbor_plan {
  * at most 4 GiB apart).
  * bias [T, heads] fp32 or NULL, in the plan's entry order; -inf masks an entry: its key and value are not used.  A list without a live entry gives o = 0.
  * stats [n, heads, 2] fp32, written by the forward and read by the backward pass: largest score (-inf: none) and the log of the sum of exp(score - largest).
+ * lse (NULL: not wanted): their sum, the log-sum-exp of a list's scores (-inf: none), which is not enough for the backward pass: next to scores of the type's lowest value the
+ * log is lost in it.
  * Forward: out [n, heads, dim].  Backward: dq [n, heads, dim], dk / dv [rows, kv_heads, dim] (contiguous; rows that no list names get zero), dbias [T, heads] or NULL.
  * No atomics: the same bits on every run.  Workspace: marius_neighbor_attention_workspace_bytes. */
 typedef struct marius_neighbor_attention {
@@ -638,6 +640,7 @@ typedef struct marius_neighbor_attention {
     int64_t q_row, q_head, k_row, k_head, v_row, v_head;
     const float* bias;
     float* stats;
+    float* lse; /* forward: [n, heads] or NULL */
 } marius_neighbor_attention;
 size_t marius_neighbor_attention_workspace_bytes(const marius_neighbor_plan* plan, int32_t heads, int32_t kv_heads, int32_t dim, int32_t backward);
 int marius_neighbor_attention_forward(const marius_neighbor_plan* plan, const marius_neighbor_attention* desc, void* out, void* workspace, size_t workspace_bytes,

@@ -252,17 +252,20 @@ void attention_call(AttentionCall& c, uintptr_t plan, const Tensor& plan_index, 
         m.bias = (const float*)c.bias.data_ptr();
     }
 }
-std::pair<Tensor, Tensor> neighbor_attention(uintptr_t entry, uintptr_t workspace_entry, uintptr_t plan, const Tensor& plan_index, const Tensor& q, const Tensor& k, const Tensor& v,
-                                             std::optional<double> scale, const MaybeTensor& bias) {
+std::tuple<Tensor, Tensor, MaybeTensor> neighbor_attention(uintptr_t entry, uintptr_t workspace_entry, uintptr_t plan, const Tensor& plan_index, const Tensor& q, const Tensor& k,
+                                                           const Tensor& v, std::optional<double> scale, const MaybeTensor& bias, bool return_lse) {
     AttentionCall c;
     attention_call(c, plan, plan_index, q, k, v, scale, bias);
     const c10::OptionalDeviceGuard guard(q.device());
     Tensor out = at::empty(q.sizes(), q.options()), stats = at::empty({q.size(0), q.size(1), 2}, q.options().dtype(at::kFloat));
     c.m.stats = (float*)stats.data_ptr();
+    MaybeTensor lse;
+    if (return_lse) lse = at::empty({q.size(0), q.size(1)}, stats.options());
+    c.m.lse = (float*)data(lse);
     const size_t need = ((decltype(&marius_neighbor_attention_workspace_bytes))workspace_entry)(c.plan, c.m.heads, c.m.kv_heads, c.m.dim, 0);
     const Tensor ws = need ? bytes(need, q) : Tensor();
     check(((decltype(&marius_neighbor_attention_forward))entry)(c.plan, &c.m, out.data_ptr(), need ? ws.data_ptr() : nullptr, need, stream_of(q.device())), "neighbor_attention");
-    return {out, stats};
+    return {out, stats, lse};
 }
 std::tuple<Tensor, Tensor, Tensor, MaybeTensor> neighbor_attention_backward(uintptr_t entry, uintptr_t workspace_entry, uintptr_t plan, const Tensor& plan_index, const Tensor& grad_out,
                                                                             const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& stats, std::optional<double> scale,

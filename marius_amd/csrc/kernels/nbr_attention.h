@@ -15,7 +15,7 @@ struct NaArgs {
     int64_t q_hd, k_hd, v_hd, go_hd;                            // head strides, bytes
     uint32_t q_ld, k_ld, v_ld, go_ld;                           // row strides, bytes (an address is one multiply-add of 32 bits by 32 on 64)
     const float* bias;                                          // [T, H] or NULL
-    float *out_bias, *stats, *part;
+    float *out_bias, *stats, *lse, *part;                       // lse: [n, H] or NULL (m + log l of a list, for the caller; the sweeps use `stats`)
     float2* part2;                                              // a part's (m, sum), or its delta
     float4* rowstats;                                           // [n, H]: m, log l, delta of a target's list, for the sweep over the rows' lists
     void *out, *dk, *dv;                                        // contiguous [n, H, D], [rows, Hkv, D]
@@ -125,6 +125,14 @@ template <int UN>
 __device__ __forceinline__ void load_biases(const NaArgs& A, int t, int end, int h, float (&b)[UN]) {
 #pragma unroll
     for (int u = 0; u < UN; ++u) b[u] = t + u < end ? A.bias[(uint64_t)(uint32_t)(t + u) * (uint32_t)A.H + h] : -NA_INF;
+}
+
+// a list's statistics, from its largest score and its sum
+__device__ __forceinline__ void store_stats(const NaArgs& A, int64_t o, float m, float sum) {
+    const float logl = sum == 0.f ? 0.f : logf(sum);
+    A.stats[o * 2] = m;
+    A.stats[o * 2 + 1] = logl;
+    if (A.lse) A.lse[o] = m + logl;
 }
 
 // p from a score and its list's (m, log l); a list without a live entry has m = -inf

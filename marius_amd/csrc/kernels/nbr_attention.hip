@@ -96,10 +96,7 @@ __global__ __launch_bounds__(64 * NA_WAVES) void nbr_attention_kernel(NaArgs A) 
         for (int e = 0; e < VEC; ++e) acc[e] *= inv;
         const int64_t o = (int64_t)it.x * A.H + w.h;
         part.store((T*)A.out + o * A.D, acc);
-        if (w.l == 0) {
-            A.stats[o * 2] = m;
-            A.stats[o * 2 + 1] = sum == 0.f ? 0.f : logf(sum);
-        }
+        if (w.l == 0) store_stats(A, o, m, sum);
     }
 }
 
@@ -156,10 +153,7 @@ __global__ __launch_bounds__(64 * NA_JOIN) void nbr_attention_join_kernel(NaArgs
     for (int e = 0; e < VEC; ++e) acc[e] *= inv;
     const int64_t o = (int64_t)sp.x * A.H + w.h;
     part.store((T*)A.out + o * A.D, acc);
-    if (w.l == 0) {
-        A.stats[o * 2] = m;
-        A.stats[o * 2 + 1] = sum == 0.f ? 0.f : logf(sum);
-    }
+    if (w.l == 0) store_stats(A, o, m, sum);
 }
 struct ForwardPass {
     static constexpr bool ROWS = false;
@@ -234,6 +228,7 @@ extern "C" int marius_neighbor_attention_forward(const marius_neighbor_plan* P, 
     MARIUS_REQUIRE(P->n_slots == 0 || (workspace && P->splits && workspace_bytes >= marius_neighbor_attention_workspace_bytes(P, m->heads, m->kv_heads, m->dim, 0)),
                    "neighbor_attention_forward: workspace too small");
     A.out = out;
+    A.lse = m->lse;
     A.part2 = (float2*)workspace;
     A.part = (float*)((char*)workspace + na_small_bytes(P, A.H));
     na_launch_typed<ForwardPass>(A, m->type, as_stream(stream));

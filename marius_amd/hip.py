@@ -18,7 +18,7 @@ REDUCE_SUM, REDUCE_MEAN = 0, 1
 LOSS = {"SOFTMAX_CE": 0, "RANKING": 1, "CROSS_ENTROPY": 2, "BCE_AFTER_SIGMOID": 3, "BCE_WITH_LOGITS": 4, "MSE": 5, "SOFTPLUS": 6}
 LP_TRAIN_ONLY, LP_STORE_SCORES, LP_KEEP_DADJ = 1, 2, 4   # marius_lp_desc.flags
 MT_STATE_WORDS = 625
-ABI_VERSION = 12  # include/marius_hip.h MARIUS_HIP_ABI_VERSION
+ABI_VERSION = 13  # include/marius_hip.h MARIUS_HIP_ABI_VERSION
 
 
 class MariusHipError(RuntimeError):
@@ -77,7 +77,7 @@ class NeighborPlanDesc(C.Structure):  # marius_neighbor_plan
 
 class NeighborAttention(C.Structure):  # marius_neighbor_attention
     _fields_ = [("heads", _i32), ("kv_heads", _i32), ("dim", _i32), ("type", _i32), ("scale", _f32), ("reserved_", _i32), ("q", _vp), ("k", _vp), ("v", _vp), ("q_row", _i64),
-                ("q_head", _i64), ("k_row", _i64), ("k_head", _i64), ("v_row", _i64), ("v_head", _i64), ("bias", _vp), ("stats", _vp)]
+                ("q_head", _i64), ("k_row", _i64), ("k_head", _i64), ("v_row", _i64), ("v_head", _i64), ("bias", _vp), ("stats", _vp), ("lse", _vp)]
 
 
 class AdamWTensor(C.Structure):  # marius_adamw_tensor
@@ -855,13 +855,16 @@ def _plan(plan):
     return plan
 
 
-def neighbor_attention(q, k, v, plan, scale=None, bias=None):
+def neighbor_attention(q, k, v, plan, scale=None, bias=None, return_lse=False):
     """(out [n, heads, dim], stats [n, heads, 2]): every target's softmax attention over its list in `plan`.  q [n, heads, dim], k and v [rows, kv_heads, dim] of
     one type (float32, bfloat16, float16), any strides with contiguous heads; query heads share key heads where there are fewer.  scale: dim ** -0.5 unless
     given.  bias [entries, heads] float32 is added to the scores, -inf masks an entry.  A list without a live entry gives zeros.  stats (a list's largest score, the
-    log of its sum) is what the backward pass needs; their sum is the log-sum-exp."""
+    log of its sum) is what the backward pass needs; their sum is the log-sum-exp, [n, heads], returned as a third result where `return_lse` (-inf for a list without a
+    live entry)."""
     _dev(q)
-    return _ops().neighbor_attention(_entry("marius_neighbor_attention_forward"), _entry("marius_neighbor_attention_workspace_bytes"), _plan(plan).address, plan.index, q, k, v, scale, bias)
+    out, stats, lse = _ops().neighbor_attention(_entry("marius_neighbor_attention_forward"), _entry("marius_neighbor_attention_workspace_bytes"), _plan(plan).address, plan.index, q, k, v,
+                                                scale, bias, return_lse)
+    return (out, stats, lse) if return_lse else (out, stats)
 
 
 def neighbor_attention_backward(grad_out, q, k, v, stats, plan, scale=None, bias=None, need_dbias=True):
