@@ -125,10 +125,10 @@ def _prepare_attention(c, g, dev):
 def _run_attention_own(s):
     from marius_amd import hip
 
-    out, lse = hip.neighbor_attention(s["q"], s["k"], s["v"], s["plan"], bias=s["bias"])
+    out, stats, lse = hip.neighbor_attention(s["q"], s["k"], s["v"], s["plan"], bias=s["bias"], return_lse=True)
     if s["c"]["way"] == "forward":
         return {"out": out, "lse": lse}
-    dq, dk, dv, dbias = hip.neighbor_attention_backward(s["grad"], s["q"], s["k"], s["v"], lse, s["plan"], bias=s["bias"])
+    dq, dk, dv, dbias = hip.neighbor_attention_backward(s["grad"], s["q"], s["k"], s["v"], stats, s["plan"], bias=s["bias"])
     return {"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv, "dbias": dbias}
 
 
