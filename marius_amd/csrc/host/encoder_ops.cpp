@@ -87,9 +87,9 @@ void norm_call(NormCall& c, const Tensor& x, const MaybeTensor& block, const May
     require(m.kind >= 0, "residual_norm: kind is one of RMS, LAYER");
     m.gate_activation = activation == "NONE" ? MARIUS_ACT_NONE : activation == "RELU" ? MARIUS_ACT_RELU : activation == "SIGMOID" ? MARIUS_ACT_SIGMOID : -1;
     require(m.gate_activation >= 0, "Unsupported activation function");
-    require(n == 0 || (d >= 1 && d <= 8192), "residual_norm: rows of 1 to 8192 elements, got ", d);
+    require((d >= 1 || n == 0) && d <= 8192, "residual_norm: rows of 1 to 8192 elements, got ", d);
     require(eps >= 0, "residual_norm: eps must not be negative");
-    m.d = (int32_t)std::min<int64_t>(d, 8192);
+    m.d = (int32_t)d;
     m.stream_type = m.type = type_of("stream", x);
     m.has_block = block.has_value();
     if (block) {
