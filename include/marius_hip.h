@@ -601,7 +601,7 @@ int marius_residual_norm_backward(const marius_residual_norm* desc, const marius
  *   entry), keys [T] (the rows once more, for marius_sort_unique), status [4] (ZEROED by the caller): bit 0: offsets that do not ascend from 0 and cover
  *   their list, bit 1: a row outside [0, rows).  A caller reads status before it goes on: the calls below and the attention take the lists as they are.
  * marius_nbr_plan_reverse: the entries grouped by row, in list order: r_offsets [rows + 1], r_owner [T]; perm of marius_sort_unique = r_entry.
- *   (The attention reads index, r_owner and r_entry four entries at a time: allocate four more than T; what they hold does not matter.)
+ *   (The attention reads index, r_owner and r_entry four entries at a time, for an empty list too: allocate four more than T, also where T is 0; what they hold does not matter.)
  * marius_nbr_plan_items: lists cut into work items of at most `chunk` entries: items {list, first, end, slot or -1} (at most n + T / chunk; the longest first),
  *   splits {list, first slot, parts, 0} of the lists that were cut (at most T / chunk), totals [3] = items, slots, splits.  Workspace:
  *   marius_nbr_plan_items_workspace_bytes, at a multiple of 16 bytes. */

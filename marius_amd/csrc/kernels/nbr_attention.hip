@@ -173,12 +173,15 @@ static size_t na_small_bytes(const marius_neighbor_plan* P, int heads) { return 
 
 static int na_args(const marius_neighbor_plan* P, const marius_neighbor_attention* m, const char* what, NaArgs& A) {
     MARIUS_REQUIRE(P && m, "%s: null descriptor", what);
-    MARIUS_REQUIRE(P->n >= 0 && P->rows >= 0 && P->T >= 0 && P->n_items >= 0 && P->n_splits >= 0 && P->r_n_items >= 0 && P->r_n_splits >= 0, "%s: bad plan", what);
+    MARIUS_REQUIRE(P->n >= 0 && P->rows >= 0 && P->T >= 0 && P->n_items >= P->n && P->n_splits >= 0 && P->n_slots >= 0 && P->r_n_items >= 0 && P->r_n_splits >= 0 && P->r_n_slots >= 0,
+                   "%s: bad plan", what);  // (a list without a work item would not be written)
     MARIUS_REQUIRE(float_type_ok(m->type), "%s: types are MARIUS_F32 / BF16 / F16", what);
     MARIUS_REQUIRE(m->heads > 0 && m->kv_heads > 0 && m->heads % m->kv_heads == 0 && m->heads <= 1024, "%s: query heads (up to 1024) are a multiple of the key heads", what);
     MARIUS_REQUIRE(m->dim > 0 && m->dim <= 256, "%s: heads of 1 to 256 elements", what);
-    MARIUS_REQUIRE(P->n == 0 || (m->q && P->items), "%s: null pointer", what);
-    MARIUS_REQUIRE(P->T == 0 || (m->k && m->v && P->index), "%s: null pointer", what);
+    MARIUS_REQUIRE(P->n == 0 || m->q, "%s: null pointer", what);
+    MARIUS_REQUIRE(P->T == 0 || (m->k && m->v), "%s: null pointer", what);
+    MARIUS_REQUIRE(P->n_items == 0 || (P->items && P->index), "%s: null pointer", what);  // (an item of no entries reads numbers ahead as well)
+    MARIUS_REQUIRE(P->n_splits == 0 || P->splits, "%s: null pointer", what);
     const int64_t size = m->type == MARIUS_F32 ? 4 : 2;
     for (int64_t row : {m->q_row, m->k_row, m->v_row})
         MARIUS_REQUIRE(row >= 0 && row * size < (1ll << 32), "%s: rows are at most 4 GiB apart", what);
@@ -225,7 +228,7 @@ extern "C" int marius_neighbor_attention_forward(const marius_neighbor_plan* P, 
     if (rc) return rc;
     if (P->n == 0) return MARIUS_OK;
     MARIUS_REQUIRE(out && m->stats, "neighbor_attention_forward: null output");
-    MARIUS_REQUIRE(P->n_slots == 0 || (workspace && P->splits && workspace_bytes >= marius_neighbor_attention_workspace_bytes(P, m->heads, m->kv_heads, m->dim, 0)),
+    MARIUS_REQUIRE(P->n_slots == 0 || (workspace && workspace_bytes >= marius_neighbor_attention_workspace_bytes(P, m->heads, m->kv_heads, m->dim, 0)),
                    "neighbor_attention_forward: workspace too small");
     A.out = out;
     A.lse = m->lse;
@@ -241,8 +244,10 @@ extern "C" int marius_neighbor_attention_backward(const marius_neighbor_plan* P,
     const int rc = na_args(P, m, "neighbor_attention_backward", A);
     if (rc) return rc;
     MARIUS_REQUIRE(P->n == 0 || (grad_out && dq && m->stats), "neighbor_attention_backward: null pointer");
-    MARIUS_REQUIRE(P->rows == 0 || (m->k && m->v && dk && dv && P->r_items), "neighbor_attention_backward: null pointer");
-    MARIUS_REQUIRE(P->T == 0 || (P->r_owner && P->r_entry), "neighbor_attention_backward: null pointer");
+    MARIUS_REQUIRE(P->rows == 0 || (m->k && m->v && dk && dv), "neighbor_attention_backward: null pointer");
+    MARIUS_REQUIRE(P->r_n_items >= P->rows, "neighbor_attention_backward: bad plan");
+    MARIUS_REQUIRE(P->r_n_items == 0 || (P->r_items && P->r_owner && (P->r_entry || !m->bias)), "neighbor_attention_backward: null pointer");
+    MARIUS_REQUIRE(P->r_n_splits == 0 || P->r_splits, "neighbor_attention_backward: null pointer");
     MARIUS_REQUIRE(!dbias || m->bias, "neighbor_attention_backward: the gradient of a bias that is not there");
     const size_t need = marius_neighbor_attention_workspace_bytes(P, m->heads, m->kv_heads, m->dim, 1);
     MARIUS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "neighbor_attention_backward: workspace too small");

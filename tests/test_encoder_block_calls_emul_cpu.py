@@ -1,4 +1,5 @@
 """tests/test_gpu_encoder_block_calls.py on the CPU build of its kernel files (tests/emul), and what is refused there."""
+import ctypes as C
 import os
 import sys
 
@@ -30,3 +31,27 @@ def test_residual_norm_refuses_wide_rows_even_where_there_are_none(HE):
     got = HE.residual_norm_backward(*(torch.zeros(0, 8192) for _ in range(4)), *(torch.ones(8192) for _ in range(5)), post_norm=True)
     assert all(not got[k].any() for k in ("dgate", "dpost_weight", "dpost_bias", "dpre_weight", "dpre_bias"))
     assert HE.residual_norm(torch.zeros(0, 0))[1].shape == (0, 0)
+
+
+def test_neighbor_attention_c_abi_refuses_plans_without_their_arrays(HE):
+    """the kernels read numbers of every work item, an empty list's too, and a list is written by its item: what a plan says that it has has to be there"""
+    L, P = HE.lib(), HE.ptr
+    q, k, out, stats, ws = torch.ones(2, 1, 4), torch.ones(3, 1, 4), torch.zeros(2, 1, 4), torch.zeros(2, 1, 2), torch.zeros(4096)
+    dk, dv, bias = torch.zeros(3, 1, 4), torch.zeros(3, 1, 4), torch.zeros(1)
+    plan = HE.NeighborPlan(torch.zeros(0, dtype=torch.int64), torch.zeros(2, dtype=torch.int64), 3)
+    assert plan.desc.n_items == 2 and plan.desc.r_n_items == 3 and plan.num_entries == 0
+
+    def calls(**change):
+        d = HE.NeighborPlanDesc.from_buffer_copy(plan.desc)
+        for name, value in change.items():
+            setattr(d, name, value)
+        m = HE.NeighborAttention(heads=1, kv_heads=1, dim=4, scale=1.0, q=q.data_ptr(), k=k.data_ptr(), v=k.data_ptr(), q_row=4, k_row=4, v_row=4, stats=stats.data_ptr())
+        forward = L.marius_neighbor_attention_forward(C.byref(d), C.byref(m), P(out), P(ws), 16384, None)
+        m.bias = bias.data_ptr()
+        return forward, L.marius_neighbor_attention_backward(C.byref(d), C.byref(m), P(q), 4, 4, P(out), P(dk), P(dv), None, P(ws), 16384, None)
+
+    assert calls() == (0, 0)
+    assert calls(index=None) == (1, 1) and calls(items=None) == (1, 1)
+    assert calls(n_items=1) == (1, 1) and calls(n_splits=1, n_slots=2, splits=None) == (1, 1)      # fewer items than lists; a cut list without its parts
+    for change in (dict(r_owner=None), dict(r_entry=None), dict(r_items=None), dict(r_n_items=2), dict(r_n_splits=1, r_n_slots=2, r_splits=None)):
+        assert calls(**change) == (0, 1), change
