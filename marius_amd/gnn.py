@@ -107,7 +107,9 @@ class DENSEGraph:
         return self.plan_relations_[1]
 
     def neighborPlan(self):
-        """the attention's plan of this layer's lists (outgoing, incoming neighbours, the target's own row), made once between two prepareForNextLayer calls"""
+        """the attention's plan of this layer's lists (outgoing, incoming neighbours, the target's own row) once they are mapped, made once between two prepareForNextLayer calls"""
+        if self.unmapped():
+            raise H.MariusHipError("the graph's lists are not mapped yet: performMap comes before neighborPlan")
         if self.plan_ is None:
             lists = [(m.contiguous(), o.contiguous()) for m, o in ((self.out_neighbors_mapping_, self.out_offsets_), (self.in_neighbors_mapping_, self.in_offsets_)) if m is not None]
             first = self.getLayerOffset()
@@ -117,8 +119,14 @@ class DENSEGraph:
             self.plan_ = H.NeighborPlan(*lists[0], rows, *(lists[1] if len(lists) > 1 else (None, None)), self_offset=first)
         return self.plan_
 
+    def unmapped(self):
+        """sampled lists that performMap has not seen yet"""
+        return self.src_sorted_edges_ is None or len(self.in_neighbors_vec_) + len(self.out_neighbors_vec_) > 0
+
     def performMap(self):
         """graph.cpp:361-398"""
+        if self.unmapped():
+            self.plan_ = self.plan_relations_ = None
         dev = self.node_ids_.device
         n = self.node_ids_.numel()
         first = True
@@ -490,7 +498,8 @@ class GraphAttentionEncoder(torch.nn.Module):
         self.norms = torch.nn.ModuleList([ResidualNorm(dim, post_norm=post_norm, kind=kind, gate=gate, residual_scale=residual_scale, device=device) for _ in range(layers)])
 
     def forward(self, features, dense_graph, train=True):
-        dense_graph.performMap()
+        if dense_graph.unmapped():
+            dense_graph.performMap()
         x, h = self.first(torch.matmul(features, self.project.t()))
         for i, (layer, norm) in enumerate(zip(self.layers, self.norms)):
             block = layer(h, dense_graph, train)

@@ -55,3 +55,15 @@ def test_neighbor_attention_c_abi_refuses_plans_without_their_arrays(HE):
     assert calls(n_items=1) == (1, 1) and calls(n_splits=1, n_slots=2, splits=None) == (1, 1)      # fewer items than lists; a cut list without its parts
     for change in (dict(r_owner=None), dict(r_entry=None), dict(r_items=None), dict(r_n_items=2), dict(r_n_splits=1, r_n_slots=2, r_splits=None)):
         assert calls(**change) == (0, 1), change
+
+
+# ------------------------------------------------------------------------------------------------ graphs and encoders
+@pytest.fixture()
+def G(HE):
+    from marius_amd import gnn
+
+    return gnn
+
+
+def test_emulated_plans_are_of_mapped_lists(HE, G):
+    T.test_plans_are_of_mapped_lists(HE, G, CPU)

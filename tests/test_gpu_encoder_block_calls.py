@@ -30,3 +30,26 @@ def test_log_sum_exp_beside_the_output(H, dev, masked, heads, kv, dim, kind):
     value, mag = R.attention(q, k, v, rows, owner, dim ** -0.5, None if bias is None else bias.cpu())["stats"]
     R.close(lse, value.sum(-1), mag.sum(-1), 1, "lse")
     assert bool((lse[1] == -math.inf).all()) and (masked != 6 or bool((lse == -math.inf).all()))
+
+
+# ------------------------------------------------------------------------------------------------ graphs
+def test_plans_are_of_mapped_lists(H, G, dev):
+    """a graph whose lists are not mapped yet has no plan (it would leave every target alone with itself); mapping new lists drops the plan of the old ones, mapping again what is
+    mapped keeps it: an encoder takes a graph that its caller has mapped, and takes it twice"""
+    make = lambda: T.sampled(G, dev, 100, 900, [5], True, True, 20, 2)  # noqa: E731
+    graph, other = make(), T.sampled(G, dev, 100, 900, [9], True, True, 20, 7)
+    for call in (graph.neighborPlan, lambda: graph.entryRelations(5)):
+        with pytest.raises(H.MariusHipError, match="performMap"):
+            call()
+    graph.performMap()
+    plan, edges = graph.neighborPlan(), graph.src_sorted_edges_.size(0) + graph.dst_sorted_edges_.size(0)
+    assert plan.num_entries == edges + 20 and edges > 100 and graph.neighborPlan() is plan
+    enc = G.GraphAttentionEncoder(8, 16, 3, 1, 4, num_relations=5, device=dev)
+    features = torch.randn(100, 8, generator=torch.Generator().manual_seed(1)).to(dev)
+    want = enc(features[: make().node_ids_.numel()], make())
+    for mapped in (graph, graph):
+        assert torch.equal(enc(features[: graph.node_ids_.numel()], mapped), want)
+    graph.hop_offsets_, graph.node_ids_, graph.graph_ = other.hop_offsets_, other.node_ids_, other.graph_
+    graph.in_offsets_, graph.out_offsets_, graph.in_neighbors_vec_, graph.out_neighbors_vec_ = other.in_offsets_, other.out_offsets_, other.in_neighbors_vec_, other.out_neighbors_vec_
+    graph.performMap()
+    assert graph.neighborPlan() is not plan and graph.neighborPlan().num_entries == graph.src_sorted_edges_.size(0) + graph.dst_sorted_edges_.size(0) + 20
