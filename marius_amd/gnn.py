@@ -88,13 +88,17 @@ class DENSEGraph:
         self.in_num_neighbors_ = self.out_num_neighbors_ = None
         self.plan_ = self.plan_relations_ = None
 
+    def liveLists(self):
+        """(mapping, offsets, edges) of the layer's directions that have entries: prepareForNextLayer leaves the offsets of one that has none as they were"""
+        both = (self.out_neighbors_mapping_, self.out_offsets_, self.src_sorted_edges_), (self.in_neighbors_mapping_, self.in_offsets_, self.dst_sorted_edges_)
+        return [(m, o, e) for m, o, e in both if m is not None and m.numel() > 0]
+
     def entryRelations(self, num_relations):
         """the relation of every entry of the layer's plan, in its order; num_relations for a target's own row.  Made, and checked, once for a plan"""
         plan = self.neighborPlan()
         if self.plan_relations_ is None or self.plan_relations_[0] != num_relations:
             relation = torch.full((plan.num_entries,), -1, **_i64(plan.device))
-            edges = [e for m, e in ((self.out_neighbors_mapping_, self.src_sorted_edges_), (self.in_neighbors_mapping_, self.dst_sorted_edges_)) if m is not None]
-            for part, e in enumerate(edges):
+            for part, (_, _, e) in enumerate(self.liveLists()):
                 if e.size(1) != 3:
                     raise H.MariusHipError("relation biases need edges of three columns")
                 relation[plan.places(part)] = e.select(1, 1)
@@ -111,10 +115,10 @@ class DENSEGraph:
         if self.unmapped():
             raise H.MariusHipError("the graph's lists are not mapped yet: performMap comes before neighborPlan")
         if self.plan_ is None:
-            lists = [(m.contiguous(), o.contiguous()) for m, o in ((self.out_neighbors_mapping_, self.out_offsets_), (self.in_neighbors_mapping_, self.in_offsets_)) if m is not None]
+            lists = [(m.contiguous(), o.contiguous()) for m, o, _ in self.liveLists()]
             first = self.getLayerOffset()
             rows = self.node_ids_.numel()
-            if not lists:  # (a graph without sampled neighbours: every target attends to itself)
+            if not lists:  # (no sampled neighbours: every target attends to itself)
                 lists = [(torch.zeros(0, **_i64(self.node_ids_.device)), torch.zeros(rows - first, **_i64(self.node_ids_.device)))]
             self.plan_ = H.NeighborPlan(*lists[0], rows, *(lists[1] if len(lists) > 1 else (None, None)), self_offset=first)
         return self.plan_

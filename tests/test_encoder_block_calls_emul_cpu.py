@@ -67,3 +67,9 @@ def G(HE):
 
 def test_emulated_plans_are_of_mapped_lists(HE, G):
     T.test_plans_are_of_mapped_lists(HE, G, CPU)
+
+
+@pytest.mark.parametrize("out_edges", [[[2, 1, 3]], []])
+@pytest.mark.parametrize("in_edges", [[[3, 0, 2], [2, 4, 1], [1, 2, 0]], [[3, 3, 2]], []])
+def test_emulated_encoder_over_layers_whose_lists_run_out(HE, G, in_edges, out_edges):
+    T.test_encoder_over_layers_whose_lists_run_out(HE, G, CPU, in_edges, out_edges)

@@ -53,3 +53,33 @@ def test_plans_are_of_mapped_lists(H, G, dev):
     graph.in_offsets_, graph.out_offsets_, graph.in_neighbors_vec_, graph.out_neighbors_vec_ = other.in_offsets_, other.out_offsets_, other.in_neighbors_vec_, other.out_neighbors_vec_
     graph.performMap()
     assert graph.neighborPlan() is not plan and graph.neighborPlan().num_entries == graph.src_sorted_edges_.size(0) + graph.dst_sorted_edges_.size(0) + 20
+
+
+@pytest.mark.parametrize("out_edges", [[[2, 1, 3]], []])
+@pytest.mark.parametrize("in_edges", [[[3, 0, 2], [2, 4, 1], [1, 2, 0]], [[3, 3, 2]], []])
+def test_encoder_over_layers_whose_lists_run_out(H, G, dev, in_edges, out_edges):
+    """a chain 3 -> 2 -> 1 -> 0 whose later layers have no neighbours in one direction or in both (dropout sampling leaves such graphs): a target without any has itself.
+    Bound as for the other encoder steps: 4000 roundings of fp32 at a tensor's largest entry."""
+    i64 = lambda v, shape=(-1,): torch.tensor(v, dtype=torch.int64).reshape(shape).to(dev)  # noqa: E731
+
+    def make():
+        ends = lambda edges, col: [0, *(sum(e[col] >= t for e in edges) for t in (2, 1))]  # noqa: E731  (lists of the targets 2, 1, 0)
+        vec = lambda edges: [i64(edges, (-1, 3))] if edges else []  # noqa: E731
+        base = i64([[0, 0, 1]], (1, 3))
+        return G.DENSEGraph(torch.tensor([0, 1, 2, 3, 4]).to(dev), i64([3, 2, 1, 0]), i64(ends(in_edges, 2)), vec(in_edges), i64(ends(out_edges, 0)), vec(out_edges), G.MariusGraph(base, base, 4))
+
+    torch.manual_seed(2)
+    enc = G.GraphAttentionEncoder(6, 16, 3, 3, 4, kv_heads=2, num_relations=5, residual_scale=0.9, device=dev)
+    with torch.no_grad():
+        for layer in enc.layers:
+            layer.relation_bias.copy_(torch.randn(6, 4, generator=torch.Generator().manual_seed(4)))
+    features = torch.randn(4, 6, generator=torch.Generator().manual_seed(3))
+    leaves = {n: p.detach().cpu().double().requires_grad_(True) for n, p in enc.named_parameters()}
+    want = T.encoder_reference(enc, features.double(), make(), leaves)
+    want.square().sum().backward()
+    got = enc(features.to(dev), make())
+    got.square().sum().backward()
+    assert got.shape == (1, 3) and float((got.detach().cpu().double() - want.detach()).abs().max()) <= 4000 * R.U * float(want.abs().max())
+    for n, p in enc.named_parameters():
+        g = leaves[n].grad
+        assert float((p.grad.cpu().double() - g).abs().max()) <= 4000 * R.U * float(g.abs().max()) + 1e-12, n
