@@ -346,17 +346,24 @@ struct AdamWTensors {
         for (size_t i = 1; i < spans.size(); ++i) require(spans[i - 1].second <= spans[i].first, "AdamWTensors: a tensor appears twice, or overlaps another");
     }
 };
-// `entry`: marius_adamw_step; `step`: an int or an int64 device tensor
-void adamw_step(uintptr_t entry, uintptr_t workspace_entry, AdamWTensors& a, const std::vector<MaybeTensor>& grads, const py::object& step, double lr, double beta1, double beta2, double eps,
-                double weight_decay, const MaybeTensor& grad_scale, bool capturing) {
+// A step's arguments, checked; nothing is launched and nothing changes until they are used.  `step`: an int or an int64 device tensor
+struct AdamWCall {
+    std::vector<marius_adamw_tensor> table;
+    std::vector<size_t> strided;  // gradients that are not contiguous
+    MaybeTensor counter;
+    int64_t step = 0;
+    int grad_type = -1;           // -1: no gradient at all
+};
+AdamWCall adamw_call(uintptr_t check_entry, AdamWTensors& a, const std::vector<MaybeTensor>& grads, const py::object& step, double lr, double beta1, double beta2, double eps,
+                     double weight_decay, const MaybeTensor& grad_scale, bool capturing) {
     const size_t count = a.params.size();
     require(grads.size() == count, "adamw_step: ", grads.size(), " gradients for ", count, " parameters");
     const at::Device device = a.states[0][0].device();
-    std::vector<marius_adamw_tensor> table(a.table);  // (a copy: two threads may step at once)
-    std::vector<Tensor> copies;
+    AdamWCall c;
+    c.table = a.table;  // (a copy: two threads may step at once)
     std::optional<at::ScalarType> kind;
     for (size_t i = 0; i < count; ++i) {
-        marius_adamw_tensor& t = table[i];
+        marius_adamw_tensor& t = c.table[i];
         if (!grads[i]) {
             t.n = 0;
             continue;
@@ -369,27 +376,45 @@ void adamw_step(uintptr_t entry, uintptr_t workspace_entry, AdamWTensors& a, con
                 " is no longer what the states were made for");
         t.param = w.data_ptr();
         t.grad = g.data_ptr();
-        if (!g.is_contiguous()) {
-            copies.push_back(g.contiguous());
-            t.grad = copies.back().data_ptr();
-        }
+        if (!g.is_contiguous()) c.strided.push_back(i);
     }
     const bool on_device = THPVariable_Check(step.ptr());
-    MaybeTensor counter;
     if (on_device) {
-        counter = THPVariable_Unpack(step.ptr());
-        require(counter->scalar_type() == at::kLong && counter->numel() == 1 && counter->device() == device, "adamw_step: a step on the device is one int64 on ", device);
+        c.counter = THPVariable_Unpack(step.ptr());
+        require(c.counter->scalar_type() == at::kLong && c.counter->numel() == 1 && c.counter->device() == device, "adamw_step: a step on the device is one int64 on ", device);
+    } else {
+        c.step = step.cast<int64_t>();
     }
     require(!grad_scale || (grad_scale->scalar_type() == at::kFloat && grad_scale->numel() == 1 && grad_scale->device() == device), "adamw_step: grad_scale is one float32 on ", device);
     require(on_device || !capturing, "adamw_step: a captured step needs its number on the device (a replay would repeat this one's)");
-    if (!kind) return;
+    if (!kind) return c;
     require(*kind == at::kFloat || *kind == at::kBFloat16 || *kind == at::kHalf, "adamw_step: float32, bfloat16 or float16 gradients required, got ", *kind);
-    const int grad_type = *kind == at::kFloat ? MARIUS_F32 : *kind == at::kBFloat16 ? MARIUS_BF16 : MARIUS_F16;
+    c.grad_type = *kind == at::kFloat ? MARIUS_F32 : *kind == at::kBFloat16 ? MARIUS_BF16 : MARIUS_F16;
+    check(((decltype(&marius_adamw_check))check_entry)(c.table.data(), (int32_t)count, a.type, c.grad_type, a.bits, c.step, (const int64_t*)data(c.counter), lr, beta1, beta2, eps,
+                                                       weight_decay),
+          "adamw_step");
+    return c;
+}
+void adamw_check(uintptr_t check_entry, AdamWTensors& a, const std::vector<MaybeTensor>& grads, const py::object& step, double lr, double beta1, double beta2, double eps,
+                 double weight_decay, const MaybeTensor& grad_scale, bool capturing) {
+    adamw_call(check_entry, a, grads, step, lr, beta1, beta2, eps, weight_decay, grad_scale, capturing);
+}
+void adamw_step(uintptr_t check_entry, uintptr_t entry, uintptr_t workspace_entry, AdamWTensors& a, const std::vector<MaybeTensor>& grads, const py::object& step, double lr, double beta1,
+                double beta2, double eps, double weight_decay, const MaybeTensor& grad_scale, bool capturing) {
+    AdamWCall c = adamw_call(check_entry, a, grads, step, lr, beta1, beta2, eps, weight_decay, grad_scale, capturing);
+    if (c.grad_type < 0) return;
+    const size_t count = a.params.size();
+    const at::Device device = a.states[0][0].device();
     const c10::OptionalDeviceGuard guard(device);
+    std::vector<Tensor> copies;
+    for (size_t i : c.strided) {
+        copies.push_back(grads[i]->contiguous());
+        c.table[i].grad = copies.back().data_ptr();
+    }
     const size_t need = ((decltype(&marius_adamw_workspace_bytes))workspace_entry)((int32_t)count);
     const Tensor ws = need ? bytes(need, a.states[0][0]) : Tensor();
-    check(((decltype(&marius_adamw_step))entry)(table.data(), (int32_t)count, a.type, grad_type, a.bits, on_device ? 0 : step.cast<int64_t>(), (const int64_t*)data(counter), lr, beta1,
-                                                beta2, eps, weight_decay, (const float*)data(grad_scale), need ? ws.data_ptr() : nullptr, need, stream_of(device)),
+    check(((decltype(&marius_adamw_step))entry)(c.table.data(), (int32_t)count, a.type, c.grad_type, a.bits, c.step, (const int64_t*)data(c.counter), lr, beta1, beta2, eps, weight_decay,
+                                                (const float*)data(grad_scale), need ? ws.data_ptr() : nullptr, need, stream_of(device)),
           "adamw_step");
     for (size_t i = 0; i < count; ++i)  // a graph that saved the old values may not go back through the new ones
         if (grads[i] && !a.params[i].is_inference()) a.params[i].unsafeGetTensorImpl()->bump_version();
@@ -406,6 +431,7 @@ void bind_encoder_ops(py::module_& m) {
         .def(py::init<std::vector<Tensor>, std::vector<Tensor>, std::vector<Tensor>, std::optional<std::vector<Tensor>>, std::optional<std::vector<Tensor>>>())
         .def_property_readonly("device", [](const AdamWTensors& a) { return a.states[0][0].device(); })
         .def_readonly("params", &AdamWTensors::params);
+    m.def("adamw_check", &adamw_check);
     m.def("adamw_step", &adamw_step);
 }
 

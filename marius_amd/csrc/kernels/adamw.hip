@@ -230,17 +230,15 @@ using namespace marius;
 
 extern "C" size_t marius_adamw_workspace_bytes(int32_t count) { return count > AW_TENSORS ? (size_t)count * (sizeof(AwTensor) + sizeof(int)) : 0; }
 
-extern "C" int marius_adamw_step(const marius_adamw_tensor* tensors, int32_t count, int32_t param_type, int32_t grad_type, int32_t state_bits, int64_t step,
-                                 const int64_t* step_dev, double lr, double beta1, double beta2, double eps, double weight_decay, const float* grad_scale,
-                                 void* workspace, size_t workspace_bytes, marius_stream_t stream) {
+extern "C" int marius_adamw_check(const marius_adamw_tensor* tensors, int32_t count, int32_t param_type, int32_t grad_type, int32_t state_bits, int64_t step,
+                                  const int64_t* step_dev, double lr, double beta1, double beta2, double eps, double weight_decay) {
     MARIUS_REQUIRE(count >= 0 && (count == 0 || tensors), "adamw_step: bad tensor list");
     MARIUS_REQUIRE(float_type_ok(param_type) && float_type_ok(grad_type), "adamw_step: types are MARIUS_F32 / BF16 / F16");
     MARIUS_REQUIRE(state_bits == 32 || state_bits == 8, "adamw_step: states are held in 32 or in 8 bits");
     MARIUS_REQUIRE(step_dev || step >= 1, "adamw_step: steps are counted from 1");
     MARIUS_REQUIRE(lr >= 0 && beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0 && weight_decay >= 0, "adamw_step: lr, eps, weight_decay >= 0, betas in [0, 1)");
     int64_t tiles = 0;
-    int live = 0;
-    for (int k = 0; k < count; ++k) {  // before anything is launched: a refused list leaves every tensor as it was
+    for (int k = 0; k < count; ++k) {
         const marius_adamw_tensor& s = tensors[k];
         MARIUS_REQUIRE(s.n >= 0, "adamw_step: bad size of tensor %d", k);
         if (s.n == 0) continue;
@@ -248,8 +246,18 @@ extern "C" int marius_adamw_step(const marius_adamw_tensor* tensors, int32_t cou
         const int64_t more = cdiv(s.n, AW_TILE);
         MARIUS_REQUIRE(tiles + more < (1ll << 24), "adamw_step: over 2^35 elements in one call");  // (a launch holds less than 2^32 lanes)
         tiles += more;
-        ++live;
     }
+    return MARIUS_OK;
+}
+
+extern "C" int marius_adamw_step(const marius_adamw_tensor* tensors, int32_t count, int32_t param_type, int32_t grad_type, int32_t state_bits, int64_t step,
+                                 const int64_t* step_dev, double lr, double beta1, double beta2, double eps, double weight_decay, const float* grad_scale,
+                                 void* workspace, size_t workspace_bytes, marius_stream_t stream) {
+    // before anything is launched: a refused list leaves every tensor as it was
+    const int rc = marius_adamw_check(tensors, count, param_type, grad_type, state_bits, step, step_dev, lr, beta1, beta2, eps, weight_decay);
+    if (rc) return rc;
+    int live = 0;
+    for (int k = 0; k < count; ++k) live += tensors[k].n > 0;
     if (live == 0) return MARIUS_OK;
     const bool many = live > AW_TENSORS;
     MARIUS_REQUIRE(!many || (workspace && workspace_bytes >= marius_adamw_workspace_bytes(count)), "adamw_step: workspace too small");
@@ -273,7 +281,7 @@ extern "C" int marius_adamw_step(const marius_adamw_tensor* tensors, int32_t cou
     A.count = live;
     AwTable T{};
     int filled = 0, at = 0;
-    tiles = 0;
+    int64_t tiles = 0;
     for (int k = 0; k < count; ++k) {
         const marius_adamw_tensor& s = tensors[k];
         if (s.n == 0) continue;

@@ -150,6 +150,7 @@ SIGNATURES = {
     "marius_bin_sum_workspace_bytes": (_sz, [_i64, _i32, _i32]),
     "marius_bin_sum": (C.c_int, [_vp, _vp, _i64, _i32, _i32, _vp, _vp, _sz, _vp]),
     "marius_adamw_step": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i64, _vp, _f64, _f64, _f64, _f64, _f64, _vp, _vp, _sz, _vp]),
+    "marius_adamw_check": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i64, _vp, _f64, _f64, _f64, _f64, _f64]),
     "marius_adamw_workspace_bytes": (_sz, [_i32]),
     "marius_owner_offsets_counts": (C.c_int, [_vp, _vp, _i64, _i32, _vp, _vp, _vp]),
     "marius_a2a_record_words": (_i32, [_i32]),
@@ -913,8 +914,15 @@ def adamw_step(tensors, grads, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, 
     they are.  step counts from 1: a number, or an int64 device tensor of one element (a captured call has to take that: a replay reads it anew).  grad_scale: float32
     device tensor of one element every gradient is multiplied by (a clipping factor, the inverse of a loss scale)."""
     _require(isinstance(tensors, _ops().AdamWTensors), "adamw_step: AdamWTensors are needed")
-    _ops().adamw_step(_entry("marius_adamw_step"), _entry("marius_adamw_workspace_bytes"), tensors, grads, step, lr, beta1, beta2, eps, weight_decay, grad_scale,
-                      torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing())
+    _ops().adamw_step(_entry("marius_adamw_check"), _entry("marius_adamw_step"), _entry("marius_adamw_workspace_bytes"), tensors, grads, step, lr, beta1, beta2, eps, weight_decay,
+                      grad_scale, torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing())
+
+
+def adamw_check(tensors, grads, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2, grad_scale=None):
+    """refuses what adamw_step refuses of these arguments and does nothing else: for a step of several calls, none of which shall run if one is refused"""
+    _require(isinstance(tensors, _ops().AdamWTensors), "adamw_step: AdamWTensors are needed")
+    _ops().adamw_check(_entry("marius_adamw_check"), tensors, grads, step, lr, beta1, beta2, eps, weight_decay, grad_scale,
+                       torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing())
 
 
 def profile_enable(on=True, only=None):

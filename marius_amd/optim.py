@@ -35,17 +35,24 @@ class AdamW:
 
     @torch.no_grad()
     def step(self, grad_scale=None):
-        """one step; grad_scale: float32 device tensor of one element that multiplies every gradient (a clipping factor, the inverse of a loss scale)"""
-        if self.capturable:
-            for t in self._step_dev.values():
-                t.add_(1)
+        """one step; grad_scale: float32 device tensor of one element that multiplies every gradient (a clipping factor, the inverse of a loss scale).  A step that is
+        refused does not count and leaves every parameter and state as it was."""
+        calls = []
         for at, tensors in self._groups:
             grads = [self.params[i].grad for i in at]
             for kind in {g.dtype for g in grads if g is not None}:   # (one kind of gradient in every program we know of)
-                H.adamw_step(tensors, [g if g is not None and g.dtype == kind else None for g in grads], self._step_dev[tensors.device] if self.capturable else self.num_steps + 1,
-                             self.lr, *self.betas, self.eps, self.weight_decay, grad_scale)
+                calls.append((tensors, [g if g is not None and g.dtype == kind else None for g in grads], self._step_dev[tensors.device] if self.capturable else self.num_steps + 1,
+                              self.lr, *self.betas, self.eps, self.weight_decay, grad_scale))
+        if self.capturable or len(calls) > 1:  # (a single call checks itself before it launches)
+            for call in calls:
+                H.adamw_check(*call)
+        if self.capturable:
+            for t in self._step_dev.values():
+                t.add_(1)
+        for call in calls:
+            H.adamw_step(*call)
         if not self.capturable:
-            self.num_steps += 1  # (a refused step does not count)
+            self.num_steps += 1
 
     def state_dict(self):
         steps = int(next(iter(self._step_dev.values()))) if self.capturable else self.num_steps

@@ -73,3 +73,26 @@ def test_emulated_plans_are_of_mapped_lists(HE, G):
 @pytest.mark.parametrize("in_edges", [[[3, 0, 2], [2, 4, 1], [1, 2, 0]], [[3, 3, 2]], []])
 def test_emulated_encoder_over_layers_whose_lists_run_out(HE, G, in_edges, out_edges):
     T.test_encoder_over_layers_whose_lists_run_out(HE, G, CPU, in_edges, out_edges)
+
+
+# ------------------------------------------------------------------------------------------------ AdamW
+@pytest.mark.parametrize("capturable", [False, True])
+def test_emulated_refused_steps(HE, capturable):
+    for what in range(4):
+        T.test_a_refused_step_changes_nothing(HE, CPU, what, capturable)
+
+
+def test_adamw_check_refuses_and_does_nothing(HE):
+    p, m, v = (torch.ones(300) for _ in range(3))
+    t = HE.AdamWTensors([p], [m], [v])
+    refused(HE, "gradient 0 is not", HE.adamw_check, t, [torch.zeros(299)], 1)
+    refused(HE, "counted from 1", HE.adamw_check, t, [p], 0)
+    refused(HE, "AdamWTensors are needed", HE.adamw_check, [p], [p], 1)
+    HE.adamw_check(t, [torch.ones(300)], 1)
+    assert all(bool((x == 1).all()) for x in (p, m, v))
+    L, table = HE.lib(), HE.AdamWTensor(param=p.data_ptr(), grad=p.data_ptr(), exp_avg=m.data_ptr(), exp_avg_sq=v.data_ptr(), n=300)
+    call = lambda table, *a: L.marius_adamw_check(table, 1, 0, 0, 32, *a)  # noqa: E731
+    assert call(C.byref(table), 1, None, 1e-3, 0.9, 0.999, 1e-8, 0.0) == 0
+    for bad in ((0, None, 1e-3, 0.9, 0.999, 1e-8, 0.0), (1, None, float("nan"), 0.9, 0.999, 1e-8, 0.0), (1, None, 1e-3, 1.0, 0.999, 1e-8, 0.0), (1, None, 1e-3, 0.9, 0.999, -1.0, 0.0)):
+        assert call(C.byref(table), *bad) == 1, bad
+    assert call(None, 1, None, 1e-3, 0.9, 0.999, 1e-8, 0.0) == 1

@@ -83,3 +83,38 @@ def test_encoder_over_layers_whose_lists_run_out(H, G, dev, in_edges, out_edges)
     for n, p in enc.named_parameters():
         g = leaves[n].grad
         assert float((p.grad.cpu().double() - g).abs().max()) <= 4000 * R.U * float(g.abs().max()) + 1e-12, n
+
+
+# ------------------------------------------------------------------------------------------------ AdamW
+def refusals_of_a_step(dev):
+    """(what is wrong with it, parameters, what makes it wrong) of optimizer steps that are refused at their last call or argument"""
+    two = lambda: torch.ones(2, device=dev)  # noqa: E731
+    return [("one float32", [F32], lambda ps, opt: dict(grad_scale=two())),
+            ("not a dense tensor", [F32, BF16], lambda ps, opt: setattr(ps[1], "grad", ps[1].grad.to_sparse())),
+            ("betas in", [F32, F16], lambda ps, opt: setattr(opt, "betas", (0.9, 1.0))),
+            ("no longer what", [F32, BF16], lambda ps, opt: setattr(ps[1], "data", torch.ones(9, device=dev, dtype=BF16)))]
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("what", range(4))
+def test_a_refused_step_changes_nothing(H, dev, what, capturable):
+    """whichever of a step's calls is refused: no parameter, no state and no count is changed, and the step that follows is the first"""
+    from marius_amd.optim import AdamW
+
+    message, kinds, spoil = refusals_of_a_step(dev)[what]
+    ps = [torch.nn.Parameter(torch.ones(8, device=dev, dtype=kind)) for kind in kinds]
+    fresh = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    opt, other = AdamW(ps, capturable=capturable), AdamW(fresh, capturable=capturable)
+    for p in ps + fresh:
+        p.grad = torch.full_like(p, 0.5)
+    kept = [(p, p.detach().clone(), p.grad) for p in ps]
+    with pytest.raises(H.MariusHipError, match=message):
+        opt.step(**(spoil(ps, opt) or {}))
+    assert opt.state_dict()["num_steps"] == 0 and not any(bool(t.any()) for t in opt.exp_avg + opt.exp_avg_sq)
+    assert all(torch.equal(p, before) for p, before, _ in kept if p.numel() == 8)
+    opt.betas = (0.9, 0.999)
+    for p, before, g in kept:
+        p.data, p.grad = before, g
+    opt.step()
+    other.step()
+    assert all(torch.equal(a, b) for a, b in zip(ps, fresh)) and bool((ps[0] < 1).all())
