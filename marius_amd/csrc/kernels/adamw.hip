@@ -14,6 +14,8 @@
 // per lane (16-byte loads of every stream; the 32 lanes of a block share its scale by shuffles), and finds its tensor by binary search: up to 64 tensors in
 // the launch's own arguments, more in a table that short launches copy from theirs into the workspace of this call (300 tensors, 20 M elements in 8 bits: 56 us
 // against 86 with a launch for every 64 tensors, each of which fills and drains the card anew; 200 M elements in fp32: 1095 us, 5.1 TB/s).
+// With the step's number on the device one lane of a workgroup takes the two factors behind the loads: the times are those of a number on the host (in every lane, the 300
+// tensors in 8 bits took 7 us more).
 #include "row_types.h"
 
 namespace marius {
@@ -135,11 +137,6 @@ __device__ __forceinline__ void adamw_tile(const AwStep& A, const AwTensor& t, i
     const int64_t i = (int64_t)tile * AW_TILE + (int)threadIdx.x * AW_EPT;
     const int left = t.n - i >= AW_EPT ? AW_EPT : t.n > i ? (int)(t.n - i) : 0;
     float rate = A.rate, inv_root = A.inv_root;
-    if (A.step_dev) {
-        const double step = (double)*A.step_dev;
-        rate = (float)(A.lr / (1.0 - pow(A.beta1_d, step)));
-        inv_root = (float)(1.0 / sqrt(1.0 - pow(A.beta2_d, step)));
-    }
     const float gs = A.grad_scale ? *A.grad_scale : 1.f;
     float p[AW_EPT], g[AW_EPT], m[AW_EPT], v[AW_EPT], r[AW_EPT];
     aw_load<P>((const P*)t.p, i, left, p);
@@ -157,6 +154,17 @@ __device__ __forceinline__ void adamw_tile(const AwStep& A, const AwTensor& t, i
     } else {
         aw_load<float>((const float*)t.m, i, left, m);
         aw_load<float>((const float*)t.v, i, left, v);
+    }
+    if (A.step_dev) {  // (uniform) one lane takes the powers of 64 bits while the loads are under way
+        __shared__ float factors[2];
+        if (threadIdx.x == 0) {
+            const double step = (double)*A.step_dev;
+            factors[0] = (float)(A.lr / (1.0 - pow(A.beta1_d, step)));
+            factors[1] = (float)(1.0 / sqrt(1.0 - pow(A.beta2_d, step)));
+        }
+        __syncthreads();
+        rate = factors[0];
+        inv_root = factors[1];
     }
 #pragma unroll
     for (int e = 0; e < AW_EPT; ++e) {
