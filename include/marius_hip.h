@@ -49,7 +49,7 @@ enum {
  * marius_table_absmax_counted; marius_lp_layout lost the operand planes of the removed bf16x6 kernels and the stream-K partials; 8:
  * marius_lp_desc.upd_*, marius_segment_update.fused_below, marius_lp_fuses_endpoint_update, marius_segment_plan_occ_single; 9: the
  * fixed-capacity exchange entry points marius_a2a_capacity / marius_a2a_rows_post / marius_a2a_rows_wait, negative ids = padding slots in
- * marius_merge_unique_runs / marius_segment_plan; 10: marius_a2a_publish / marius_a2a_record_* / marius_owner_offsets_counts, marius_layer_post_hook*, marius_prepare_maps; 11: marius_lp_layout.flash_cfg, marius_prepare_maps_preferred, the neighbour-sampling / GraphSage entry points marius_nbr_* and marius_segment_gather_sum; 12: marius_residual_norm_*, marius_nbr_plan_* / marius_neighbor_attention_*, marius_bin_sum, marius_adamw_step; 13: marius_neighbor_attention.lse, marius_adamw_check).  Every binder
+ * marius_merge_unique_runs / marius_segment_plan; 10: marius_a2a_publish / marius_a2a_record_* / marius_owner_offsets_counts, marius_layer_post_hook*, marius_prepare_maps; 11: marius_lp_layout.flash_cfg, marius_prepare_maps_preferred, the neighbour-sampling / GraphSage entry points marius_nbr_* and marius_segment_gather_sum; 12: marius_residual_norm_*, marius_nbr_plan_* / marius_neighbor_attention_*, marius_bin_sum, marius_adamw_step; 13: marius_neighbor_attention.lse, marius_adamw_check, marius_adamw_step's step_count).  Every binder
  * compares the value it was built against with what the loaded library returns and refuses to run on a mismatch: marius_amd/hip.py lib(),
  * the host module's init (bindings.cpp), and the plug-in recipe of INTEGRATION.md. */
 #define MARIUS_HIP_ABI_VERSION 13
@@ -654,7 +654,7 @@ size_t marius_bin_sum_workspace_bytes(int64_t T, int32_t heads, int32_t bins);
 int marius_bin_sum(const float* values, const int64_t* bin, int64_t T, int32_t heads, int32_t bins, float* out, void* workspace, size_t workspace_bytes, marius_stream_t stream);
 
 /* AdamW over many tensors (adamw.hip): p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps), moments m and v updated first; t = step (from 1),
- * or *step_dev (a captured call replays with the step it finds there).  Every gradient is multiplied by *grad_scale (NULL: 1).  All tensors of a call have
+ * or, on the device, step_dev[0] for all tensors (step_count 1) or step_dev[k] for tensor k (step_count = count); a captured call replays with the steps it finds there.  Every gradient is multiplied by *grad_scale (NULL: 1).  All tensors of a call have
  * parameters of param_type and gradients of grad_type; more than 64 of them go through a table in `workspace` (marius_adamw_workspace_bytes(count) bytes, 0 up to 64).  state_bits 32: exp_avg / exp_avg_sq fp32 [n].  state_bits 8: e4m3 codes [n] and one
  * fp32 scale for every 256 elements [ceil(n / 256)]; exp_avg_sq then holds the ROOT of the second moment (value = code * scale in both), and a root above zero stays
  * above zero. */
@@ -668,9 +668,9 @@ typedef struct marius_adamw_tensor {
 size_t marius_adamw_workspace_bytes(int32_t count);
 /* refuses what marius_adamw_step refuses of these arguments and launches nothing: for a caller whose step takes several calls, of which none shall run if one is refused */
 int marius_adamw_check(const marius_adamw_tensor* tensors, int32_t count, int32_t param_type, int32_t grad_type, int32_t state_bits, int64_t step, const int64_t* step_dev,
-                       double lr, double beta1, double beta2, double eps, double weight_decay);
+                       int32_t step_count, double lr, double beta1, double beta2, double eps, double weight_decay);
 int marius_adamw_step(const marius_adamw_tensor* tensors, int32_t count, int32_t param_type, int32_t grad_type, int32_t state_bits, int64_t step, const int64_t* step_dev,
-                      double lr, double beta1, double beta2, double eps, double weight_decay, const float* grad_scale, void* workspace, size_t workspace_bytes,
+                      int32_t step_count, double lr, double beta1, double beta2, double eps, double weight_decay, const float* grad_scale, void* workspace, size_t workspace_bytes,
                       marius_stream_t stream);
 
 #ifdef __cplusplus

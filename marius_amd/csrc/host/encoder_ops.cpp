@@ -346,13 +346,14 @@ struct AdamWTensors {
         for (size_t i = 1; i < spans.size(); ++i) require(spans[i - 1].second <= spans[i].first, "AdamWTensors: a tensor appears twice, or overlaps another");
     }
 };
-// A step's arguments, checked; nothing is launched and nothing changes until they are used.  `step`: an int or an int64 device tensor
+// A step's arguments, checked; nothing is launched and nothing changes until they are used.  `step`: an int or an int64 device tensor (of one number, or one for each parameter)
 struct AdamWCall {
     std::vector<marius_adamw_tensor> table;
     std::vector<size_t> strided;  // gradients that are not contiguous
     MaybeTensor counter;
     int64_t step = 0;
     int grad_type = -1;           // -1: no gradient at all
+    int32_t steps() const { return counter ? (int32_t)counter->numel() : 1; }
 };
 AdamWCall adamw_call(uintptr_t check_entry, AdamWTensors& a, const std::vector<MaybeTensor>& grads, const py::object& step, double lr, double beta1, double beta2, double eps,
                      double weight_decay, const MaybeTensor& grad_scale, bool capturing) {
@@ -381,7 +382,8 @@ AdamWCall adamw_call(uintptr_t check_entry, AdamWTensors& a, const std::vector<M
     const bool on_device = THPVariable_Check(step.ptr());
     if (on_device) {
         c.counter = THPVariable_Unpack(step.ptr());
-        require(c.counter->scalar_type() == at::kLong && c.counter->numel() == 1 && c.counter->device() == device, "adamw_step: a step on the device is one int64 on ", device);
+        require(c.counter->scalar_type() == at::kLong && (c.counter->numel() == 1 || c.counter->numel() == (int64_t)count) && c.counter->is_contiguous() && c.counter->device() == device,
+                "adamw_step: a step on the device is one int64, or one for each parameter, on ", device);
     } else {
         c.step = step.cast<int64_t>();
     }
@@ -390,8 +392,8 @@ AdamWCall adamw_call(uintptr_t check_entry, AdamWTensors& a, const std::vector<M
     if (!kind) return c;
     require(*kind == at::kFloat || *kind == at::kBFloat16 || *kind == at::kHalf, "adamw_step: float32, bfloat16 or float16 gradients required, got ", *kind);
     c.grad_type = *kind == at::kFloat ? MARIUS_F32 : *kind == at::kBFloat16 ? MARIUS_BF16 : MARIUS_F16;
-    check(((decltype(&marius_adamw_check))check_entry)(c.table.data(), (int32_t)count, a.type, c.grad_type, a.bits, c.step, (const int64_t*)data(c.counter), lr, beta1, beta2, eps,
-                                                       weight_decay),
+    check(((decltype(&marius_adamw_check))check_entry)(c.table.data(), (int32_t)count, a.type, c.grad_type, a.bits, c.step, (const int64_t*)data(c.counter), c.steps(), lr,
+                                                       beta1, beta2, eps, weight_decay),
           "adamw_step");
     return c;
 }
@@ -413,8 +415,8 @@ void adamw_step(uintptr_t check_entry, uintptr_t entry, uintptr_t workspace_entr
     }
     const size_t need = ((decltype(&marius_adamw_workspace_bytes))workspace_entry)((int32_t)count);
     const Tensor ws = need ? bytes(need, a.states[0][0]) : Tensor();
-    check(((decltype(&marius_adamw_step))entry)(c.table.data(), (int32_t)count, a.type, c.grad_type, a.bits, c.step, (const int64_t*)data(c.counter), lr, beta1, beta2, eps, weight_decay,
-                                                (const float*)data(grad_scale), need ? ws.data_ptr() : nullptr, need, stream_of(device)),
+    check(((decltype(&marius_adamw_step))entry)(c.table.data(), (int32_t)count, a.type, c.grad_type, a.bits, c.step, (const int64_t*)data(c.counter), c.steps(), lr, beta1, beta2, eps,
+                                                weight_decay, (const float*)data(grad_scale), need ? ws.data_ptr() : nullptr, need, stream_of(device)),
           "adamw_step");
     for (size_t i = 0; i < count; ++i)  // a graph that saved the old values may not go back through the new ones
         if (grads[i] && !a.params[i].is_inference()) a.params[i].unsafeGetTensorImpl()->bump_version();

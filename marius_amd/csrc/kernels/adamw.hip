@@ -31,23 +31,25 @@ struct AwTensor {
 };
 struct AwTable {
     AwTensor t[AW_TENSORS];
-    int first[AW_TENSORS];  // first tile of every tensor
+    int first[AW_TENSORS];        // first tile of every tensor
+    uint16_t number[AW_TENSORS];  // its number in the caller's list, behind the part's first
 };
 struct AwStep {
-    int count;
+    int count, steps;           // steps: 0, one number for all tensors on the device; 1, one for each
     float decay, rate, beta1, omb1, beta2, omb2, inv_root, eps;
     const float* grad_scale;
-    const int64_t* step_dev;    // the step's number on the device: rate and inv_root are taken from it
+    const int64_t* step_dev;    // the steps' numbers on the device: rate and inv_root are taken from them
     double lr, beta1_d, beta2_d;
 };
 static_assert(sizeof(AwTable) + sizeof(AwStep) <= 4096, "kernel arguments");
 
 // a part of the table, from the launch's arguments to memory: tensors [at, at + count)
-__global__ __launch_bounds__(64) void adamw_table_kernel(AwTable P, int count, int at, AwTensor* __restrict__ t, int* __restrict__ first) {
+__global__ __launch_bounds__(64) void adamw_table_kernel(AwTable P, int count, int at, int base, AwTensor* __restrict__ t, int* __restrict__ first, int* __restrict__ number) {
     const int i = threadIdx.x;
     if (i >= count) return;
     t[at + i] = P.t[i];
     first[at + i] = P.first[i];
+    number[at + i] = base + P.number[i];
 }
 
 template <typename X>
@@ -132,7 +134,7 @@ __device__ __forceinline__ int aw_find(const int* first, int count, int tile) {
     return lo;
 }
 template <typename P, typename G, bool BITS8>
-__device__ __forceinline__ void adamw_tile(const AwStep& A, const AwTensor& t, int tile) {
+__device__ __forceinline__ void adamw_tile(const AwStep& A, const AwTensor& t, int tile, int number) {
 #pragma clang fp contract(off)
     const int64_t i = (int64_t)tile * AW_TILE + (int)threadIdx.x * AW_EPT;
     const int left = t.n - i >= AW_EPT ? AW_EPT : t.n > i ? (int)(t.n - i) : 0;
@@ -158,7 +160,7 @@ __device__ __forceinline__ void adamw_tile(const AwStep& A, const AwTensor& t, i
     if (A.step_dev) {  // (uniform) one lane takes the powers of 64 bits while the loads are under way
         __shared__ float factors[2];
         if (threadIdx.x == 0) {
-            const double step = (double)*A.step_dev;
+            const double step = (double)A.step_dev[A.steps ? number : 0];
             factors[0] = (float)(A.lr / (1.0 - pow(A.beta1_d, step)));
             factors[1] = (float)(1.0 / sqrt(1.0 - pow(A.beta2_d, step)));
         }
@@ -201,19 +203,19 @@ __device__ __forceinline__ void adamw_tile(const AwStep& A, const AwTensor& t, i
 template <typename P, typename G, bool BITS8>
 __global__ __launch_bounds__(AW_T) void adamw_kernel(AwTable P_, AwStep A) {
     const int k = aw_find(P_.first, A.count, (int)blockIdx.x);
-    adamw_tile<P, G, BITS8>(A, P_.t[k], (int)blockIdx.x - P_.first[k]);
+    adamw_tile<P, G, BITS8>(A, P_.t[k], (int)blockIdx.x - P_.first[k], P_.number[k]);
 }
 template <typename P, typename G, bool BITS8>
-__global__ __launch_bounds__(AW_T) void adamw_many_kernel(const AwTensor* __restrict__ t, const int* __restrict__ first, AwStep A) {
+__global__ __launch_bounds__(AW_T) void adamw_many_kernel(const AwTensor* __restrict__ t, const int* __restrict__ first, const int* __restrict__ number, AwStep A) {
     const int k = aw_find(first, A.count, (int)blockIdx.x);
-    adamw_tile<P, G, BITS8>(A, t[k], (int)blockIdx.x - first[k]);
+    adamw_tile<P, G, BITS8>(A, t[k], (int)blockIdx.x - first[k], number[k]);
 }
 
-// one launch over the tensors of `table` (up to 64), or over those of the table in memory
+// one launch over the tensors of `table` (up to 64), or over those of the table in memory: t, then first, then number
 template <typename P, typename G, bool BITS8>
 static void launch_adamw(const AwTable* table, const AwTensor* t, const int* first, const AwStep& A, unsigned tiles, hipStream_t st) {
     if (table) adamw_kernel<P, G, BITS8><<<dim3(tiles), dim3(AW_T), 0, st>>>(*table, A);
-    else adamw_many_kernel<P, G, BITS8><<<dim3(tiles), dim3(AW_T), 0, st>>>(t, first, A);
+    else adamw_many_kernel<P, G, BITS8><<<dim3(tiles), dim3(AW_T), 0, st>>>(t, first, first + A.count, A);
 }
 template <typename P, typename G>
 static void launch_adamw_bits(bool bits8, const AwTable* table, const AwTensor* t, const int* first, const AwStep& A, unsigned tiles, hipStream_t st) {
@@ -236,14 +238,15 @@ static void launch_adamw_typed(int param_type, int grad_type, bool bits8, const 
 
 using namespace marius;
 
-extern "C" size_t marius_adamw_workspace_bytes(int32_t count) { return count > AW_TENSORS ? (size_t)count * (sizeof(AwTensor) + sizeof(int)) : 0; }
+extern "C" size_t marius_adamw_workspace_bytes(int32_t count) { return count > AW_TENSORS ? (size_t)count * (sizeof(AwTensor) + 2 * sizeof(int)) : 0; }
 
 extern "C" int marius_adamw_check(const marius_adamw_tensor* tensors, int32_t count, int32_t param_type, int32_t grad_type, int32_t state_bits, int64_t step,
-                                  const int64_t* step_dev, double lr, double beta1, double beta2, double eps, double weight_decay) {
+                                  const int64_t* step_dev, int32_t step_count, double lr, double beta1, double beta2, double eps, double weight_decay) {
     MARIUS_REQUIRE(count >= 0 && (count == 0 || tensors), "adamw_step: bad tensor list");
     MARIUS_REQUIRE(float_type_ok(param_type) && float_type_ok(grad_type), "adamw_step: types are MARIUS_F32 / BF16 / F16");
     MARIUS_REQUIRE(state_bits == 32 || state_bits == 8, "adamw_step: states are held in 32 or in 8 bits");
     MARIUS_REQUIRE(step_dev || step >= 1, "adamw_step: steps are counted from 1");
+    MARIUS_REQUIRE(!step_dev || step_count == 1 || step_count == count, "adamw_step: one step on the device, or one for each tensor");
     MARIUS_REQUIRE(lr >= 0 && beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0 && weight_decay >= 0, "adamw_step: lr, eps, weight_decay >= 0, betas in [0, 1)");
     int64_t tiles = 0;
     for (int k = 0; k < count; ++k) {
@@ -259,15 +262,19 @@ extern "C" int marius_adamw_check(const marius_adamw_tensor* tensors, int32_t co
 }
 
 extern "C" int marius_adamw_step(const marius_adamw_tensor* tensors, int32_t count, int32_t param_type, int32_t grad_type, int32_t state_bits, int64_t step,
-                                 const int64_t* step_dev, double lr, double beta1, double beta2, double eps, double weight_decay, const float* grad_scale,
+                                 const int64_t* step_dev, int32_t step_count, double lr, double beta1, double beta2, double eps, double weight_decay, const float* grad_scale,
                                  void* workspace, size_t workspace_bytes, marius_stream_t stream) {
     // before anything is launched: a refused list leaves every tensor as it was
-    const int rc = marius_adamw_check(tensors, count, param_type, grad_type, state_bits, step, step_dev, lr, beta1, beta2, eps, weight_decay);
+    const int rc = marius_adamw_check(tensors, count, param_type, grad_type, state_bits, step, step_dev, step_count, lr, beta1, beta2, eps, weight_decay);
     if (rc) return rc;
-    int live = 0;
-    for (int k = 0; k < count; ++k) live += tensors[k].n > 0;
+    int live = 0, last = 0;
+    for (int k = 0; k < count; ++k)
+        if (tensors[k].n > 0) {
+            ++live;
+            last = k;
+        }
     if (live == 0) return MARIUS_OK;
-    const bool many = live > AW_TENSORS;
+    const bool many = live > AW_TENSORS || last > UINT16_MAX;
     MARIUS_REQUIRE(!many || (workspace && workspace_bytes >= marius_adamw_workspace_bytes(count)), "adamw_step: workspace too small");
     hipStream_t st = as_stream(stream);
     AwTensor* t_dev = (AwTensor*)workspace;
@@ -283,25 +290,30 @@ extern "C" int marius_adamw_step(const marius_adamw_tensor* tensors, int32_t cou
     A.eps = (float)eps;
     A.grad_scale = grad_scale;
     A.step_dev = step_dev;
+    A.steps = step_count > 1;
     A.lr = lr;
     A.beta1_d = beta1;
     A.beta2_d = beta2;
     A.count = live;
     AwTable T{};
-    int filled = 0, at = 0;
+    int filled = 0, at = 0, base = 0;
     int64_t tiles = 0;
+    auto send = [&] {
+        adamw_table_kernel<<<dim3(1), dim3(64), 0, st>>>(T, filled, at, base, t_dev, first_dev, first_dev + live);
+        at += filled;
+        filled = 0;
+    };
     for (int k = 0; k < count; ++k) {
         const marius_adamw_tensor& s = tensors[k];
         if (s.n == 0) continue;
+        if (many && filled > 0 && (filled == AW_TENSORS || k - base > UINT16_MAX)) send();
+        if (many && filled == 0) base = k;
+        T.number[filled] = (uint16_t)(k - base);
         T.t[filled] = AwTensor{s.param, s.grad, s.exp_avg, s.exp_avg_sq, s.exp_avg_scale, s.exp_avg_sq_scale, s.n};
         T.first[filled++] = (int)tiles;
         tiles += cdiv(s.n, AW_TILE);
-        if (many && (filled == AW_TENSORS || at + filled == live)) {
-            adamw_table_kernel<<<dim3(1), dim3(64), 0, st>>>(T, filled, at, t_dev, first_dev);
-            at += filled;
-            filled = 0;
-        }
     }
+    if (many) send();
     launch_adamw_typed(param_type, grad_type, state_bits == 8, many ? nullptr : &T, t_dev, first_dev, A, (unsigned)tiles, st);
     return check_launch("adamw_step");
 }

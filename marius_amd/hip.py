@@ -149,8 +149,8 @@ SIGNATURES = {
     "marius_neighbor_attention_backward": (C.c_int, [C.POINTER(NeighborPlanDesc), C.POINTER(NeighborAttention), _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "marius_bin_sum_workspace_bytes": (_sz, [_i64, _i32, _i32]),
     "marius_bin_sum": (C.c_int, [_vp, _vp, _i64, _i32, _i32, _vp, _vp, _sz, _vp]),
-    "marius_adamw_step": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i64, _vp, _f64, _f64, _f64, _f64, _f64, _vp, _vp, _sz, _vp]),
-    "marius_adamw_check": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i64, _vp, _f64, _f64, _f64, _f64, _f64]),
+    "marius_adamw_step": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i64, _vp, _i32, _f64, _f64, _f64, _f64, _f64, _vp, _vp, _sz, _vp]),
+    "marius_adamw_check": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i64, _vp, _i32, _f64, _f64, _f64, _f64, _f64]),
     "marius_adamw_workspace_bytes": (_sz, [_i32]),
     "marius_owner_offsets_counts": (C.c_int, [_vp, _vp, _i64, _i32, _vp, _vp, _vp]),
     "marius_a2a_record_words": (_i32, [_i32]),
@@ -911,7 +911,8 @@ def AdamWTensors(params, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_avg_sq_
 
 def adamw_step(tensors, grads, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2, grad_scale=None):
     """One AdamW step over all tensors of an AdamWTensors (marius_adamw_step), in place.  grads: one per parameter, of one type; None leaves its parameter and states as
-    they are.  step counts from 1: a number, or an int64 device tensor of one element (a captured call has to take that: a replay reads it anew).  grad_scale: float32
+    they are.  step counts from 1: a number, or an int64 device tensor of one element or of one for each parameter (a captured call has to take that: a replay reads it
+    anew).  Moments that were never updated belong to step 1, whatever the other parameters have taken: their bias correction is their own.  grad_scale: float32
     device tensor of one element every gradient is multiplied by (a clipping factor, the inverse of a loss scale)."""
     _require(isinstance(tensors, _ops().AdamWTensors), "adamw_step: AdamWTensors are needed")
     _ops().adamw_step(_entry("marius_adamw_check"), _entry("marius_adamw_step"), _entry("marius_adamw_workspace_bytes"), tensors, grads, step, lr, beta1, beta2, eps, weight_decay,

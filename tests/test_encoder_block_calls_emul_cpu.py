@@ -92,7 +92,20 @@ def test_adamw_check_refuses_and_does_nothing(HE):
     assert all(bool((x == 1).all()) for x in (p, m, v))
     L, table = HE.lib(), HE.AdamWTensor(param=p.data_ptr(), grad=p.data_ptr(), exp_avg=m.data_ptr(), exp_avg_sq=v.data_ptr(), n=300)
     call = lambda table, *a: L.marius_adamw_check(table, 1, 0, 0, 32, *a)  # noqa: E731
-    assert call(C.byref(table), 1, None, 1e-3, 0.9, 0.999, 1e-8, 0.0) == 0
-    for bad in ((0, None, 1e-3, 0.9, 0.999, 1e-8, 0.0), (1, None, float("nan"), 0.9, 0.999, 1e-8, 0.0), (1, None, 1e-3, 1.0, 0.999, 1e-8, 0.0), (1, None, 1e-3, 0.9, 0.999, -1.0, 0.0)):
+    assert call(C.byref(table), 1, None, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0) == 0
+    for bad in ((0, None, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0), (1, None, 1, float("nan"), 0.9, 0.999, 1e-8, 0.0), (1, None, 1, 1e-3, 1.0, 0.999, 1e-8, 0.0), (1, None, 1, 1e-3, 0.9, 0.999, -1.0, 0.0),
+                (0, p.data_ptr(), 2, 1e-3, 0.9, 0.999, 1e-8, 0.0)):
         assert call(C.byref(table), *bad) == 1, bad
-    assert call(None, 1, None, 1e-3, 0.9, 0.999, 1e-8, 0.0) == 1
+    assert call(None, 1, None, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0) == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_emulated_counts_of_steps(HE, bits):
+    for capturable in (False, True):
+        T.test_every_parameter_counts_its_own_steps(HE, CPU, bits, capturable)
+
+
+def test_emulated_steps_on_the_device(HE):
+    for count in (3, 70):
+        T.test_a_step_on_the_device_for_every_tensor(HE, CPU, count)
+    T.test_steps_of_tensors_far_apart_in_a_long_list(HE, CPU)

@@ -118,3 +118,112 @@ def test_a_refused_step_changes_nothing(H, dev, what, capturable):
     opt.step()
     other.step()
     assert all(torch.equal(a, b) for a, b in zip(ps, fresh)) and bool((ps[0] < 1).all())
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_every_parameter_counts_its_own_steps(H, dev, bits, capturable):
+    """gradients that come late, now and then, always: every parameter moves as it does in an optimizer of its own that steps when it has a gradient (the same bits), and by the
+    definition with its own number of steps; the counts are saved and loaded"""
+    from marius_amd.optim import AdamW
+
+    hy = dict(lr=1e-2, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1)
+    make = lambda: [torch.nn.Parameter(torch.randn(s, generator=torch.Generator().manual_seed(s)).to(k).to(dev)) for s, k in ((300, F32), (5, F32), (700, F32), (9, BF16))]  # noqa: E731
+    ps, alone = make(), make()
+    opt, single = AdamW(ps, state_bits=bits, capturable=capturable, **hy), [AdamW([p], state_bits=bits, capturable=capturable, **hy) for p in alone]
+    when = [lambda t: t >= 6, lambda t: True, lambda t: t % 3 == 1, lambda t: t >= 6]
+    counts = [0] * 4
+    for t in range(12):
+        before = [(p.detach().clone(), m.detach().clone(), v.detach().clone()) for p, m, v in zip(ps, opt.exp_avg, opt.exp_avg_sq)]
+        for i, (p, q) in enumerate(zip(ps, alone)):
+            g = torch.randn(p.shape, generator=torch.Generator().manual_seed(10 * t + i)).to(p.dtype).to(dev)
+            p.grad, q.grad = (g, g.clone()) if when[i](t) else (None, None)
+        if t == 8:  # a program that ends and goes on
+            opt, old = AdamW(ps, state_bits=bits, capturable=capturable), opt
+            opt.load_state_dict(old.state_dict())
+        opt.step()
+        for i, s in enumerate(single):
+            counts[i] += when[i](t)
+            if when[i](t):
+                s.step()
+            if bits == 32 and when[i](t):
+                (want, mag), _, _ = R.adamw(before[i][0], ps[i].grad, before[i][1], before[i][2], counts[i], 1e-2, 0.9, 0.99, 1e-8, 0.1)
+                R.close(ps[i].detach(), want, mag, 1, "parameter %d at %d" % (i, t))
+        assert all(torch.equal(a, b) for a, b in zip(ps, alone)), t
+        assert all(torch.equal(a.float(), s.exp_avg[0].float()) for a, s in zip(opt.exp_avg, single)), t
+        assert opt.steps == counts and opt.num_steps == max(counts)
+    assert counts == [6, 12, 4, 6] and opt.state_dict()["steps"] == counts
+    old = opt.state_dict()
+    del old["steps"]                                                            # a state of one count for all
+    opt.load_state_dict(old)
+    assert opt.steps == [12] * 4
+
+
+@pytest.mark.parametrize("count", [3, 70])
+def test_a_step_on_the_device_for_every_tensor(H, dev, count):
+    """one call over tensors whose steps differ: each gets what a call for it alone gives it; gradients that are absent in between; more tensors than one launch's arguments hold"""
+    sizes = [1 + 37 * (i % 5) for i in range(count)]
+    ps, gs, ms, vs, _, _ = T.adamw_case(H, dev, sizes, F32, F32, 32, 5)
+    qs, _, ns, ws, _, _ = T.adamw_case(H, dev, sizes, F32, F32, 32, 5)
+    steps = torch.arange(1, count + 1).to(dev)
+    there = [None if i % 7 == 2 else g for i, g in enumerate(gs)]
+    H.adamw_step(H.AdamWTensors(ps, ms, vs), there, steps)
+    for i in range(count):
+        if there[i] is not None:
+            H.adamw_step(H.AdamWTensors([qs[i]], [ns[i]], [ws[i]]), [gs[i]], steps[i:i + 1])
+    for a, b in ((ps, qs), (ms, ns), (vs, ws)):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    for bad in (steps[:2], steps.repeat(2), steps.repeat_interleave(2)[::2][:2]):
+        with pytest.raises(H.MariusHipError, match="one int64, or one for each"):
+            H.adamw_step(H.AdamWTensors(ps, ms, vs), there, bad)
+
+
+def test_steps_of_tensors_far_apart_in_a_long_list(H, dev):
+    """200,000 tensors of which a few have gradients, over 65,536 places apart: the step of each is its own"""
+    n, far = 200_000, [0, 1, 65_535, 65_536, 65_600, 140_000, 199_999]
+    flat = [torch.full((n,), x, device=dev) for x in (1.0, 0.0, 0.0)]
+    grads = [None] * n
+    for i in far:
+        grads[i] = torch.full((1,), 0.5, device=dev)
+    steps = torch.zeros(n, dtype=torch.int64, device=dev)
+    steps[far] = torch.tensor([1, 2, 3, 4, 50, 60, 70]).to(dev)
+    tensors = H.AdamWTensors(*(list(f.split(1)) for f in flat))
+    for live in (far, [5, 199_999]):
+        for i in far:
+            grads[i] = torch.full((1,), 0.5, device=dev) if i in live else None
+        before = [f.clone() for f in flat]
+        H.adamw_step(tensors, grads, steps, weight_decay=0.0)
+        moved = [i for i in live if i in far]
+        assert sorted((flat[0] != before[0]).nonzero().flatten().tolist()) == moved
+        for i in moved:
+            (want, mag), _, _ = R.adamw(before[0][i], grads[i], before[1][i], before[2][i], int(steps[i]), 1e-3, 0.9, 0.999, 1e-8, 0.0)
+            R.close(flat[0][i:i + 1], want.reshape(1), mag.reshape(1), 1, str(i))
+
+
+def test_optimizer_captured_with_a_parameter_that_has_no_gradient(H, dev):
+    """AdamW.step captured and replayed with eager work between the replays: the counts, states and parameters of the eager optimizer, the one without a gradient untouched"""
+    from marius_amd.optim import AdamW
+
+    make = lambda: [torch.nn.Parameter(torch.randn(s, generator=torch.Generator().manual_seed(s)).to(dev)) for s in (300, 5, 700)]  # noqa: E731
+    ps, qs = make(), make()
+    opt, eager = AdamW(ps, capturable=True), AdamW(qs, capturable=True)
+    grads = [torch.zeros(300, device=dev), None, torch.zeros(700, device=dev)]
+    for p, q, g in zip(ps, qs, grads):
+        p.grad, q.grad = g, None if g is None else g.clone()
+    for t in range(2):                                                          # eager steps first
+        for o in (opt, eager):
+            o.step()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for r in range(3):
+        for g, q in zip(grads, qs):
+            if g is not None:
+                g.normal_()
+                q.grad.copy_(g)
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert opt.steps == eager.steps == [3 + r, 0, 3 + r]
+        assert all(torch.equal(a, b) for one, two in ((ps, qs), (opt.exp_avg, eager.exp_avg), (opt.exp_avg_sq, eager.exp_avg_sq)) for a, b in zip(one, two)), r
