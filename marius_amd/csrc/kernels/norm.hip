@@ -40,12 +40,16 @@ enum { SUM_POST_W = 0, SUM_POST_B, SUM_PRE_W, SUM_PRE_B, SUM_GATE, SUMS };
 
 // (sigmoid: the hardware's exponential and reciprocal, a step of fp32 or two together)
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
-__device__ __forceinline__ float gate_act(float v, int act) { return act == MARIUS_ACT_RELU ? (v < 0.f ? 0.f : v) : act == MARIUS_ACT_SIGMOID ? sigmoid(v) : v; }
-// act' from the gate g and a = act(g)
-__device__ __forceinline__ float gate_slope(float g, float a, int act) {
+// sigmoid(v) -> v, its slope: t / (1 + t)^2 of t = exp(-|v|), because a (1 - a) of a rounded a cancels where the gate is almost open (0.9 % off at v = 12, zero from 17 on)
+__device__ __forceinline__ float sigmoid_slope(float& v) {
+    const float t = __expf(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.f + t);
+    v = v >= 0.f ? r : t * r;
+    return t * r * r;
+}
+// act'(g)
+__device__ __forceinline__ float gate_slope(float g, int act) {
     if (act == MARIUS_ACT_RELU) return g <= 0.f ? 0.f : 1.f;
-    if (act == MARIUS_ACT_SIGMOID) return a * (1.f - a);
-    return 1.f;
+    return act == MARIUS_ACT_SIGMOID ? sigmoid_slope(g) : 1.f;
 }
 
 // 1 / sqrt(v) within a step of fp32; the instruction takes no subnormal numbers, which an eps of zero and rows below 1e-19 leave
@@ -294,9 +298,12 @@ __global__ __launch_bounds__(!BLK ? NORM_T : NCH > 1 ? NORM_MAX_T / 2 : NORM_MAX
                 if (live) EACH(NCH, VEC) acc[SUM_GATE][j][e] += u[j][e];
             } else {
                 R.get(gp, gc);
-                if (A.act == MARIUS_ACT_RELU) EACH(NCH, VEC) u[j][e] = gc[j][e] <= 0.f ? 0.f : u[j][e];
-                R.open(gc, A.act);
-                if (A.act == MARIUS_ACT_SIGMOID) EACH(NCH, VEC) u[j][e] *= gc[j][e] * (1.f - gc[j][e]);
+                if (A.act == MARIUS_ACT_SIGMOID) {
+                    EACH(NCH, VEC) u[j][e] *= sigmoid_slope(gc[j][e]);
+                } else if (A.act == MARIUS_ACT_RELU) {
+                    EACH(NCH, VEC) u[j][e] = gc[j][e] <= 0.f ? 0.f : u[j][e];
+                    R.open(gc, A.act);
+                }
                 if (live) R.template store<T>(A.dgate, row, A.dgate_ld, u);
             }
             EACH(NCH, VEC) dt[j][e] *= gc[j][e];
@@ -361,8 +368,7 @@ __global__ __launch_bounds__(1024) void residual_norm_sums_kernel(NormSumArgs A)
 #pragma unroll
         for (int q = 0; q < 32; ++q) t += red[q * 32 + threadIdx.x];
         if (k == SUM_GATE) {
-            const float g = element_any(A.gate, A.type, c);
-            t *= gate_slope(g, gate_act(g, A.act), A.act);
+            t *= gate_slope(element_any(A.gate, A.type, c), A.act);
         }
         element_store_any(A.out[k], A.type, c, t);
     }

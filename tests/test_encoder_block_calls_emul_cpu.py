@@ -109,3 +109,10 @@ def test_emulated_steps_on_the_device(HE):
     for count in (3, 70):
         T.test_a_step_on_the_device_for_every_tensor(HE, CPU, count)
     T.test_steps_of_tensors_far_apart_in_a_long_list(HE, CPU)
+
+
+# ------------------------------------------------------------------------------------------------ residual norm
+def test_emulated_sigmoid_gates_far_from_zero(HE):
+    for gate in ("channel", "element"):
+        for kind in (F32, BF16):
+            T.test_sigmoid_gates_far_from_zero(HE, CPU, gate, kind)

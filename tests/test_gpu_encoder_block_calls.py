@@ -1,6 +1,7 @@
 """Calls of the encoder block's operators that their documentation allows and tests/test_gpu_encoder_block.py does not make: outputs beside the main ones, graphs and optimizers in
 states that a program reaches, inputs at the ends of their ranges.  Bounds: tests/encoder_block_reference.py."""
 import math
+from unittest import mock
 
 import pytest
 import torch
@@ -227,3 +228,28 @@ def test_optimizer_captured_with_a_parameter_that_has_no_gradient(H, dev):
         torch.cuda.synchronize()
         assert opt.steps == eager.steps == [3 + r, 0, 3 + r]
         assert all(torch.equal(a, b) for one, two in ((ps, qs), (opt.exp_avg, eager.exp_avg), (opt.exp_avg_sq, eager.exp_avg_sq)) for a, b in zip(one, two)), r
+
+
+# ------------------------------------------------------------------------------------------------ residual norm
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("gate", ["channel", "element"])
+def test_sigmoid_gates_far_from_zero(H, dev, gate, kind):
+    """the gradient of a gate that is almost open or almost shut: sigmoid's slope is as small on one side as on the other, and as exact (a (1 - a) from a rounded a is zero from
+    17 on); at +-90 it is below fp32's normal numbers, and at +-200 zero"""
+    n, d = 7, 60
+    x, z, _, pw, pb, w, b, gy, gh = T.norm_inputs(n, d, F32, kind, None, True, True, dev, 4)
+    far = torch.tensor([s * v for s in (-1, 1) for v in (8, 9.5, 11, 12, 13, 14, 15, 15.5, 16, 16.5, 17, 18, 20, 25, 30, 40, 60, 80)] + [0, -0.5, 0.5, 4, -4, 2] * 4)
+    g = far.to(kind).to(dev) if gate == "element" else far.to(dev)
+    g = g.expand(n, d).contiguous() if gate == "element" else g
+    how = dict(post_norm=True, kind="LAYER", eps=1e-3, residual_scale=1.0, gate_activation="SIGMOID")
+    params = (g, pw, pb, w, b)
+    y = H.residual_norm(x, z, *params, **how)[0]
+    got = H.residual_norm_backward(gy, gh, y, z, *params, **how)
+    # (sigmoid (1 - sigmoid) cancels in 64 bits, too: 2^-53 beside a slope of 1.4e-11 at 25 are 130 roundings of fp32, from 37 on the difference is zero)
+    with mock.patch.object(R, "slope", lambda v, name: torch.exp(-v.abs()) / (1 + torch.exp(-v.abs())) ** 2):
+        R.check_residual_norm_backward(got, gy, gh, y, z, *params, True, True, "LAYER", 1e-3, 1.0, "SIGMOID")
+    small = got["dgate"].reshape(-1, d)[:, torch.tensor([10, 28])].abs().float()
+    assert bool((small > 0).all())                                             # at -17 and 17
+    for v in (90.0, -90.0, 200.0, -200.0):
+        edge = H.residual_norm_backward(gy, gh, y, z, torch.full_like(g, v), *params[1:], **how)["dgate"]
+        assert bool(edge.isfinite().all()) and float(edge.abs().max()) < 1e-30
