@@ -82,6 +82,11 @@ def test_emulated_refused_steps(HE, capturable):
         T.test_a_refused_step_changes_nothing(HE, CPU, what, capturable)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_emulated_gradients_that_are_not_contiguous(HE, bits):
+    T.test_gradients_that_are_not_contiguous(HE, CPU, bits)
+
+
 def test_adamw_check_refuses_and_does_nothing(HE):
     p, m, v = (torch.ones(300) for _ in range(3))
     t = HE.AdamWTensors([p], [m], [v])

@@ -201,6 +201,22 @@ def test_steps_of_tensors_far_apart_in_a_long_list(H, dev):
             R.close(flat[0][i:i + 1], want.reshape(1), mag.reshape(1), 1, str(i))
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_that_are_not_contiguous(H, dev, bits):
+    """a column, a transposed matrix, a broadcast number: the step of a contiguous copy, in parameters and states"""
+    sizes, runs = [200, 600, 64], []
+    wide = torch.randn(200, 2, generator=torch.Generator().manual_seed(1)).to(dev)
+    grads = [wide[:, 0], torch.randn(30, 20, generator=torch.Generator().manual_seed(2)).to(dev).t(), torch.full((1,), 0.25, device=dev).expand(64)]
+    for copied in (False, True):
+        ps, _, ms, vs, sm, sv = T.adamw_case(H, dev, sizes, F32, F32, bits, 1)
+        start = [p.clone() for p in ps]
+        tensors = H.AdamWTensors([p.view(20, 30) if i == 1 else p for i, p in enumerate(ps)], ms, vs, sm, sv)
+        H.adamw_step(tensors, [g.contiguous() if copied else g for g in grads], 4)
+        assert not any(torch.equal(p, s) for p, s in zip(ps, start))
+        runs.append([t.float() for ts in (ps, ms, vs, sm or [], sv or []) for t in ts])
+    assert not any(g.is_contiguous() for g in grads) and all(torch.equal(a, b) for a, b in zip(*runs))
+
+
 def test_optimizer_captured_with_a_parameter_that_has_no_gradient(H, dev):
     """AdamW.step captured and replayed with eager work between the replays: the counts, states and parameters of the eager optimizer, the one without a gradient untouched"""
     from marius_amd.optim import AdamW
@@ -253,3 +269,61 @@ def test_sigmoid_gates_far_from_zero(H, dev, gate, kind):
     for v in (90.0, -90.0, 200.0, -200.0):
         edge = H.residual_norm_backward(gy, gh, y, z, torch.full_like(g, v), *params[1:], **how)["dgate"]
         assert bool(edge.isfinite().all()) and float(edge.abs().max()) < 1e-30
+
+
+# ------------------------------------------------------------------------------------------------ streams
+def test_launches_follow_the_current_stream(H, dev):
+    """inputs that are written on a side stream behind some 10 ms of products, by calls on that stream: a launch on any other stream would find the old ones.  The old inputs are
+    valid too, and their results differ."""
+    n, rows, heads, dim = 50, 60, 4, 32
+    old_lists = [t.to(dev) for t in T.lists(n, rows, [(i + 1) % 9 for i in range(n - 4)] + [40, 80, 0, 80], 1)]
+    new_lists = [(old_lists[0] * 7 + 3) % rows, old_lists[1]]
+    shapes = dict(q=(n, heads, dim), k=(rows, heads, dim), v=(rows, heads, dim), g=(n, heads, dim), x=(rows, 128), z=(rows, 128), p=(500,), grad=(500,))
+    rnd = lambda seed: {name: torch.randn(s, generator=torch.Generator().manual_seed(seed + i)).to(dev) for i, (name, s) in enumerate(shapes.items())}  # noqa: E731
+    old, new, w = rnd(0), rnd(100), torch.linspace(0.5, 1.5, 128, device=dev)
+    plan, bins = H.NeighborPlan(*new_lists, rows), torch.arange(rows).to(dev) % 7
+
+    def calls(t, lists):
+        made = H.NeighborPlan(*lists, rows)
+        out, stats, lse = H.neighbor_attention(t["q"], t["k"], t["v"], plan, return_lse=True)
+        y, h = H.residual_norm(t["x"], t["z"], w, pre_weight=w, post_norm=True)
+        back = H.residual_norm_backward(t["x"], t["z"], y, t["z"], w, pre_weight=w, post_norm=True)
+        m, v = torch.zeros_like(t["p"]), torch.zeros_like(t["p"])
+        H.adamw_step(H.AdamWTensors([t["p"]], [m], [v]), [t["grad"]], 3)
+        return [made.index, made._r_owner[:made.num_entries], out, stats, lse, *H.neighbor_attention_backward(t["g"], t["q"], t["k"], t["v"], stats, plan)[:3], y, h,
+                *(g for g in back.values() if g is not None), H.bin_sum(t["x"], bins, 7), t["p"], m, v]
+
+    want, stale = (calls({k: v.clone() for k, v in t.items()}, lists) for t, lists in ((new, new_lists), (old, old_lists)))
+    assert not any(torch.equal(a, b) for a, b in zip(want, stale))
+    inputs, lists = {k: v.clone() for k, v in old.items()}, [t.clone() for t in old_lists]
+    big = torch.randn(4096, 4096, device=dev)
+    side = torch.cuda.Stream(device=dev)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(10):
+            big @ big
+        for name, t in inputs.items():
+            t.copy_(new[name])
+        for t, fresh in zip(lists, new_lists):
+            t.copy_(fresh)
+        # the plan first: its readbacks wait for the products, so a second delay stands in front of the others
+        made = H.NeighborPlan(*lists, rows)
+        assert torch.equal(made.index, want[0]) and torch.equal(made._r_owner[:made.num_entries], want[1])
+        for name, t in inputs.items():
+            t.copy_(old[name])
+        side.synchronize()
+        for _ in range(10):
+            big @ big
+        for name, t in inputs.items():
+            t.copy_(new[name])
+        delayed = not side.query()
+        out, stats, lse = H.neighbor_attention(inputs["q"], inputs["k"], inputs["v"], plan, return_lse=True)
+        y, h = H.residual_norm(inputs["x"], inputs["z"], w, pre_weight=w, post_norm=True)
+        back = H.residual_norm_backward(inputs["x"], inputs["z"], y, inputs["z"], w, pre_weight=w, post_norm=True)
+        sums = H.bin_sum(inputs["x"], bins, 7)
+        m, v = torch.zeros(500, device=dev), torch.zeros(500, device=dev)
+        H.adamw_step(H.AdamWTensors([inputs["p"]], [m], [v]), [inputs["grad"]], 3)
+        got = [out, stats, lse, *H.neighbor_attention_backward(inputs["g"], inputs["q"], inputs["k"], inputs["v"], stats, plan)[:3], y, h,
+               *(g for g in back.values() if g is not None), sums, inputs["p"], m, v]
+    side.synchronize()
+    assert delayed and len(got) == len(want) - 2 and all(torch.equal(a, b) for a, b in zip(got, want[2:]))
