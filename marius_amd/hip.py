@@ -832,8 +832,9 @@ class NeighborPlan:
 
     def record_stream(self, stream):
         """the plan is in use on `stream` (torch.Tensor.record_stream of everything it holds)"""
-        for t in (self._index, self._items, self._splits, self._r_owner, self._r_entry, self._r_items, self._r_splits):
-            t.record_stream(stream)
+        for t in (self._index, self._items, self._splits, self._r_owner, self._r_entry, self._r_items, self._r_splits, self.owner, self.offsets, *self._starts):
+            if t is not None:
+                t.record_stream(stream)
 
     def places(self, part):
         """where a part's entries lie in the plan's order: part 0, 1 (the lists, entry by entry) or "own" (the targets' own rows) -> int64 positions.  A bias is laid out by them."""

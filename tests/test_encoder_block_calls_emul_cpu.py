@@ -121,3 +121,8 @@ def test_emulated_sigmoid_gates_far_from_zero(HE):
     for gate in ("channel", "element"):
         for kind in (F32, BF16):
             T.test_sigmoid_gates_far_from_zero(HE, CPU, gate, kind)
+
+
+# ------------------------------------------------------------------------------------------------ plans
+def test_emulated_plan_is_recorded_whole(HE):
+    T.test_a_plan_in_use_on_another_stream_is_recorded_whole(HE, CPU)

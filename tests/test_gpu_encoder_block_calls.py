@@ -327,3 +327,19 @@ def test_launches_follow_the_current_stream(H, dev):
                *(g for g in back.values() if g is not None), sums, inputs["p"], m, v]
     side.synchronize()
     assert delayed and len(got) == len(want) - 2 and all(torch.equal(a, b) for a, b in zip(got, want[2:]))
+
+
+# ------------------------------------------------------------------------------------------------ plans
+def test_a_plan_in_use_on_another_stream_is_recorded_whole(H, dev):
+    """record_stream reaches every tensor that the plan holds, what `places` reads among them"""
+    index, offsets = T.lists(4, 9, [2, 0, 3, 1], 1)
+    plan = H.NeighborPlan(index.to(dev), offsets.to(dev), 9, index.to(dev), offsets.to(dev), 5)
+    seen = set()
+    with mock.patch.object(torch.Tensor, "record_stream", lambda t, stream: seen.add(t.data_ptr())):
+        plan.record_stream(None)
+    held, todo = [], list(vars(plan).values())
+    while todo:
+        x = todo.pop()
+        todo += list(x) if isinstance(x, (list, tuple)) else []
+        held += [x] if torch.is_tensor(x) else []
+    assert len(held) >= 9 and {t.data_ptr() for t in held if t.numel() > 0} <= seen
