@@ -828,11 +828,12 @@ class NeighborPlan:
         d.index, d.items, d.splits, d.r_owner, d.r_entry, d.r_items, d.r_splits = (t.data_ptr() for t in (self._index, self._items, self._splits, self._r_owner, self._r_entry,
                                                                                                         self._r_items, self._r_splits))
         (d.n_items, d.n_slots, d.n_splits, _), (d.r_n_items, d.r_n_slots, d.r_n_splits, _) = counts
-        self._starts, self._ends, self._own = (lists[1], lists[3]), (ta, tb), own >= 0
+        # (the offsets are the caller's, who may write other ones into them: those of the first of two lists are kept, the others follow from the plan's own)
+        self._starts, self._ends, self._own = None if index_b is None else lists[1].clone(), (ta, tb), own >= 0
 
     def record_stream(self, stream):
         """the plan is in use on `stream` (torch.Tensor.record_stream of everything it holds)"""
-        for t in (self._index, self._items, self._splits, self._r_owner, self._r_entry, self._r_items, self._r_splits, self.owner, self.offsets, *self._starts):
+        for t in (self._index, self._items, self._splits, self._r_owner, self._r_entry, self._r_items, self._r_splits, self.owner, self.offsets, self._starts):
             if t is not None:
                 t.record_stream(stream)
 
@@ -842,14 +843,16 @@ class NeighborPlan:
         if part == "own":
             _require(self._own, "NeighborPlan.places: the plan has no own rows")
             return ends[1:] - 1
-        starts = self._starts[part]
-        _require(starts is not None, "NeighborPlan.places: the plan has one list")
+        _require(part == 0 or self._starts is not None, "NeighborPlan.places: the plan has one list")
         # a target's entries of list 0 open its part of the plan, those of list 1 follow them
-        length = torch.diff(starts, append=starts.new_tensor([self._ends[part]]))
+        length = torch.diff(ends) - (1 if self._own else 0)
+        if self._starts is not None:
+            of_first = torch.diff(self._starts, append=self._starts.new_tensor([self._ends[0]]))
+            length = of_first if part == 0 else length - of_first
         first = ends[:-1] if part == 0 else ends[1:] - (1 if self._own else 0) - length
         total = self._ends[part]
         owner = torch.repeat_interleave(torch.arange(self.n, device=self.device), length, output_size=total)
-        return first[owner] + torch.arange(total, device=self.device) - starts[owner]
+        return first[owner] + torch.arange(total, device=self.device) - (length.cumsum(0) - length)[owner]
 
 
 def _plan(plan):

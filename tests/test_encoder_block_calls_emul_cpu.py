@@ -126,3 +126,7 @@ def test_emulated_sigmoid_gates_far_from_zero(HE):
 # ------------------------------------------------------------------------------------------------ plans
 def test_emulated_plan_is_recorded_whole(HE):
     T.test_a_plan_in_use_on_another_stream_is_recorded_whole(HE, CPU)
+
+
+def test_emulated_plan_keeps_no_hold_on_its_lists(HE):
+    T.test_a_plan_keeps_no_hold_on_the_lists_it_was_made_of(HE, CPU)

@@ -343,3 +343,19 @@ def test_a_plan_in_use_on_another_stream_is_recorded_whole(H, dev):
         todo += list(x) if isinstance(x, (list, tuple)) else []
         held += [x] if torch.is_tensor(x) else []
     assert len(held) >= 9 and {t.data_ptr() for t in held if t.numel() > 0} <= seen
+
+
+def test_a_plan_keeps_no_hold_on_the_lists_it_was_made_of(H, dev):
+    """a program that samples into the same buffers batch after batch: the plan, and where its entries lie, stay those of the lists that it was made of"""
+    a, oa = T.lists(4, 9, [2, 0, 3, 1], 1)
+    b, ob = T.lists(4, 9, [0, 4, 1, 0], 2)
+    for second in (False, True):
+        for own in (None, 5):
+            buffers = [t.to(dev) for t in ((a, oa, b, ob) if second else (a, oa))]
+            plan = H.NeighborPlan(buffers[0], buffers[1], 9, *buffers[2:], self_offset=own)
+            for t in buffers:
+                t.zero_()
+            assert torch.equal(plan.index[plan.places(0)].cpu().long(), a)
+            assert not second or torch.equal(plan.index[plan.places(1)].cpu().long(), b)
+            every = [plan.places(p) for p in ([0, 1] if second else [0]) + ([] if own is None else ["own"])]
+            assert torch.equal(torch.cat(every).sort()[0].cpu(), torch.arange(plan.num_entries))
