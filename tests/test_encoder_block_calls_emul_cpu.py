@@ -130,3 +130,14 @@ def test_emulated_plan_is_recorded_whole(HE):
 
 def test_emulated_plan_keeps_no_hold_on_its_lists(HE):
     T.test_a_plan_keeps_no_hold_on_the_lists_it_was_made_of(HE, CPU)
+
+
+def test_neighbor_plan_refuses_offsets_of_lists_that_are_not_there(HE):
+    """offsets over an index of no entries are zeros: others belong to another index"""
+    i64 = lambda *v: torch.tensor(v, dtype=torch.int64)  # noqa: E731
+    for bad in (i64(0, 3), i64(1, 1), i64(0, -1)):
+        refused(HE, "ascend", HE.NeighborPlan, i64(), bad, 3)
+        refused(HE, "ascend", HE.NeighborPlan, i64(0, 1, 2), i64(0, 2), 3, i64(), bad)
+        refused(HE, "ascend", HE.NeighborPlan, i64(), bad, 3, i64(0, 1, 2), i64(0, 2), self_offset=1)
+    plan = HE.NeighborPlan(i64(), i64(0, 0), 3, i64(0, 1, 2), i64(0, 2), self_offset=1)
+    assert plan.num_entries == 5 and plan.places(0).numel() == 0 and plan.places(1).tolist() == [0, 1, 3] and plan.places("own").tolist() == [2, 4]
