@@ -293,12 +293,14 @@ std::tuple<Tensor, Tensor, Tensor, MaybeTensor> neighbor_attention_backward(uint
 }
 
 // ---------------------------------------------------------------------------------------------------------------- AdamW
-// The tensors of an optimizer: parameters (they may be given new memory between steps: their addresses are read at every one) and states.
+// The tensors of an optimizer: parameters and states.  Both may be given new memory between steps: their addresses are read at every one, and looked over when one has changed.
 struct AdamWTensors {
     std::vector<Tensor> params;
     std::vector<std::vector<Tensor>> states;  // exp_avg, exp_avg_sq (, their scales)
     std::vector<marius_adamw_tensor> table;
+    std::vector<const void*> seen;            // the parameters' addresses when they were looked over
     int type = 0, bits = 32;
+    at::Device device = at::kCPU;
 
     AdamWTensors(std::vector<Tensor> p, std::vector<Tensor> m, std::vector<Tensor> v, std::optional<std::vector<Tensor>> ms, std::optional<std::vector<Tensor>> vs)
         : params(std::move(p)) {
@@ -312,29 +314,37 @@ struct AdamWTensors {
         }
         for (const auto& s : states) require(s.size() == params.size(), "AdamWTensors: lists of different lengths");
         type = type_of("parameters", params[0]);
-        const at::Device device = params[0].device();
+        device = params[0].device();
         table.resize(params.size());
         for (size_t i = 0; i < params.size(); ++i) {
             const Tensor& w = params[i];
             require(w.scalar_type() == params[0].scalar_type() && w.is_contiguous(), "AdamWTensors: parameter ", i, " is not a contiguous ", params[0].scalar_type(), " tensor");
             require(w.device() == device, "AdamWTensors: tensors of parameter ", i, " are contiguous and on ", device);
-            for (size_t k = 0; k < states.size(); ++k) {
-                const Tensor& s = states[k][i];
-                require(s.device() == device && s.is_contiguous(), "AdamWTensors: tensors of parameter ", i, " are contiguous and on ", device);
-                if (k < 2)
-                    require(s.numel() == w.numel() && s.scalar_type() == (bits == 32 ? at::kFloat : at::kFloat8_e4m3fn), "AdamWTensors: states of parameter ", i, " are ",
-                            bits == 32 ? "float32" : "float8_e4m3fn", " of its size");
-                else
-                    require(s.scalar_type() == at::kFloat && s.numel() == (w.numel() + 255) / 256, "AdamWTensors: scales of parameter ", i, " are float32, one for 256");
-            }
-            marius_adamw_tensor& t = table[i];
-            t.exp_avg = states[0][i].data_ptr();
-            t.exp_avg_sq = states[1][i].data_ptr();
-            t.exp_avg_scale = bits == 8 ? (float*)states[2][i].data_ptr() : nullptr;
-            t.exp_avg_sq_scale = bits == 8 ? (float*)states[3][i].data_ptr() : nullptr;
-            t.n = w.numel();
+            table[i].n = w.numel();
         }
-        // no tensor twice, none inside another: every launch updates all of them at once
+        seen.resize(params.size());
+        for (size_t i = 0; i < params.size(); ++i) look_at_states(i);
+        look_for_overlaps();
+    }
+    // what a step writes besides the parameters, as it is now
+    void look_at_states(size_t i) {
+        marius_adamw_tensor& t = table[i];
+        for (size_t k = 0; k < states.size(); ++k) {
+            const Tensor& s = states[k][i];
+            require(s.device() == device && s.is_contiguous(), "AdamWTensors: tensors of parameter ", i, " are contiguous and on ", device);
+            if (k < 2)
+                require(s.numel() == t.n && s.scalar_type() == (bits == 32 ? at::kFloat : at::kFloat8_e4m3fn), "AdamWTensors: states of parameter ", i, " are ",
+                        bits == 32 ? "float32" : "float8_e4m3fn", " of its size");
+            else
+                require(s.scalar_type() == at::kFloat && s.numel() == (t.n + 255) / 256, "AdamWTensors: scales of parameter ", i, " are float32, one for 256");
+        }
+        t.exp_avg = states[0][i].data_ptr();
+        t.exp_avg_sq = states[1][i].data_ptr();
+        t.exp_avg_scale = bits == 8 ? (float*)states[2][i].data_ptr() : nullptr;
+        t.exp_avg_sq_scale = bits == 8 ? (float*)states[3][i].data_ptr() : nullptr;
+    }
+    // no tensor twice, none inside another: every launch updates all of them at once
+    void look_for_overlaps() {
         std::vector<std::pair<const char*, const char*>> spans;
         auto span = [&](const Tensor& t) {
             if (t.numel() > 0) spans.emplace_back((const char*)t.data_ptr(), (const char*)t.data_ptr() + t.nbytes());
@@ -344,6 +354,21 @@ struct AdamWTensors {
             for (const Tensor& t : s) span(t);
         std::sort(spans.begin(), spans.end());
         for (size_t i = 1; i < spans.size(); ++i) require(spans[i - 1].second <= spans[i].first, "AdamWTensors: a tensor appears twice, or overlaps another");
+        for (size_t i = 0; i < params.size(); ++i) seen[i] = params[i].data_ptr();
+    }
+    void refresh() {
+        bool moved = false;
+        for (size_t i = 0; i < params.size(); ++i) {
+            const marius_adamw_tensor& t = table[i];
+            bool same = states[0][i].data_ptr() == t.exp_avg && states[1][i].data_ptr() == t.exp_avg_sq && states[0][i].numel() == t.n && states[1][i].numel() == t.n;
+            if (bits == 8) same = same && states[2][i].data_ptr() == t.exp_avg_scale && states[3][i].data_ptr() == t.exp_avg_sq_scale;
+            if (!same) {
+                seen[i] = nullptr;  // (looked over again next time, too, if this is refused)
+                look_at_states(i);
+            }
+            moved = moved || !same || params[i].data_ptr() != seen[i];
+        }
+        if (moved) look_for_overlaps();
     }
 };
 // A step's arguments, checked; nothing is launched and nothing changes until they are used.  `step`: an int or an int64 device tensor (of one number, or one for each parameter)
@@ -359,8 +384,9 @@ AdamWCall adamw_call(uintptr_t check_entry, AdamWTensors& a, const std::vector<M
                      double weight_decay, const MaybeTensor& grad_scale, bool capturing) {
     const size_t count = a.params.size();
     require(grads.size() == count, "adamw_step: ", grads.size(), " gradients for ", count, " parameters");
-    const at::Device device = a.states[0][0].device();
+    const at::Device device = a.device;
     AdamWCall c;
+    a.refresh();
     c.table = a.table;  // (a copy: two threads may step at once)
     std::optional<at::ScalarType> kind;
     for (size_t i = 0; i < count; ++i) {
@@ -406,7 +432,7 @@ void adamw_step(uintptr_t check_entry, uintptr_t entry, uintptr_t workspace_entr
     AdamWCall c = adamw_call(check_entry, a, grads, step, lr, beta1, beta2, eps, weight_decay, grad_scale, capturing);
     if (c.grad_type < 0) return;
     const size_t count = a.params.size();
-    const at::Device device = a.states[0][0].device();
+    const at::Device device = a.device;
     const c10::OptionalDeviceGuard guard(device);
     std::vector<Tensor> copies;
     for (size_t i : c.strided) {
@@ -431,7 +457,7 @@ void bind_encoder_ops(py::module_& m) {
     m.def("neighbor_attention_backward", &neighbor_attention_backward);
     py::class_<AdamWTensors>(m, "AdamWTensors")
         .def(py::init<std::vector<Tensor>, std::vector<Tensor>, std::vector<Tensor>, std::optional<std::vector<Tensor>>, std::optional<std::vector<Tensor>>>())
-        .def_property_readonly("device", [](const AdamWTensors& a) { return a.states[0][0].device(); })
+        .def_property_readonly("device", [](const AdamWTensors& a) { return a.device; })
         .def_readonly("params", &AdamWTensors::params);
     m.def("adamw_check", &adamw_check);
     m.def("adamw_step", &adamw_step);

@@ -141,3 +141,11 @@ def test_neighbor_plan_refuses_offsets_of_lists_that_are_not_there(HE):
         refused(HE, "ascend", HE.NeighborPlan, i64(), bad, 3, i64(0, 1, 2), i64(0, 2), self_offset=1)
     plan = HE.NeighborPlan(i64(), i64(0, 0), 3, i64(0, 1, 2), i64(0, 2), self_offset=1)
     assert plan.num_entries == 5 and plan.places(0).numel() == 0 and plan.places(1).tolist() == [0, 1, 3] and plan.places("own").tolist() == [2, 4]
+
+
+def test_emulated_parameters_given_one_memory(HE):
+    T.test_parameters_given_one_memory_after_their_optimizer_was_made(HE, CPU)
+
+
+def test_emulated_states_given_new_memory(HE):
+    T.test_states_given_new_memory(HE, CPU)

@@ -359,3 +359,50 @@ def test_a_plan_keeps_no_hold_on_the_lists_it_was_made_of(H, dev):
             assert not second or torch.equal(plan.index[plan.places(1)].cpu().long(), b)
             every = [plan.places(p) for p in ([0, 1] if second else [0]) + ([] if own is None else ["own"])]
             assert torch.equal(torch.cat(every).sort()[0].cpu(), torch.arange(plan.num_entries))
+
+
+def test_parameters_given_one_memory_after_their_optimizer_was_made(H, dev):
+    """new memory between two steps is read at the next one; the memory of another parameter or of a state is refused: two workgroups would write one element"""
+    from marius_amd.optim import AdamW
+
+    p, q, r = (torch.nn.Parameter(torch.ones(300, device=dev)) for _ in range(3))
+    opt = AdamW([p, q, r])
+    for t in (p, q, r):
+        t.grad = torch.ones_like(t)
+    opt.step()
+    own, flat = q.data, torch.ones(500, device=dev)
+    for bad in (p.data, opt.exp_avg[2].data, opt.exp_avg_sq[0].data):
+        q.data = bad
+        with pytest.raises(H.MariusHipError, match="appears twice, or overlaps"):
+            opt.step()
+    p.data, q.data = flat[:300], flat[200:]
+    with pytest.raises(H.MariusHipError, match="appears twice, or overlaps"):
+        opt.step()
+    q.data, p.data = own, torch.ones(300, device=dev)
+    opt.step()
+    fresh = torch.ones(300, device=dev)
+    r.data = fresh
+    opt.step()
+    assert opt.num_steps == 3 and r.data_ptr() == fresh.data_ptr() and bool((fresh < 1).all()) and bool((p < 1).all()) and bool((q < 1).all())
+
+
+def test_states_given_new_memory(H, dev):
+    """a state whose tensor is given other memory (loaded from elsewhere, say) is read and written there; memory that does not fit is refused"""
+    ps, gs, ms, vs, sm, sv = T.adamw_case(H, dev, [300, 700], F32, F32, 8, 3)
+    qs, hs, ns, ws, tm, tv = T.adamw_case(H, dev, [300, 700], F32, F32, 8, 3)
+    one, two = H.AdamWTensors(ps, ms, vs, sm, sv), H.AdamWTensors(qs, ns, ws, tm, tv)
+    H.adamw_step(one, gs, 1)
+    H.adamw_step(two, hs, 1)
+    for t in (ns[1], ws[0], tm[1]):
+        old = t.data
+        t.data = old.clone()
+        old.zero_()
+    H.adamw_step(one, gs, 2)
+    H.adamw_step(two, hs, 2)
+    assert all(torch.equal(a.float(), b.float()) for x, y in ((ps, qs), (ms, ns), (vs, ws), (sm, tm), (sv, tv)) for a, b in zip(x, y))
+    for t, bad in ((ns[0], ns[0][:200].clone()), (tm[0], tm[0][:1].clone()), (ws[1], torch.zeros(700, 2, device=dev).to(torch.float8_e4m3fn)[:, 0]), (ns[0], ns[0][:200])):
+        kept, t.data = t.data, bad
+        with pytest.raises(H.MariusHipError, match="of its size|one for 256|contiguous"):
+            H.adamw_step(two, hs, 3)
+        t.data = kept
+    H.adamw_step(two, hs, 3)
