@@ -444,6 +444,8 @@ class ResidualNorm(torch.nn.Module):
     def __init__(self, dim, post_norm=False, pre_norm=True, kind="RMS", eps=1e-6, bias=False, gate="NONE", gate_activation="NONE", gate_init=1.0, residual_scale=1.0, device="cuda:0"):
         super().__init__()
         vec = lambda there, value: torch.nn.Parameter(torch.full((dim,), value, device=device)) if there else None  # noqa: E731
+        if gate not in ("NONE", "CHANNEL", "ELEMENT"):
+            raise H.MariusHipError("ResidualNorm: gate is one of NONE, CHANNEL, ELEMENT")
         self.gate_kind = gate
         self.post_weight, self.post_bias = vec(post_norm, 1.0), vec(post_norm and bias, 0.0)
         self.pre_weight, self.pre_bias = vec(pre_norm, 1.0), vec(pre_norm and bias, 0.0)
@@ -452,6 +454,8 @@ class ResidualNorm(torch.nn.Module):
 
     def forward(self, x, block=None, gate=None):
         if block is None:
+            if gate is not None:
+                raise H.MariusHipError("ResidualNorm: a gate without a block that it opens")
             how = dict(self.how, post_norm=False, residual_scale=1.0, gate_activation="NONE")
             return x, _ResidualNorm.apply(x, None, None, None, None, self.pre_weight, self.pre_bias, how)[0]
         if (self.gate_kind == "ELEMENT") != (gate is not None):

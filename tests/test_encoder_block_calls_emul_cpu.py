@@ -149,3 +149,10 @@ def test_emulated_parameters_given_one_memory(HE):
 
 def test_emulated_states_given_new_memory(HE):
     T.test_states_given_new_memory(HE, CPU)
+
+
+def test_residual_norm_module_refuses_gates_it_would_leave_out(HE, G):
+    refused(HE, "gate is one of", G.ResidualNorm, 4, gate="channel", device=CPU)
+    refused(HE, "gate is one of", G.GraphAttentionEncoder, 4, 8, 2, 1, 2, gate=None, device=CPU)
+    for gate in ("NONE", "CHANNEL", "ELEMENT"):
+        refused(HE, "without a block", G.ResidualNorm(4, gate=gate, device=CPU), torch.zeros(2, 4), None, torch.zeros(2, 4))
