@@ -418,18 +418,19 @@ AdamWCall adamw_call(uintptr_t check_entry, AdamWTensors& a, const std::vector<M
     if (!kind) return c;
     require(*kind == at::kFloat || *kind == at::kBFloat16 || *kind == at::kHalf, "adamw_step: float32, bfloat16 or float16 gradients required, got ", *kind);
     c.grad_type = *kind == at::kFloat ? MARIUS_F32 : *kind == at::kBFloat16 ? MARIUS_BF16 : MARIUS_F16;
-    check(((decltype(&marius_adamw_check))check_entry)(c.table.data(), (int32_t)count, a.type, c.grad_type, a.bits, c.step, (const int64_t*)data(c.counter), c.steps(), lr,
-                                                       beta1, beta2, eps, weight_decay),
-          "adamw_step");
+    if (check_entry)  // (marius_adamw_step makes these checks itself, before it launches)
+        check(((decltype(&marius_adamw_check))check_entry)(c.table.data(), (int32_t)count, a.type, c.grad_type, a.bits, c.step, (const int64_t*)data(c.counter), c.steps(), lr,
+                                                           beta1, beta2, eps, weight_decay),
+              "adamw_step");
     return c;
 }
 void adamw_check(uintptr_t check_entry, AdamWTensors& a, const std::vector<MaybeTensor>& grads, const py::object& step, double lr, double beta1, double beta2, double eps,
                  double weight_decay, const MaybeTensor& grad_scale, bool capturing) {
     adamw_call(check_entry, a, grads, step, lr, beta1, beta2, eps, weight_decay, grad_scale, capturing);
 }
-void adamw_step(uintptr_t check_entry, uintptr_t entry, uintptr_t workspace_entry, AdamWTensors& a, const std::vector<MaybeTensor>& grads, const py::object& step, double lr, double beta1,
+void adamw_step(uintptr_t entry, uintptr_t workspace_entry, AdamWTensors& a, const std::vector<MaybeTensor>& grads, const py::object& step, double lr, double beta1,
                 double beta2, double eps, double weight_decay, const MaybeTensor& grad_scale, bool capturing) {
-    AdamWCall c = adamw_call(check_entry, a, grads, step, lr, beta1, beta2, eps, weight_decay, grad_scale, capturing);
+    AdamWCall c = adamw_call(0, a, grads, step, lr, beta1, beta2, eps, weight_decay, grad_scale, capturing);
     if (c.grad_type < 0) return;
     const size_t count = a.params.size();
     const at::Device device = a.device;

@@ -919,7 +919,7 @@ def adamw_step(tensors, grads, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, 
     anew).  Moments that were never updated belong to step 1, whatever the other parameters have taken: their bias correction is their own.  grad_scale: float32
     device tensor of one element every gradient is multiplied by (a clipping factor, the inverse of a loss scale)."""
     _require(isinstance(tensors, _ops().AdamWTensors), "adamw_step: AdamWTensors are needed")
-    _ops().adamw_step(_entry("marius_adamw_check"), _entry("marius_adamw_step"), _entry("marius_adamw_workspace_bytes"), tensors, grads, step, lr, beta1, beta2, eps, weight_decay,
+    _ops().adamw_step(_entry("marius_adamw_step"), _entry("marius_adamw_workspace_bytes"), tensors, grads, step, lr, beta1, beta2, eps, weight_decay,
                       grad_scale, torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing())
 
 
