@@ -521,6 +521,8 @@ def node_classification_step(encoder, features, dense_graph, labels, lr, reducti
     """Model::train_batch, NODE_CLASSIFICATION branch (src/cpp/src/nn/model.cpp:317-328): y_pred for the batch's target nodes, CrossEntropyLoss
     (src/cpp/src/nn/loss.cpp:88-102), backward, the dense Adagrad step of every layer parameter (marius_dense_adagrad_step: optim.cpp:114-145;
     the sums live in `.adagrad_sum` of the parameters), or optimizer.step() where one is given (marius_amd.optim.AdamW; lr is its own then).  Returns (loss, y_pred)."""
+    if optimizer is None and any(p.dtype != torch.float32 for p in encoder.parameters()):
+        raise H.MariusHipError("node_classification_step: the Adagrad step needs float32 parameters")
     for p in encoder.parameters():
         p.grad = None
     y = encoder(features, dense_graph, True)

@@ -277,6 +277,8 @@ def adagrad_rule(grad, state, lr, eps=1e-10):
 
 def dense_adagrad_step(param, state_sum, grad, lr, eps=1e-10, weight_decay=0.0):
     _dev(param)
+    if any(t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != param.numel() for t in (param, state_sum, grad)):
+        raise MariusHipError("dense_adagrad_step: parameter, sum and gradient are contiguous float32 tensors of one size")
     check(lib().marius_dense_adagrad_step(ptr(param), ptr(state_sum), ptr(grad), param.numel(), lr, eps, weight_decay, stream_ptr()),
           "dense_adagrad_step")
 

@@ -156,3 +156,19 @@ def test_residual_norm_module_refuses_gates_it_would_leave_out(HE, G):
     refused(HE, "gate is one of", G.GraphAttentionEncoder, 4, 8, 2, 1, 2, gate=None, device=CPU)
     for gate in ("NONE", "CHANNEL", "ELEMENT"):
         refused(HE, "without a block", G.ResidualNorm(4, gate=gate, device=CPU), torch.zeros(2, 4), None, torch.zeros(2, 4))
+
+
+def test_adagrad_refuses_parameters_that_are_not_float32(HE, G):
+    """an encoder in bfloat16 goes forward and back, but the Adagrad step reads and writes four bytes an element"""
+    import test_gpu_encoder_block as B
+
+    graph = B.sampled(G, CPU, 50, 400, [4], True, True, 6, 1)
+    enc = G.GraphAttentionEncoder(6, 8, 3, 1, 4, device=CPU).bfloat16()
+    x, labels = torch.randn(graph.node_ids_.numel(), 6).bfloat16(), torch.zeros(6, dtype=torch.int64)
+    refused(HE, "float32", G.node_classification_step, enc, x, graph, labels, 0.1)
+    assert all(p.grad is None for p in enc.parameters())                       # before the pass
+    w, s = torch.ones(8), torch.ones(8)
+    for bad in ((w.bfloat16(), s, w), (w, s.half(), w), (w, s, w.double()), (w, s[:4], w), (w, s, torch.ones(16)[::2]), (torch.ones(16)[::2], s, w)):
+        refused(HE, "float32", HE.dense_adagrad_step, *bad, 0.1)
+    HE.dense_adagrad_step(w, s, torch.ones(8), 0.1)
+    assert bool((w < 1).all())
