@@ -597,7 +597,7 @@ int marius_residual_norm_backward(const marius_residual_norm* desc, const marius
 
 /* Neighbour lists in both directions, made once for a sampled batch or a graph and used by every pass over it (nbr_plan.hip).
  * marius_nbr_plan_lists: the list of target i is its part of list a (entries offsets_a[i] .. offsets_a[i + 1), the last one ends at T_a), then of list b (T_b = 0:
- *   none; offsets of a list without entries are NULL or zeros), then its own row self_offset + i (self_offset < 0: none).  T = T_a + T_b (+ n).  Out: offsets [n + 1], index / owner [T] (row and target of every
+ *   none; the offsets of a list without entries are not read), then its own row self_offset + i (self_offset < 0: none).  T = T_a + T_b (+ n).  Out: offsets [n + 1], index / owner [T] (row and target of every
  *   entry), keys [T] (the rows once more, for marius_sort_unique), status [4] (ZEROED by the caller): bit 0: offsets that do not ascend from 0 and cover
  *   their list, bit 1: a row outside [0, rows).  A caller reads status before it goes on: the calls below and the attention take the lists as they are.
  * marius_nbr_plan_reverse: the entries grouped by row, in list order: r_offsets [rows + 1], r_owner [T]; perm of marius_sort_unique = r_entry.

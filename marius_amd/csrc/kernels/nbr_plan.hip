@@ -321,7 +321,7 @@ extern "C" int marius_nbr_plan_lists(const int64_t* index_a, const int64_t* offs
     MARIUS_REQUIRE(workspace && workspace_bytes >= marius_nbr_plan_workspace_bytes(n), "nbr_plan_lists: workspace too small");
     hipStream_t st = as_stream(stream);
     NpSource S{};
-    S.lists = NpLists{index_a, offsets_a, index_b, offsets_b, T_a, T_b, n, rows, self_offset};
+    S.lists = NpLists{index_a, T_a > 0 ? offsets_a : nullptr, index_b, T_b > 0 ? offsets_b : nullptr, T_a, T_b, n, rows, self_offset};
     S.n = n;
     S.status = status;
     NpOut O{};

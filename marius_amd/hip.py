@@ -788,6 +788,8 @@ class NeighborPlan:
         _require(all(t.dtype == torch.int64 and t.dim() == 1 for t in lists), "NeighborPlan: index and offsets are int64 vectors")
         dev, n, ta, tb = index.device, offsets.numel(), index.numel(), 0 if index_b is None else index_b.numel()
         _require(offsets_b is None or offsets_b.numel() == n, "NeighborPlan: the lists differ in their number of targets")
+        for t, o in ((ta, offsets), (tb, offsets_b)):  # (the library does not look at the offsets of a list that has no entries)
+            _require(t > 0 or o is None or not bool(o.any()), "NeighborPlan: offsets have to ascend from 0 to the end of their list")
         own = -1 if self_offset is None else int(self_offset)
         _require(self_offset is None or 0 <= own <= num_rows - n, "NeighborPlan: a target's own row lies outside the rows")
         total = ta + tb + (n if own >= 0 else 0)
