@@ -13,7 +13,7 @@
 // Bound by HBM: 28 bytes an element with fp32 states, 16.1 with 8-bit ones (fp32 parameters and gradients).  A workgroup takes tiles of 2048 elements, eight
 // per lane (16-byte loads of every stream; the 32 lanes of a block share its scale by shuffles), and finds its tensor by binary search: up to 64 tensors in
 // the launch's own arguments, more in a table that short launches copy from theirs into the workspace of this call (300 tensors, 20 M elements in 8 bits: 56 us
-// against 86 with a launch for every 64 tensors, each of which fills and drains the card anew; 200 M elements in fp32: 1095 us, 5.1 TB/s).
+// against 86 with a launch for every 64 tensors, each of which fills and drains the card anew; 200 M elements in fp32: 1072 us, 5.2 TB/s).
 // With the step's number on the device one lane of a workgroup takes the two factors behind the loads: the times are those of a number on the host (in every lane, the 300
 // tensors in 8 bits took 7 us more).
 #include "row_types.h"

@@ -15,10 +15,12 @@
 //     dw = sum over rows of (gradient of the norm's output) times (normalised row),   db = sum over rows of that gradient
 //
 // Bound by HBM: every element is read once and written once, about ten operations each (forward, 100,000 rows of 512, fp32 stream and bf16 block: 124 us, 4.9 TB/s;
-// back, 160,000 rows of 100 in fp32: 82 us, 4.7 TB/s).  A row lives in registers, four elements a lane: in 1 to 64 lanes of one wave
+// back, 160,000 rows of 100 in fp32: 82 us, 4.7 TB/s).  A row lives in registers up to 4096 elements, four elements a lane: in 1 to 64 lanes of one wave
 // (several rows per wave where they are short) or, longer than 256 elements, in a workgroup, so the statistics cost lane moves (and a barrier), not passes over memory.
 // Four elements, not eight, for the 16-bit types too: the backward pass holds five rows and five sums a lane, and with eight elements one wave per SIMD was
-// left (50,000 rows of 1024 in bf16: 579 us, against 190 us now).
+// left (50,000 rows of 1024 in bf16: 579 us, against 190 us now).  Rows of 4097 to 8192 elements hold 16 a lane: forward 50,000 rows of 8192 in bf16 639 us (5.1 TB/s), but back
+// some registers go to scratch, most of them with a channel gate: 969 us (5.1 TB/s) without a gate, 1245 (5.3) with one for each element, 1519 (3.2) with one for each channel.
+// A row whose squares leave fp32 (elements above 1.8e19) is normalised to zeros.
 // Sums over rows are deterministic: a workgroup adds its rows in order in registers, its lanes in a fixed order in LDS, and a second launch adds the
 // workgroups' partials in order.  Statistics, sums and the residual are fp32; y and h are rounded once each, at their stores (h comes from the unrounded y).
 #include "row_types.h"
@@ -38,7 +40,7 @@ struct NormArgs {
 };
 enum { SUM_POST_W = 0, SUM_POST_B, SUM_PRE_W, SUM_PRE_B, SUM_GATE, SUMS };
 
-// (sigmoid: the hardware's exponential and reciprocal, a step of fp32 or two together)
+// (sigmoid: the hardware's exponential and reciprocal: a step of fp32 or two, and |v| more from the exponential's rounded argument where it counts)
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 // sigmoid(v) -> v, its slope: t / (1 + t)^2 of t = exp(-|v|), because a (1 - a) of a rounded a cancels where the gate is almost open (0.9 % off at v = 12, zero from 17 on)
 __device__ __forceinline__ float sigmoid_slope(float& v) {
@@ -52,7 +54,7 @@ __device__ __forceinline__ float gate_slope(float g, int act) {
     return act == MARIUS_ACT_SIGMOID ? sigmoid_slope(g) : 1.f;
 }
 
-// 1 / sqrt(v) within a step of fp32; the instruction takes no subnormal numbers, which an eps of zero and rows below 1e-19 leave
+// 1 / sqrt(v) within a step of fp32 (a rounded root and quotient would cost more than they give: a gradient's fp32 error is 2.2e-7 against 2.0e-7); the instruction takes no subnormal numbers, which an eps of zero and rows below 1e-19 leave
 __device__ __forceinline__ float inverse_root(float v) {
     const bool tiny = v < 0x1p-96f;
     return __builtin_amdgcn_rsqf(tiny ? v * 0x1p96f : v) * (tiny ? 0x1p48f : 1.f);
@@ -374,7 +376,9 @@ __global__ __launch_bounds__(1024) void residual_norm_sums_kernel(NormSumArgs A)
     }
 }
 
-// a row of up to 64 pieces of four elements stays in one wave, a longer one takes a workgroup of as many waves as hold it (four pieces a lane beyond 4096 elements)
+// A row of up to 64 pieces of four elements stays in one wave, several of them side by side where they are short (160,000 rows of 100 back: 82 us, a workgroup for each 268); a
+// longer one takes a workgroup of as many waves as hold it, and beyond 4096 elements four pieces a lane.  (Two pieces in twice the lanes: 50,000 rows of 8192 in bf16 back
+// 1040 us against 969, with a channel gate 1429 against 1519; 40,000 of 5000 forward 319 against 385, back 696 against 664.)
 struct NormShape {
     int vec, tpr, nch, threads;
     bool blk;
