@@ -657,7 +657,7 @@ int marius_bin_sum(const float* values, const int64_t* bin, int64_t T, int32_t h
  * or, on the device, step_dev[0] for all tensors (step_count 1) or step_dev[k] for tensor k (step_count = count); a captured call replays with the steps it finds there.  Every gradient is multiplied by *grad_scale (NULL: 1).  All tensors of a call have
  * parameters of param_type and gradients of grad_type; more than 64 of them go through a table in `workspace` (marius_adamw_workspace_bytes(count) bytes, 0 up to 64).  state_bits 32: exp_avg / exp_avg_sq fp32 [n].  state_bits 8: e4m3 codes [n] and one
  * fp32 scale for every 256 elements [ceil(n / 256)]; exp_avg_sq then holds the ROOT of the second moment (value = code * scale in both), and a root above zero stays
- * above zero. */
+ * above zero.  A gradient that is not finite spoils its element; with states in 8 bits an infinity spoils its block of 256, whose scale it is. */
 typedef struct marius_adamw_tensor {
     void* param;
     const void* grad;

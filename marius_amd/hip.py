@@ -922,7 +922,8 @@ def adamw_step(tensors, grads, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, 
     """One AdamW step over all tensors of an AdamWTensors (marius_adamw_step), in place.  grads: one per parameter, of one type; None leaves its parameter and states as
     they are.  step counts from 1: a number, or an int64 device tensor of one element or of one for each parameter (a captured call has to take that: a replay reads it
     anew).  Moments that were never updated belong to step 1, whatever the other parameters have taken: their bias correction is their own.  grad_scale: float32
-    device tensor of one element every gradient is multiplied by (a clipping factor, the inverse of a loss scale)."""
+    device tensor of one element every gradient is multiplied by (a clipping factor, the inverse of a loss scale).  A gradient that is not finite spoils its element (an
+    infinity, with states in 8 bits, its block of 256): a program that scales its loss looks for them before the step."""
     _require(isinstance(tensors, _ops().AdamWTensors), "adamw_step: AdamWTensors are needed")
     _ops().adamw_step(_entry("marius_adamw_step"), _entry("marius_adamw_workspace_bytes"), tensors, grads, step, lr, beta1, beta2, eps, weight_decay,
                       grad_scale, torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing())

@@ -87,6 +87,11 @@ def test_emulated_gradients_that_are_not_contiguous(HE, bits):
     T.test_gradients_that_are_not_contiguous(HE, CPU, bits)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_emulated_gradients_that_are_not_finite(HE, bits):
+    T.test_gradients_that_are_not_finite_spoil_no_more_than_they_have_to(HE, CPU, bits)
+
+
 def test_adamw_check_refuses_and_does_nothing(HE):
     p, m, v = (torch.ones(300) for _ in range(3))
     t = HE.AdamWTensors([p], [m], [v])

@@ -406,3 +406,24 @@ def test_states_given_new_memory(H, dev):
             H.adamw_step(two, hs, 3)
         t.data = kept
     H.adamw_step(two, hs, 3)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_that_are_not_finite_spoil_no_more_than_they_have_to(H, dev, bits):
+    """a NaN its element, an infinity its element or, as the scale of an 8-bit block, its block; every other element of the tensor and the tensors beside it are those of a step
+    without them"""
+    runs = []
+    for spoilt in (False, True):
+        ps, gs, ms, vs, sm, sv = T.adamw_case(H, dev, [1000, 300], F32, F32, bits, 2)
+        if spoilt:
+            gs[0][10], gs[0][600] = math.nan, math.inf
+        tensors = H.AdamWTensors(ps, ms, vs, sm, sv)
+        for step in (1, 2):
+            H.adamw_step(tensors, gs, step)
+        runs.append(ps)
+    bad = torch.zeros(1000, dtype=torch.bool)
+    bad[10], bad[600] = True, True
+    if bits == 8:
+        bad[512:768] = True
+    got, want = runs[1][0].cpu(), runs[0][0].cpu()
+    assert bool((got[bad] != want[bad]).all()) and not bool(got[bad].isfinite().any()) and torch.equal(got[~bad], want[~bad]) and torch.equal(runs[1][1], runs[0][1])
